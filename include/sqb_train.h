@@ -85,6 +85,113 @@ int sqb_add_layernorm_bwd(const void* dy, int dy_dtype, const float* x_out, cons
                           void* dh_bf16, float* dweight, float* dbias, void* workspace,
                           size_t ws_bytes, int64_t N, int64_t C, void* stream);
 
+/* ---- Token log-probabilities and the losses on them -------------------------
+ * logits are an (S, T, V) view, unit stride on V, element strides ss (sequence)
+ * and st (token), any alignment of the element's size; row r is sequence r / T,
+ * token r % T (a packed batch: S = 1, T = all rows).  targets (S * T) are int64; a
+ * negative one leaves its row out: the row is not read, its log-probability is 0
+ * and its gradient row zero.  One of V or more gives NaN.  S * T < 2^31. */
+
+/* Per row: logp = log softmax(logits)[target] as fp32 and/or in 64 bits (either
+ * pointer may be NULL), and stats = (max, sum of exp(x - max)), fp32 (S * T, 2),
+ * 8-byte aligned (a row left out: (0, 1)). */
+int sqb_logp_fwd(const void* logits, const int64_t* targets, float* logp, double* logp_double,
+                 float* stats, int64_t S, int64_t T, int64_t V, int64_t ss, int64_t st, int dtype,
+                 void* stream);
+
+/* dlogits[r, c] = g_row[r] * scale[0] * ([c == target] - softmax(logits)[r, c]) in the
+ * logits' dtype, strides dss and dst; scale (one fp32 on the device) may be NULL.  Rows
+ * whose 16-byte phase is the logits' are written with vector stores. */
+int sqb_logp_bwd(const void* logits, const int64_t* targets, const float* stats,
+                 const float* g_row, const float* scale, void* dlogits, int64_t S, int64_t T,
+                 int64_t V, int64_t ss, int64_t st, int64_t dss, int64_t dst, int dtype,
+                 void* stream);
+
+/* Preference loss over P pairs from the rows' log-probabilities in 64 bits (0 where
+ * left out): sequence p < P is chosen, P + p its rejected one.  Sequence s has rows
+ * [cu_seqlens[s], cu_seqlens[s + 1]) (2P + 1 entries, held inside [0, N]), or with
+ * cu_seqlens NULL rows [s * T, (s + 1) * T), N = 2P * T.  With r = sum of logp -
+ * ref_logps[s] (fp32, NULL: 0) and z = beta * (r_chosen - r_rejected):
+ *   loss = mean of -(1 - label_smoothing) log sigmoid(z) - label_smoothing log sigmoid(-z),
+ *   rewards (2P, fp32) = beta * r,   g_row (N, fp32) = d loss / d logp
+ * (rows of no sequence are not written).  pair_loss: P doubles of scratch. */
+int sqb_preference_finish(const double* logp, const int64_t* cu_seqlens, const float* ref_logps,
+                          int64_t P, int64_t T, int64_t N, double beta, double label_smoothing,
+                          double* pair_loss, float* loss, float* rewards, float* g_row,
+                          void* stream);
+
+/* Weight (fp32, N) of every row in the policy loss: 1 / counted rows, or with
+ * per_sequence 1 / (counted rows of its sequence * sequences that have any); 0 for a
+ * row left out by its target or by cu_seqlens.  counts: S int32 of scratch.  row_seq
+ * (int32, N; needed with cu_seqlens): the row's sequence, -1 for none. */
+int sqb_policy_weights(const int64_t* targets, const int64_t* cu_seqlens, int64_t S, int64_t T,
+                       int64_t N, int per_sequence, int32_t* counts, float* weight,
+                       int32_t* row_seq, void* stream);
+
+/* Per row of weight w != 0, with r = exp(logp - old_logp) (1 for NULL), A = adv[row]
+ * (adv_by_seq: of its sequence, row_seq's or row / T) and ref_logp (NULL: no KL):
+ *   terms = (-min(r A, held(r) A), exp(ref - logp) - (ref - logp) - 1, [clipped]), held
+ *   keeping r in [1 - clip_low, 1 + clip_high]; (3, N) in 64 bits
+ *   g_row = w * d(terms[0] + kl_coef * terms[1]) / d logp
+ * and logp, stats as sqb_logp_fwd (each may be NULL, as g_row).  With dlogits, also the
+ * gradient as sqb_logp_bwd with factor g_row * grad_scale, in the same pass.  Rows of
+ * weight 0 get zeros. */
+int sqb_policy_rows(const void* logits, const int64_t* targets, const float* old_logp,
+                    const float* ref_logp, const float* adv, int adv_by_seq,
+                    const int32_t* row_seq, const float* weight, double clip_low,
+                    double clip_high, double kl_coef, float* logp, float* stats, float* g_row,
+                    double* terms, void* dlogits, float grad_scale, int64_t S, int64_t T,
+                    int64_t V, int64_t ss, int64_t st, int64_t dss, int64_t dst, int dtype,
+                    void* stream);
+
+/* loss = sum of weight * (terms[0] + kl_coef * terms[1]); stats (3) = the weighted sums of
+ * the terms, in a fixed order. */
+int sqb_policy_finish(const double* terms, const float* weight, int64_t N, double kl_coef,
+                      float* loss, float* stats, void* stream);
+
+/* ---- Global gradient norm and clipping ---------------------------------------
+ * n tensors as host arrays of device pointers (element-aligned), element counts (each
+ * at most 2^34, 0 allowed) and dtypes; the arrays are read before the call returns.
+ * norm: one fp32 on the device, sqrt of the sum of squares, summed in 64 bits in a
+ * fixed order. */
+size_t sqb_grad_norm_workspace_bytes(int64_t n_tensors);
+int sqb_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtypes,
+                  int64_t n, void* workspace, size_t ws_bytes, float* norm, void* stream);
+
+/* outs[i] = grads[i] * min(1, max_norm / (norm + 1e-6)) in out_dtypes[i], the factor and
+ * the product in fp32.  outs[i] is grads[i] (same dtype) or memory apart from every
+ * gradient; where all are in place and the factor is 1 nothing is written. */
+int sqb_grad_clip(const void* const* grads, void* const* outs, const int64_t* numel,
+                  const int32_t* dtypes, const int32_t* out_dtypes, int64_t n, float max_norm,
+                  void* workspace, size_t ws_bytes, float* norm, void* stream);
+
+/* ---- Residual step between two norms -----------------------------------------
+ * On N contiguous rows of C <= 4096 (else SQB_ERR_UNSUPPORTED), x and h each fp32 or bf16:
+ *   n = Norm(h; post_weight, post_bias)   (h itself for a NULL post_weight)
+ *   x_out = x + scale * gate * n          (x's dtype; a NULL gate is ones)
+ *   y = Norm(x_out; weight, bias)         (y_dtype; of x_out before its rounding)
+ * Norm: LayerNorm, or with `rms` an RMS norm; biases may be NULL.  gate: (gates, C), each
+ * row shared by N / gates rows in turn.  Parameters are fp32.  stats: fp32 (N, 4), the
+ * mean and 1/std of h and of x_out, 16-byte aligned. */
+int sqb_residual_norm_fwd(const void* x, int x_dtype, const void* h, int h_dtype,
+                          const float* weight, const float* bias, const float* post_weight,
+                          const float* post_bias, const float* gate, int64_t gates, float scale,
+                          float eps, int rms, void* x_out, void* y, int y_dtype, float* stats,
+                          int64_t N, int64_t C, void* stream);
+
+size_t sqb_residual_norm_workspace_bytes(int64_t N, int64_t C, int64_t gates);
+
+/* Backward from x, h and the forward's stats: dy (y_dtype), dx_out (x's dtype; NULL: 0)
+ * -> dx, dh in x's and h's dtypes and the gradient of every parameter given (fp32,
+ * overwritten; dgate (gates, C)), summed in a fixed order.  At most 65531 gates. */
+int sqb_residual_norm_bwd(const void* dy, int y_dtype, const void* dx_out, const void* x,
+                          int x_dtype, const void* h, int h_dtype, const float* weight,
+                          const float* bias, const float* post_weight, const float* post_bias,
+                          const float* gate, int64_t gates, float scale, float eps, int rms,
+                          const float* stats, void* dx, void* dh, float* dweight, float* dbias,
+                          float* dpost_weight, float* dpost_bias, float* dgate, void* workspace,
+                          size_t ws_bytes, int64_t N, int64_t C, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

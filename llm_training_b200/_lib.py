@@ -7,9 +7,12 @@ raises, and every op that needs it fails with that error.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
+
+import torch
 
 from .build import LIBPATH
 
@@ -86,7 +89,39 @@ TRAIN_SIGNATURES = {
     "sqb_add_layernorm_bwd": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int] +
                               [ctypes.c_void_p] * 10 +
                               [ctypes.c_size_t, _c_i64, _c_i64, ctypes.c_void_p]),
+    # token log-probabilities and the losses on them
+    "sqb_logp_fwd": (ctypes.c_int, [_vp] * 5 + [_c_i64] * 5 + [ctypes.c_int, _vp]),
+    "sqb_logp_bwd": (ctypes.c_int, [_vp] * 6 + [_c_i64] * 7 + [ctypes.c_int, _vp]),
+    "sqb_preference_finish": (ctypes.c_int, [_vp] * 3 + [_c_i64] * 3 + [ctypes.c_double] * 2 +
+                              [_vp] * 5),
+    "sqb_policy_weights": (ctypes.c_int, [_vp] * 2 + [_c_i64] * 3 + [ctypes.c_int] + [_vp] * 4),
+    "sqb_policy_rows": (ctypes.c_int, [_vp] * 5 + [ctypes.c_int] + [_vp] * 2 +
+                        [ctypes.c_double] * 3 + [_vp] * 5 + [ctypes.c_float] + [_c_i64] * 7 +
+                        [ctypes.c_int, _vp]),
+    "sqb_policy_finish": (ctypes.c_int, [_vp] * 2 + [_c_i64, ctypes.c_double] + [_vp] * 3),
+    # gradient norm and clipping
+    "sqb_grad_norm_workspace_bytes": (ctypes.c_size_t, [_c_i64]),
+    "sqb_grad_norm": (ctypes.c_int, [_vp] * 3 + [_c_i64, _vp, ctypes.c_size_t, _vp, _vp]),
+    "sqb_grad_clip": (ctypes.c_int, [_vp] * 5 + [_c_i64, ctypes.c_float, _vp, ctypes.c_size_t,
+                                                 _vp, _vp]),
+    # the residual step between two norms
+    "sqb_residual_norm_fwd": (ctypes.c_int, [_vp, ctypes.c_int] * 2 + [_vp] * 5 +
+                              [_c_i64, ctypes.c_float, ctypes.c_float, ctypes.c_int] +
+                              [_vp] * 2 + [ctypes.c_int, _vp, _c_i64, _c_i64, _vp]),
+    "sqb_residual_norm_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 3),
+    "sqb_residual_norm_bwd": (ctypes.c_int, [_vp, ctypes.c_int, _vp] + [_vp, ctypes.c_int] * 2 +
+                              [_vp] * 5 +
+                              [_c_i64, ctypes.c_float, ctypes.c_float, ctypes.c_int] +
+                              [_vp] * 9 + [ctypes.c_size_t, _c_i64, _c_i64, _vp]),
 }
+
+
+def on_device(device):
+    """Context in which `device` is the current one: a launch goes to the current device,
+    whatever its stream's."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def library_path() -> str:

@@ -1,0 +1,290 @@
+// Global gradient norm over many tensors, and clipping (include/sqb_train.h).
+//
+//   norm = sqrt(sum of g^2 over every tensor),  out = g * min(1, max_norm / (norm + 1e-6))
+//
+// The squares are summed in 64 bits: a square of an fp32 gradient overflows or
+// vanishes in 32 bits from 1e19 up and 1e-19 down, and the B200's 64-bit units keep
+// up with HBM (two operations for each 4 bytes).  One CTA's sum is written to its own
+// slot and the slots are added in a fixed order, so the norm is the same bits on
+// every run and on every data-parallel rank that holds the same gradients.
+//
+// The tensors' pointers and sizes travel as a kernel argument (no table in device
+// memory to fill, and a captured graph keeps its own copy).  The work is cut into
+// chunks that never cross a tensor; CTAs take chunks round-robin and find a chunk's
+// tensor by a binary search in the table.  Bound by HBM: one read for the norm, one
+// read and one write for the scaling.
+
+#include <cuda_bf16.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "sqb_train.h"
+
+namespace sqb {
+namespace gradclip {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kGrid = 148 * 4;  // 4 CTAs of 512 threads on each of 148 SMs
+constexpr int kMaxTensors = 768;
+constexpr int64_t kChunk = 16384;  // elements
+
+struct Table {
+  const void* in[kMaxTensors];
+  void* out[kMaxTensors];
+  int64_t numel[kMaxTensors];
+  int32_t end[kMaxTensors];  // chunks of tensors 0..i
+  uint8_t in_bf16[kMaxTensors], out_bf16[kMaxTensors];
+  int32_t n;
+};
+static_assert(sizeof(Table) <= 32000, "a kernel's arguments are at most 32764 bytes");
+
+__device__ __forceinline__ int tensor_of(const Table& t, int chunk) {
+  int lo = 0, hi = t.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (t.end[mid] <= chunk)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+__device__ double block_sum(double v, double* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __syncthreads();  // red may still be read by a previous reduction
+  if (lane == 0) red[warp] = v;
+  __syncthreads();
+  v = lane < (int)blockDim.x / 32 ? red[lane] : 0.0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T>
+__device__ double square_sum(const T* p, int64_t n) {
+  constexpr int kN = 16 / sizeof(T);
+  int64_t head = ((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T);
+  head = head < n ? head : n;
+  const int64_t nvec = (n - head) / kN;
+  double v = 0.0;
+  auto one = [&](float x) { v = fma((double)x, (double)x, v); };
+  if (threadIdx.x < head) one(to_f(p[threadIdx.x]));
+  for (int64_t i = threadIdx.x; i < nvec; i += kThreads) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p + head + i * kN);
+    const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int j = 0; j < kN; ++j) one(to_f(e[j]));
+  }
+  const int64_t tail = head + nvec * kN + threadIdx.x;
+  if (tail < n) one(to_f(p[tail]));
+  return v;
+}
+
+__global__ void __launch_bounds__(kThreads)
+    norm_kernel(const __grid_constant__ Table t, double* partial) {
+  __shared__ double red[32];
+  const int chunks = t.end[t.n - 1];
+  double v = 0.0;
+  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+    const int i = tensor_of(t, c);
+    const int64_t at = (int64_t)(c - (i ? t.end[i - 1] : 0)) * kChunk;
+    const int64_t n = min(kChunk, t.numel[i] - at);
+    v += t.in_bf16[i] ? square_sum(static_cast<const __nv_bfloat16*>(t.in[i]) + at, n)
+                      : square_sum(static_cast<const float*>(t.in[i]) + at, n);
+  }
+  v = block_sum(v, red);
+  if (threadIdx.x == 0) partial[blockIdx.x] = v;
+}
+
+// The norm from the CTAs' sums, the same in every thread of every CTA.
+__device__ float norm_of(const double* partial, int slots, double* red) {
+  double v = 0.0;
+  for (int i = threadIdx.x; i < slots; i += blockDim.x) v += partial[i];
+  return (float)sqrt(block_sum(v, red));
+}
+
+__global__ void __launch_bounds__(kThreads)
+    finish_kernel(const double* partial, int slots, float* norm) {
+  __shared__ double red[32];
+  const float n = norm_of(partial, slots, red);
+  if (threadIdx.x == 0) *norm = n;
+}
+
+template <typename I, typename O>
+__device__ void scale_chunk(const I* p, O* o, int64_t n, float f) {
+  constexpr int kN = 16 / sizeof(I);
+  constexpr uintptr_t kOut = kN * sizeof(O) < 16 ? kN * sizeof(O) : 16;  // a store's alignment
+  int64_t head = ((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(I);
+  head = head < n ? head : n;
+  if ((reinterpret_cast<uintptr_t>(o + head) & (kOut - 1)) != 0) {
+    for (int64_t i = threadIdx.x; i < n; i += kThreads) put(o + i, to_f(p[i]) * f);
+    return;
+  }
+  const int64_t nvec = (n - head) / kN;
+  if (threadIdx.x < head) put(o + threadIdx.x, to_f(p[threadIdx.x]) * f);
+  for (int64_t i = threadIdx.x; i < nvec; i += kThreads) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p + head + i * kN);
+    const I* e = reinterpret_cast<const I*>(&u);
+    O* q = o + head + i * kN;
+    alignas(16) O d[kN];
+#pragma unroll
+    for (int j = 0; j < kN; ++j) put(d + j, to_f(e[j]) * f);
+    if constexpr (kN * sizeof(O) == 8) {
+      *reinterpret_cast<uint2*>(q) = *reinterpret_cast<const uint2*>(d);
+    } else {
+#pragma unroll
+      for (int j = 0; j < (int)(kN * sizeof(O) / 16); ++j)
+        reinterpret_cast<uint4*>(q)[j] = reinterpret_cast<const uint4*>(d)[j];
+    }
+  }
+  const int64_t tail = head + nvec * kN + threadIdx.x;
+  if (tail < n) put(o + tail, to_f(p[tail]) * f);
+}
+
+__global__ void __launch_bounds__(kThreads)
+    clip_kernel(const __grid_constant__ Table t, const double* partial, int slots,
+                float max_norm, bool in_place, float* norm) {
+  __shared__ double red[32];
+  const float n = norm_of(partial, slots, red);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm = n;
+  float f = max_norm / (n + 1e-6f);
+  if (f > 1.f) f = 1.f;  // a NaN stays
+  if (in_place && f == 1.f) return;
+  const int chunks = t.end[t.n - 1];
+  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+    const int i = tensor_of(t, c);
+    const int64_t at = (int64_t)(c - (i ? t.end[i - 1] : 0)) * kChunk;
+    const int64_t k = min(kChunk, t.numel[i] - at);
+    const float* pf = static_cast<const float*>(t.in[i]) + at;
+    const __nv_bfloat16* pb = static_cast<const __nv_bfloat16*>(t.in[i]) + at;
+    float* of = static_cast<float*>(t.out[i]) + at;
+    __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(t.out[i]) + at;
+    if (t.in_bf16[i]) {
+      if (t.out_bf16[i])
+        scale_chunk(pb, ob, k, f);
+      else
+        scale_chunk(pb, of, k, f);
+    } else {
+      if (t.out_bf16[i])
+        scale_chunk(pf, ob, k, f);
+      else
+        scale_chunk(pf, of, k, f);
+    }
+  }
+}
+
+// Fills `t` from the next tensors at `at`; returns how many were passed.  Empty
+// tensors take no slot.
+int64_t fill(Table& t, const void* const* in, void* const* out, const int64_t* numel,
+             const int32_t* in_dtype, const int32_t* out_dtype, int64_t n, int64_t at) {
+  t.n = 0;
+  int32_t chunks = 0;
+  int64_t i = at;
+  for (; i < n && t.n < kMaxTensors; ++i) {
+    if (numel[i] == 0) continue;
+    chunks += (int32_t)((numel[i] + kChunk - 1) / kChunk);
+    t.in[t.n] = in[i];
+    t.out[t.n] = out ? out[i] : nullptr;
+    t.numel[t.n] = numel[i];
+    t.end[t.n] = chunks;
+    t.in_bf16[t.n] = in_dtype[i] == SQB_BF16;
+    t.out_bf16[t.n] = out_dtype && out_dtype[i] == SQB_BF16;
+    ++t.n;
+  }
+  return i - at;
+}
+
+// 768 tensors of this many elements are fewer than 2^31 chunks
+constexpr int64_t kMaxNumel = (int64_t)1 << 34;
+
+bool known(int32_t dtype) { return dtype == SQB_BF16 || dtype == SQB_F32; }
+
+int check(const void* const* in, void* const* out, const int64_t* numel,
+          const int32_t* in_dtype, const int32_t* out_dtype, int64_t n) {
+  for (int64_t i = 0; i < n; ++i) {
+    if (numel[i] < 0 || numel[i] > kMaxNumel) return SQB_ERR_ARG;
+    if (!known(in_dtype[i]) || (out_dtype && !known(out_dtype[i]))) return SQB_ERR_DTYPE;
+    if (numel[i] && (!in[i] || (out && !out[i]))) return SQB_ERR_ARG;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(in[i]);
+    const uintptr_t b = out ? reinterpret_cast<uintptr_t>(out[i]) : 0;
+    if (a % (in_dtype[i] == SQB_BF16 ? 2 : 4)) return SQB_ERR_ALIGN;
+    if (out && b % (out_dtype[i] == SQB_BF16 ? 2 : 4)) return SQB_ERR_ALIGN;
+  }
+  return SQB_OK;
+}
+
+int grid_of(const Table& t) { return t.end[t.n - 1] < kGrid ? t.end[t.n - 1] : kGrid; }
+
+// One launch for each table of tensors; returns the slots of `partial` they write.
+int launch_norms(Table& t, const void* const* in, const int64_t* numel, const int32_t* in_dtype,
+                 int64_t n, double* partial, cudaStream_t q) {
+  int slots = 0;
+  for (int64_t at = 0; at < n;) {
+    at += fill(t, in, nullptr, numel, in_dtype, nullptr, n, at);
+    if (t.n == 0) continue;
+    norm_kernel<<<grid_of(t), kThreads, 0, q>>>(t, partial + slots);
+    slots += grid_of(t);
+  }
+  return slots;
+}
+
+int launched() { return cudaGetLastError() == cudaSuccess ? SQB_OK : SQB_ERR_LAUNCH; }
+
+}  // namespace
+}  // namespace gradclip
+}  // namespace sqb
+
+using namespace sqb::gradclip;
+
+extern "C" size_t sqb_grad_norm_workspace_bytes(int64_t n_tensors) {
+  if (n_tensors <= 0) return 0;
+  return (size_t)((n_tensors + kMaxTensors - 1) / kMaxTensors) * kGrid * sizeof(double);
+}
+
+extern "C" int sqb_grad_norm(const void* const* grads, const int64_t* numel,
+                             const int32_t* dtypes, int64_t n, void* workspace, size_t ws_bytes,
+                             float* norm, void* stream) {
+  if (!grads || !numel || !dtypes || n <= 0 || !norm) return SQB_ERR_ARG;
+  if (const int rc = check(grads, nullptr, numel, dtypes, nullptr, n)) return rc;
+  if (!workspace || ws_bytes < sqb_grad_norm_workspace_bytes(n)) return SQB_ERR_WORKSPACE;
+  cudaStream_t q = static_cast<cudaStream_t>(stream);
+  double* partial = static_cast<double*>(workspace);
+  Table t;
+  const int slots = launch_norms(t, grads, numel, dtypes, n, partial, q);
+  finish_kernel<<<1, kThreads, 0, q>>>(partial, slots, norm);
+  return launched();
+}
+
+extern "C" int sqb_grad_clip(const void* const* grads, void* const* outs, const int64_t* numel,
+                             const int32_t* dtypes, const int32_t* out_dtypes, int64_t n,
+                             float max_norm, void* workspace, size_t ws_bytes, float* norm,
+                             void* stream) {
+  if (!grads || !outs || !numel || !dtypes || !out_dtypes || n <= 0 || !norm ||
+      !(max_norm >= 0.f))
+    return SQB_ERR_ARG;
+  if (const int rc = check(grads, outs, numel, dtypes, out_dtypes, n)) return rc;
+  if (!workspace || ws_bytes < sqb_grad_norm_workspace_bytes(n)) return SQB_ERR_WORKSPACE;
+  cudaStream_t q = static_cast<cudaStream_t>(stream);
+  double* partial = static_cast<double*>(workspace);
+  bool in_place = true;
+  for (int64_t i = 0; i < n; ++i)
+    in_place = in_place && (numel[i] == 0 || (grads[i] == outs[i] && dtypes[i] == out_dtypes[i]));
+  Table t;
+  const int slots = launch_norms(t, grads, numel, dtypes, n, partial, q);
+  if (slots == 0) finish_kernel<<<1, kThreads, 0, q>>>(partial, 0, norm);
+  for (int64_t at = 0; at < n;) {
+    at += fill(t, grads, outs, numel, dtypes, out_dtypes, n, at);
+    if (t.n == 0) continue;
+    clip_kernel<<<grid_of(t), kThreads, 0, q>>>(t, partial, slots, max_norm, in_place, norm);
+  }
+  return launched();
+}

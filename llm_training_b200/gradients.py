@@ -1,0 +1,157 @@
+"""Global gradient norm over many tensors, and clipping (csrc/sqb_gradclip.cu)."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+
+__all__ = ["grad_norm", "clip_grads", "clip_grad_norm_"]
+
+_DTYPES = {torch.float32: _lib.SQB_F32, torch.bfloat16: _lib.SQB_BF16}
+
+
+def _dense(t):
+    """Whether t's elements fill one run of memory, in whatever order."""
+    if t.is_contiguous():
+        return True
+    at = 1
+    for stride, size in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if stride != at:
+            return False
+        at *= size
+    return True
+
+
+def _checked(fn, tensors, what="gradients"):
+    """The device of `tensors`, all of them strided CUDA float32 or bfloat16 on it."""
+    device = tensors[0].device
+    for t in tensors:
+        if t.layout != torch.strided:
+            raise ValueError(f"{fn}: {what} must be strided tensors, got layout {t.layout}")
+        if t.dtype not in _DTYPES:
+            raise TypeError(f"{fn} supports float32 and bfloat16, got {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"{fn}: {what} are on {device} and {t.device}: one call takes one "
+                             "device")
+    if device.type != "cuda":
+        raise RuntimeError(f"{fn}: {what} must be CUDA tensors (the op has no CPU "
+                           "implementation)")
+    return device
+
+
+def _tables(tensors):
+    n = len(tensors)
+    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors]),
+            (ctypes.c_int32 * n)(*[_DTYPES[t.dtype] for t in tensors]))
+
+
+def _numels(tensors):
+    return (ctypes.c_int64 * len(tensors))(*[t.numel() for t in tensors])
+
+
+def _workspace(n, device):
+    nbytes = _lib.lib().sqb_grad_norm_workspace_bytes(n)
+    return torch.empty(nbytes // 8, dtype=torch.float64, device=device), nbytes
+
+
+def grad_norm(tensors):
+    """2-norm of all elements of ``tensors`` (CUDA float32 or bfloat16, any mixture, one
+    device) as a float32 scalar on their device.  The squares are summed in 64 bits in a
+    fixed order: no overflow, and the same bits on every run.  No tensors: 0."""
+    tensors = list(tensors)
+    if not tensors:
+        return torch.tensor(0.0)
+    device = _checked("grad_norm", tensors, "tensors")
+    tensors = [t if _dense(t) else t.contiguous() for t in tensors]
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    ptrs, dtypes = _tables(tensors)
+    ws, nbytes = _workspace(len(tensors), device)
+    with _lib.on_device(device):
+        _lib.check("sqb_grad_norm", _lib.lib().sqb_grad_norm(
+            ptrs, _numels(tensors), dtypes, len(tensors), ws.data_ptr(), nbytes,
+            norm.data_ptr(), torch.cuda.current_stream(device).cuda_stream))
+    return norm
+
+
+def _clip(grads, outs, max_norm, device):
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    ptrs, dtypes = _tables(grads)
+    out_ptrs, out_dtypes = (ptrs, dtypes) if outs is grads else _tables(outs)
+    ws, nbytes = _workspace(len(grads), device)
+    with _lib.on_device(device):
+        _lib.check("sqb_grad_clip", _lib.lib().sqb_grad_clip(
+            ptrs, out_ptrs, _numels(grads), dtypes, out_dtypes, len(grads), max_norm,
+            ws.data_ptr(), nbytes, norm.data_ptr(),
+            torch.cuda.current_stream(device).cuda_stream))
+    return norm
+
+
+def _bound(fn, max_norm):
+    max_norm = float(max_norm)
+    if math.isnan(max_norm) or max_norm < 0:
+        raise ValueError(f"{fn}: max_norm must not be negative, got {max_norm}")
+    return max_norm
+
+
+def clip_grads(grads, max_norm, out=None):
+    """(out, norm): the ``grads`` (CUDA float32 or bfloat16, any mixture, one device)
+    times min(1, max_norm / (norm + 1e-6)), norm their global 2-norm as ``grad_norm``
+    computes it, written to ``out``: one tensor for each gradient, of its shape, float32
+    or bfloat16 (an optimizer's fp32 buffers for bf16 gradients: the factor is applied
+    before the only rounding), sharing no memory with any gradient unless it is the same
+    tensor.  None: new tensors like the gradients."""
+    fn = "clip_grads"
+    grads, max_norm = list(grads), _bound(fn, max_norm)
+    if not grads:
+        return [], torch.tensor(0.0)
+    device = _checked(fn, grads)
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    if out is None:
+        out = [torch.empty_like(g) for g in grads]
+    else:
+        out = list(out)
+        if len(out) != len(grads) or any(o.shape != g.shape for o, g in zip(out, grads)):
+            raise ValueError(f"{fn}: out must hold one tensor of each gradient's shape")
+        if _checked(fn, out, "out") != device:
+            raise ValueError(f"{fn}: out must be on the gradients' device, {device}")
+        if not all(o.is_contiguous() for o in out):
+            raise ValueError(f"{fn}: out must be contiguous")
+        if len({o.data_ptr() for o in out if o.numel()}) < sum(o.numel() > 0 for o in out):
+            raise ValueError(f"{fn}: out holds one tensor twice")
+    return out, _clip(grads, out, max_norm, device)
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm):
+    """Scales the gradients of ``parameters`` (an iterable of tensors, or one) in place so
+    that their global 2-norm is at most ``max_norm``, and returns the norm before, a
+    float32 scalar: ``torch.nn.utils.clip_grad_norm_`` for CUDA float32 and bfloat16
+    gradients on one device, with the norm of ``grad_norm``.  A parameter listed twice
+    counts once.  Gradients below the bound are not written.  A NaN norm makes every
+    gradient NaN, as there.  No gradients: 0."""
+    fn = "clip_grad_norm_"
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    # a parameter listed twice is counted and scaled once
+    grads = [p.grad for p in dict.fromkeys(parameters) if p.grad is not None]
+    max_norm = _bound(fn, max_norm)
+    if not grads:
+        return torch.tensor(0.0)
+    device = _checked(fn, grads)
+    if all(map(_dense, grads)):
+        return _clip(grads, grads, max_norm, device)
+    # a gradient with gaps (a view of a larger buffer) goes through a copy
+    for g in grads:
+        if any(s == 0 and n > 1 for n, s in zip(g.shape, g.stride())):
+            raise ValueError(f"{fn}: a gradient expanded over its own memory cannot be scaled "
+                             "in place")
+    work = [g if _dense(g) else g.contiguous() for g in grads]
+    norm = _clip(work, work, max_norm, device)
+    for g, w in zip(grads, work):
+        if w is not g:
+            g.copy_(w)
+    return norm

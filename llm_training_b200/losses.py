@@ -1,0 +1,405 @@
+"""Losses that train on a model's answers: token log-probabilities, a preference loss
+over pairs of answers and a clipped policy loss with a KL term (csrc/sqb_logits.cu).
+
+All take CUDA float32 or bfloat16 logits with unit stride on the vocabulary (any other
+strides that do not overlap) and integer targets, where a negative target leaves its
+token out (the prompt, the padding): such a row of logits is not read and its gradient
+is zero.  A batch of S sequences is padded, logits (S, T, V) with targets (S, T), or
+packed, logits (N, V) with targets (N,) and ``cu_seqlens`` (S + 1,), the sequences'
+first rows and their end, non-decreasing; rows outside ``[cu_seqlens[0],
+cu_seqlens[S])`` are left out too.  A target past the vocabulary is never read: its
+log-probability and gradient row are NaN, as is everything summed from them.  Gradients
+reach the logits only, in their dtype and with their strides.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+__all__ = ["token_log_probs", "preference_loss", "policy_loss", "policy_loss_and_grad"]
+
+_DTYPES = {torch.float32: _lib.SQB_F32, torch.bfloat16: _lib.SQB_BF16}
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _stream(t):
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _grad_like(x):
+    """An uninitialised tensor of x's shape, strides and 16-byte phase (the gradient is
+    written with the vector stores the logits are read with)."""
+    elt = x.element_size()
+    phase = x.data_ptr() % 16 // elt
+    if phase == 0 or x.numel() == 0:
+        return torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=x.device)
+    span = 1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+    buf = torch.empty(span + phase, dtype=x.dtype, device=x.device)
+    return buf.as_strided(x.shape, x.stride(), phase)
+
+
+# ---- custom ops: x (S, T, V), t (S, T) int64 contiguous -----------------------------
+
+
+def _launch_logp(x, t, logp, logp64, stats):
+    S, T, V = x.shape
+    if S * T == 0:
+        return
+    _lib.check("sqb_logp_fwd", _lib.lib().sqb_logp_fwd(
+        x.data_ptr(), t.data_ptr(), _ptr(logp), _ptr(logp64), stats.data_ptr(), S, T, V,
+        x.stride(0), x.stride(1), _DTYPES[x.dtype], _stream(x)))
+
+
+@torch.library.custom_op("sqrtblock::logp_fwd", mutates_args=())
+def _logp_fwd(x: torch.Tensor, t: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(logp (S, T), row statistics (S, T, 2): max and sum of exp(x - max))."""
+    logp = torch.empty(t.shape, dtype=torch.float32, device=x.device)
+    stats = torch.empty((*t.shape, 2), dtype=torch.float32, device=x.device)
+    with _lib.on_device(x.device):
+        _launch_logp(x, t, logp, None, stats)
+    return logp, stats
+
+
+@_logp_fwd.register_fake
+def _(x, t):
+    return (x.new_empty(t.shape, dtype=torch.float32),
+            x.new_empty((*t.shape, 2), dtype=torch.float32))
+
+
+@torch.library.custom_op("sqrtblock::logp_bwd", mutates_args=())
+def _logp_bwd(x: torch.Tensor, t: torch.Tensor, stats: torch.Tensor, g_row: torch.Tensor,
+              scale: Optional[torch.Tensor]) -> torch.Tensor:
+    """g_row[r] * scale * ([c == t] - softmax) in x's dtype and strides."""
+    S, T, V = x.shape
+    dx = _grad_like(x)
+    if S * T:
+        with _lib.on_device(x.device):
+            _lib.check("sqb_logp_bwd", _lib.lib().sqb_logp_bwd(
+                x.data_ptr(), t.data_ptr(), stats.data_ptr(), g_row.data_ptr(), _ptr(scale),
+                dx.data_ptr(), S, T, V, x.stride(0), x.stride(1), dx.stride(0), dx.stride(1),
+                _DTYPES[x.dtype], _stream(x)))
+    return dx
+
+
+@_logp_bwd.register_fake
+def _(x, t, stats, g_row, scale):
+    return torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=x.device)
+
+
+def _logp_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs, output[1])
+    ctx.mark_non_differentiable(output[1])
+
+
+def _logp_grad(ctx, dlogp, _dstats):
+    x, t, stats = ctx.saved_tensors
+    return _logp_bwd(x, t, stats, dlogp.to(torch.float32).contiguous(), None), None
+
+
+_logp_fwd.register_autograd(_logp_grad, setup_context=_logp_setup)
+
+
+@torch.library.custom_op("sqrtblock::preference_fwd", mutates_args=())
+def _preference_fwd(x: torch.Tensor, t: torch.Tensor, ref: Optional[torch.Tensor],
+                    cu: Optional[torch.Tensor], pairs: int, beta: float, label_smoothing: float
+                    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(loss, rewards (2, P), row statistics, d loss / d logp of each row)."""
+    S, T, V = x.shape
+    dev = x.device
+    f32, f64 = torch.float32, torch.float64
+    logp = torch.empty(t.shape, dtype=f64, device=dev)
+    stats = torch.empty((*t.shape, 2), dtype=f32, device=dev)
+    # rows of a packed batch that belong to no sequence keep a zero
+    g_row = (torch.empty if cu is None else torch.zeros)(t.shape, dtype=f32, device=dev)
+    loss = torch.empty((), dtype=f32, device=dev)
+    rewards = torch.empty((2, pairs), dtype=f32, device=dev)
+    pair_loss = torch.empty(pairs, dtype=f64, device=dev)
+    with _lib.on_device(dev):
+        _launch_logp(x, t, None, logp, stats)
+        _lib.check("sqb_preference_finish", _lib.lib().sqb_preference_finish(
+            _ptr(logp), _ptr(cu), _ptr(ref), pairs, T, S * T, beta, label_smoothing,
+            pair_loss.data_ptr(), loss.data_ptr(), rewards.data_ptr(), _ptr(g_row), _stream(x)))
+    return loss, rewards, stats, g_row
+
+
+@_preference_fwd.register_fake
+def _(x, t, ref, cu, pairs, beta, label_smoothing):
+    f32 = torch.float32
+    return (x.new_empty((), dtype=f32), x.new_empty((2, pairs), dtype=f32),
+            x.new_empty((*t.shape, 2), dtype=f32), x.new_empty(t.shape, dtype=f32))
+
+
+def _preference_setup(ctx, inputs, output):
+    x, t = inputs[:2]
+    _, rewards, stats, g_row = output
+    ctx.save_for_backward(x, t, stats, g_row)
+    ctx.mark_non_differentiable(rewards, stats, g_row)
+
+
+def _loss_grad(ctx, dloss):
+    x, t, stats, g_row = ctx.saved_tensors
+    return _logp_bwd(x, t, stats, g_row, dloss.to(torch.float32).reshape(1))
+
+
+def _preference_grad(ctx, dloss, *_):
+    return _loss_grad(ctx, dloss), None, None, None, None, None, None
+
+
+_preference_fwd.register_autograd(_preference_grad, setup_context=_preference_setup)
+
+
+@torch.library.custom_op("sqrtblock::policy_fwd", mutates_args=())
+def _policy_fwd(x: torch.Tensor, t: torch.Tensor, adv: torch.Tensor,
+                old: Optional[torch.Tensor], ref: Optional[torch.Tensor],
+                cu: Optional[torch.Tensor], seqs: int, adv_by_seq: bool, per_seq: bool,
+                clip_low: float, clip_high: float, kl_coef: float, grad_scale: Optional[float]
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+                           torch.Tensor]:
+    """(loss, logps, (policy term, KL, clipped share), row statistics, d loss / d logp of
+    each row, the logits' gradient times grad_scale - empty for None)."""
+    S, T, V = x.shape
+    dev, N = x.device, S * T
+    f32, i32 = torch.float32, torch.int32
+    logps = torch.empty(t.shape, dtype=f32, device=dev)
+    rowstats = torch.empty((*t.shape, 2), dtype=f32, device=dev)
+    g_row = torch.empty(t.shape, dtype=f32, device=dev)
+    loss = torch.empty((), dtype=f32, device=dev)
+    stats = torch.empty(3, dtype=f32, device=dev)
+    dx = _grad_like(x) if grad_scale is not None else torch.empty(0, dtype=x.dtype, device=dev)
+    if N == 0:
+        return loss.zero_(), logps, stats.zero_(), rowstats, g_row, dx
+    terms = torch.empty((3, N), dtype=torch.float64, device=dev)
+    weight = torch.empty(N, dtype=f32, device=dev)
+    counts = torch.empty(seqs, dtype=i32, device=dev)
+    row_seq = torch.empty(N, dtype=i32, device=dev) if cu is not None else None
+    lib, stream = _lib.lib(), _stream(x)
+    with _lib.on_device(dev):
+        _lib.check("sqb_policy_weights", lib.sqb_policy_weights(
+            t.data_ptr(), _ptr(cu), seqs, T, N, int(per_seq), counts.data_ptr(),
+            weight.data_ptr(), _ptr(row_seq), stream))
+        _lib.check("sqb_policy_rows", lib.sqb_policy_rows(
+            x.data_ptr(), t.data_ptr(), _ptr(old), _ptr(ref), adv.data_ptr(), int(adv_by_seq),
+            _ptr(row_seq), weight.data_ptr(), clip_low, clip_high, kl_coef, logps.data_ptr(),
+            rowstats.data_ptr(), g_row.data_ptr(), terms.data_ptr(),
+            dx.data_ptr() if grad_scale is not None else None,
+            1.0 if grad_scale is None else grad_scale, S, T, V, x.stride(0), x.stride(1),
+            x.stride(0), x.stride(1), _DTYPES[x.dtype], stream))
+        _lib.check("sqb_policy_finish", lib.sqb_policy_finish(
+            terms.data_ptr(), weight.data_ptr(), N, kl_coef, loss.data_ptr(), stats.data_ptr(),
+            stream))
+    return loss, logps, stats, rowstats, g_row, dx
+
+
+@_policy_fwd.register_fake
+def _(x, t, adv, old, ref, cu, seqs, adv_by_seq, per_seq, clip_low, clip_high, kl_coef,
+      grad_scale):
+    f32 = torch.float32
+    dx = (torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=x.device)
+          if grad_scale is not None else x.new_empty(0))
+    return (x.new_empty((), dtype=f32), x.new_empty(t.shape, dtype=f32),
+            x.new_empty(3, dtype=f32), x.new_empty((*t.shape, 2), dtype=f32),
+            x.new_empty(t.shape, dtype=f32), dx)
+
+
+def _policy_setup(ctx, inputs, output):
+    x, t = inputs[:2]
+    _, logps, stats, rowstats, g_row, dx = output
+    ctx.save_for_backward(x, t, rowstats, g_row)
+    ctx.mark_non_differentiable(logps, stats, rowstats, g_row, dx)
+
+
+def _policy_grad(ctx, dloss, *_):
+    return (_loss_grad(ctx, dloss),) + (None,) * 12
+
+
+_policy_fwd.register_autograd(_policy_grad, setup_context=_policy_setup)
+
+
+# ---- public entry points --------------------------------------------------------------
+
+
+def _disjoint(x):
+    """Whether the rows of x (S, T, V), unit stride on V, occupy different memory."""
+    (S, T, V), (ss, st, _) = x.shape, x.stride()
+    if S <= 1 or T <= 1:
+        return (S <= 1 or ss >= V) and (T <= 1 or st >= V)
+    return (st >= V and ss >= (T - 1) * st + V) or (ss >= V and st >= (S - 1) * ss + V)
+
+
+def _rows(fn, logits, targets):
+    """Logits as (S, T, V) and targets as (S, T) int64, checked."""
+    if not logits.is_cuda:
+        raise RuntimeError(f"{fn}: logits must be a CUDA tensor (the op has no CPU "
+                           "implementation)")
+    if logits.dtype not in _DTYPES:
+        raise TypeError(f"{fn} supports float32 and bfloat16 logits, got {logits.dtype}")
+    if logits.dim() < 2 or logits.shape[-1] == 0:
+        raise ValueError(f"{fn}: logits must be (..., tokens, V), got {tuple(logits.shape)}")
+    if targets.shape != logits.shape[:-1] or targets.device != logits.device:
+        raise ValueError(f"{fn}: one target per row of logits on their device, got targets "
+                         f"{tuple(targets.shape)} for logits {tuple(logits.shape)}")
+    if targets.dtype.is_floating_point or targets.dtype.is_complex or targets.dtype == torch.bool:
+        raise TypeError(f"{fn}: targets must be integers, got {targets.dtype}")
+    V = logits.shape[-1]
+    x = logits
+    if x.dim() != 3:
+        x = (x.unsqueeze(0) if x.dim() == 2
+             else x.reshape(math.prod(x.shape[:-2]), x.shape[-2], V))
+    if x.shape[0] * x.shape[1] > 2**31 - 1:
+        raise ValueError(f"{fn}: at most 2**31 - 1 rows of logits")
+    if (x.stride(2) != 1 and V > 1) or not _disjoint(x):
+        x = x.contiguous()
+    return x, targets.to(torch.int64).reshape(x.shape[:2]).contiguous()
+
+
+def _sequences(fn, logits, targets, cu_seqlens):
+    """(x, t, cu_seqlens as int64 or None, sequences)."""
+    if cu_seqlens is None:
+        if logits.dim() != 3:
+            raise ValueError(f"{fn}: logits must be (sequences, tokens, V), or (rows, V) with "
+                             f"cu_seqlens, got {tuple(logits.shape)}")
+        x, t = _rows(fn, logits, targets)
+        return x, t, None, x.shape[0]
+    if logits.dim() != 2:
+        raise ValueError(f"{fn}: with cu_seqlens logits must be (rows, V), got "
+                         f"{tuple(logits.shape)}")
+    if (cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2
+            or cu_seqlens.dtype not in (torch.int32, torch.int64)
+            or cu_seqlens.device != logits.device):
+        raise ValueError(f"{fn}: cu_seqlens must be int32 or int64 (sequences + 1,) on the "
+                         "logits' device")
+    x, t = _rows(fn, logits, targets)
+    return x, t, cu_seqlens.to(torch.int64).contiguous(), cu_seqlens.numel() - 1
+
+
+def _given(fn, name, v, shapes, device):
+    """A fixed input as contiguous float32 of one of `shapes`."""
+    if v is None:
+        return None
+    if tuple(v.shape) not in shapes or v.device != device or not v.dtype.is_floating_point:
+        raise ValueError(f"{fn}: {name} must be floating point of shape "
+                         f"{' or '.join(map(str, shapes))} on the logits' device, got {v.dtype} "
+                         f"{tuple(v.shape)}")
+    if v.requires_grad:
+        raise ValueError(f"{fn}: no gradient reaches {name}: pass it detached")
+    return v.to(torch.float32).contiguous()
+
+
+def _number(fn, name, v, least=0.0, most=math.inf):
+    v = float(v)
+    if not least <= v <= most:
+        raise ValueError(f"{fn}: {name} must be in [{least}, {most}], got {v}")
+    return v
+
+
+def token_log_probs(logits, targets):
+    """Log-probability of each target under its row of logits (..., tokens, V), float32 in
+    the targets' shape; 0 where the target is negative.  Differentiable in the logits
+    (``sqrtblock::logp_fwd/bwd``): one read of the logits forward, and one read and one
+    write backward, with no softmax kept in between."""
+    x, t = _rows("token_log_probs", logits, targets)
+    return _logp_fwd(x, t)[0].view(targets.shape)
+
+
+def preference_loss(logits, targets, ref_logps=None, *, beta=0.1, label_smoothing=0.0,
+                    cu_seqlens=None):
+    """Preference loss over P pairs of answers -> (loss, chosen rewards, rejected rewards).
+
+    Of the 2P sequences the first P are the chosen answers and the last P the rejected
+    ones, in the same order.  With s the sum of a sequence's token log-probabilities and
+    ``ref_logps`` (2P,) the same sums under the reference model (None: zeros),
+
+        z = beta * ((s_chosen - ref_chosen) - (s_rejected - ref_rejected))
+        loss = mean of -(1 - label_smoothing) log sigmoid(z) - label_smoothing log sigmoid(-z)
+
+    and the rewards (P,) are beta * (s - ref), for logging (not differentiable).  Sums
+    and the loss are computed in 64 bits.  One read of the logits forward, one read and
+    one write backward: a pair's factor is known only after its last token."""
+    fn = "preference_loss"
+    x, t, cu, seqs = _sequences(fn, logits, targets, cu_seqlens)
+    if seqs == 0 or seqs % 2:
+        raise ValueError(f"{fn}: {seqs} sequences are no pairs")
+    ref = _given(fn, "ref_logps", ref_logps, [(seqs,)], x.device)
+    beta = _number(fn, "beta", beta, most=1e30)
+    label_smoothing = _number(fn, "label_smoothing", label_smoothing, most=1.0)
+    loss, rewards, _, _ = _preference_fwd(x, t, ref, cu, seqs // 2, beta, label_smoothing)
+    return loss, rewards[0], rewards[1]
+
+
+def _policy_args(fn, logits, targets, advantages, old_logps, ref_logps, clip, clip_high, kl_coef,
+                 reduction, cu_seqlens):
+    x, t, cu, seqs = _sequences(fn, logits, targets, cu_seqlens)
+    if reduction not in ("token", "sequence"):
+        raise ValueError(f"{fn}: reduction must be 'token' or 'sequence', got {reduction!r}")
+    if seqs == 0:
+        raise ValueError(f"{fn}: no sequences")
+    shape = tuple(targets.shape)
+    by_seq = [(seqs,)] if cu is not None else [(seqs,), (seqs, 1)]
+    adv = _given(fn, "advantages", advantages, [shape] + [s for s in by_seq if s != shape],
+                 x.device)
+    if adv is None:
+        raise ValueError(f"{fn}: advantages are needed")
+    old = _given(fn, "old_logps", old_logps, [shape], x.device)
+    ref = _given(fn, "ref_logps", ref_logps, [shape], x.device)
+    clip = _number(fn, "clip", clip)
+    clip_high = clip if clip_high is None else _number(fn, "clip_high", clip_high)
+    kl_coef = _number(fn, "kl_coef", kl_coef, most=1e30)
+    if kl_coef and ref is None:
+        raise ValueError(f"{fn}: a KL term needs ref_logps")
+    return (x, t, adv, old, ref, cu, seqs, tuple(adv.shape) != shape, reduction == "sequence",
+            clip, clip_high, kl_coef)
+
+
+def policy_loss(logits, targets, advantages, old_logps=None, ref_logps=None, *, clip=0.2,
+                clip_high=None, kl_coef=0.0, reduction="token", cu_seqlens=None):
+    """Clipped policy loss with a KL term -> (loss, log-probabilities, statistics).
+
+    Per counted token, with logp its log-probability, r = exp(logp - old_logps) (1 where
+    ``old_logps`` is None: the sampling policy is this one) and A its advantage,
+
+        -min(r A, min(max(r, 1 - clip), 1 + clip_high) A)
+            + kl_coef (exp(ref_logps - logp) - (ref_logps - logp) - 1)
+
+    averaged over the counted tokens (``reduction="token"``), or over each sequence's
+    counted tokens and then over the sequences that have any (``"sequence"``); 0 where no
+    token is counted.  ``clip_high`` None is ``clip``.  ``old_logps`` and ``ref_logps``
+    have the targets' shape, ``advantages`` that or one value per sequence (a 1-D tensor
+    of as many values as a packed batch has rows is one per token).  The gradient of a
+    token on the clip's border is the unclipped one.  What the inputs hold at tokens that
+    are left out is not looked at.
+
+    The log-probabilities (float32, the targets' shape, 0 at tokens left out) and the
+    statistics - (mean policy term, mean KL, share of clipped tokens), averaged as the
+    loss - are for logging and for the next step's ``old_logps``, not differentiable."""
+    args = _policy_args("policy_loss", logits, targets, advantages, old_logps, ref_logps, clip,
+                        clip_high, kl_coef, reduction, cu_seqlens)
+    loss, logps, stats, _, _, _ = _policy_fwd(*args, None)
+    return loss, logps.view(targets.shape), stats
+
+
+def policy_loss_and_grad(logits, targets, advantages, old_logps=None, ref_logps=None, *,
+                         clip=0.2, clip_high=None, kl_coef=0.0, reduction="token",
+                         cu_seqlens=None, grad_scale=1.0):
+    """``policy_loss`` and its gradient in one pass over the logits -> (loss, gradient,
+    log-probabilities, statistics).
+
+    The gradient (the logits' shape, dtype and strides) is that of ``grad_scale * loss``;
+    hand it on with ``logits.backward(gradient)``.  A token's factor needs its own row
+    only, so each row is read from HBM once and its gradient written once, where the
+    autograd form reads the logits a second time."""
+    fn = "policy_loss_and_grad"
+    args = _policy_args(fn, logits.detach(), targets, advantages, old_logps, ref_logps, clip,
+                        clip_high, kl_coef, reduction, cu_seqlens)
+    grad_scale = float(grad_scale)
+    if not math.isfinite(grad_scale):
+        raise ValueError(f"{fn}: grad_scale must be finite, got {grad_scale}")
+    loss, logps, stats, _, _, dx = _policy_fwd(*args, grad_scale)
+    return loss, dx[0] if logits.dim() == 2 else dx, logps.view(targets.shape), stats
