@@ -92,12 +92,11 @@ int sqb_add_layernorm_bwd(const void* dy, int dy_dtype, const float* x_out, cons
  * negative one leaves its row out: the row is not read, its log-probability is 0
  * and its gradient row zero.  One of V or more gives NaN.  S * T < 2^31. */
 
-/* Per row: logp = log softmax(logits)[target] as fp32 and/or in 64 bits (either
- * pointer may be NULL), and stats = (max, sum of exp(x - max)), fp32 (S * T, 2),
- * 8-byte aligned (a row left out: (0, 1)). */
-int sqb_logp_fwd(const void* logits, const int64_t* targets, float* logp, double* logp_double,
-                 float* stats, int64_t S, int64_t T, int64_t V, int64_t ss, int64_t st, int dtype,
-                 void* stream);
+/* Per row: logp = log softmax(logits)[target], and stats = (m, sum of exp(x - m)) with m
+ * a number near the row's maximum, fp32 (S * T, 2), 8-byte aligned (a row left out:
+ * (0, 1)). */
+int sqb_logp_fwd(const void* logits, const int64_t* targets, float* logp, float* stats, int64_t S,
+                 int64_t T, int64_t V, int64_t ss, int64_t st, int dtype, void* stream);
 
 /* dlogits[r, c] = g_row[r] * scale[0] * ([c == target] - softmax(logits)[r, c]) in the
  * logits' dtype, strides dss and dst; scale (one fp32 on the device) may be NULL.  Rows
@@ -107,47 +106,43 @@ int sqb_logp_bwd(const void* logits, const int64_t* targets, const float* stats,
                  int64_t V, int64_t ss, int64_t st, int64_t dss, int64_t dst, int dtype,
                  void* stream);
 
-/* Preference loss over P pairs from the rows' log-probabilities in 64 bits (0 where
- * left out): sequence p < P is chosen, P + p its rejected one.  Sequence s has rows
- * [cu_seqlens[s], cu_seqlens[s + 1]) (2P + 1 entries, held inside [0, N]), or with
- * cu_seqlens NULL rows [s * T, (s + 1) * T), N = 2P * T.  With r = sum of logp -
- * ref_logps[s] (fp32, NULL: 0) and z = beta * (r_chosen - r_rejected):
+/* Sequences: with cu_seqlens (S = 1) sequence i has rows [cu_seqlens[i],
+ * cu_seqlens[i + 1]), non-decreasing and held inside [0, N], N = S * T; rows of no
+ * sequence are left out.  NULL: sequence i has rows [i * T, (i + 1) * T). */
+
+/* Preference loss over P pairs: sequence p < P is chosen, P + p its rejected one.  With
+ * r = sum of the sequence's logp - ref_logps[i] (fp32, NULL: 0) and
+ * z = beta * (r_chosen - r_rejected):
  *   loss = mean of -(1 - label_smoothing) log sigmoid(z) - label_smoothing log sigmoid(-z),
- *   rewards (2P, fp32) = beta * r,   g_row (N, fp32) = d loss / d logp
- * (rows of no sequence are not written).  pair_loss: P doubles of scratch. */
-int sqb_preference_finish(const double* logp, const int64_t* cu_seqlens, const float* ref_logps,
-                          int64_t P, int64_t T, int64_t N, double beta, double label_smoothing,
-                          double* pair_loss, float* loss, float* rewards, float* g_row,
-                          void* stream);
+ *   rewards (2P, fp32) = beta * r,   g_row (N, fp32) = d loss / d logp,
+ * stats as sqb_logp_fwd: the gradient is sqb_logp_bwd's from stats and g_row.  T may be 0
+ * (logits, targets, stats and g_row then unused).  The sums and the loss are computed in
+ * 64 bits, in a fixed order; the workspace (8-byte aligned) needs no initialisation. */
+size_t sqb_preference_workspace_bytes(int64_t N, int64_t P);
+int sqb_preference_fwd(const void* logits, const int64_t* targets, const int64_t* cu_seqlens,
+                       const float* ref_logps, int64_t P, double beta, double label_smoothing,
+                       float* loss, float* rewards, float* stats, float* g_row, int64_t S,
+                       int64_t T, int64_t V, int64_t ss, int64_t st, int dtype, void* workspace,
+                       size_t ws_bytes, void* stream);
 
-/* Weight (fp32, N) of every row in the policy loss: 1 / counted rows, or with
- * per_sequence 1 / (counted rows of its sequence * sequences that have any); 0 for a
- * row left out by its target or by cu_seqlens.  counts: S int32 of scratch.  row_seq
- * (int32, N; needed with cu_seqlens): the row's sequence, -1 for none. */
-int sqb_policy_weights(const int64_t* targets, const int64_t* cu_seqlens, int64_t S, int64_t T,
-                       int64_t N, int per_sequence, int32_t* counts, float* weight,
-                       int32_t* row_seq, void* stream);
-
-/* Per row of weight w != 0, with r = exp(logp - old_logp) (1 for NULL), A = adv[row]
- * (adv_by_seq: of its sequence, row_seq's or row / T) and ref_logp (NULL: no KL):
- *   terms = (-min(r A, held(r) A), exp(ref - logp) - (ref - logp) - 1, [clipped]), held
- *   keeping r in [1 - clip_low, 1 + clip_high]; (3, N) in 64 bits
- *   g_row = w * d(terms[0] + kl_coef * terms[1]) / d logp
- * and logp, stats as sqb_logp_fwd (each may be NULL, as g_row).  With dlogits, also the
- * gradient as sqb_logp_bwd with factor g_row * grad_scale, in the same pass.  Rows of
- * weight 0 get zeros. */
-int sqb_policy_rows(const void* logits, const int64_t* targets, const float* old_logp,
-                    const float* ref_logp, const float* adv, int adv_by_seq,
-                    const int32_t* row_seq, const float* weight, double clip_low,
-                    double clip_high, double kl_coef, float* logp, float* stats, float* g_row,
-                    double* terms, void* dlogits, float grad_scale, int64_t S, int64_t T,
-                    int64_t V, int64_t ss, int64_t st, int64_t dss, int64_t dst, int dtype,
-                    void* stream);
-
-/* loss = sum of weight * (terms[0] + kl_coef * terms[1]); stats (3) = the weighted sums of
- * the terms, in a fixed order. */
-int sqb_policy_finish(const double* terms, const float* weight, int64_t N, double kl_coef,
-                      float* loss, float* stats, void* stream);
+/* Clipped policy loss over `seqs` sequences.  Per counted row, with
+ * r = exp(logp - old_logp) (1 for NULL), A = adv[row] (adv_by_seq: adv[sequence]) and
+ * ref_logp (NULL: no KL):
+ *   policy = -min(r A, held A), held = r kept in [1 - clip_low, 1 + clip_high],
+ *   KL = exp(ref - logp) - (ref - logp) - 1,   clipped = [held A < r A];
+ *   loss = sum of w (policy + kl_coef KL),   statistics (3) = sums of w (policy, KL, clipped)
+ * with w = 1 / counted rows, or per_sequence 1 / (counted rows of its sequence * sequences
+ * that have any); 0 where no row is counted.  logp as sqb_logp_fwd; stats and g_row (each
+ * may be NULL) as sqb_preference_fwd.  With dlogits also the gradient of
+ * grad_scale * loss, as sqb_logp_bwd writes it, in the same pass over the logits. */
+size_t sqb_policy_workspace_bytes(int64_t N, int64_t seqs);
+int sqb_policy_fwd(const void* logits, const int64_t* targets, const int64_t* cu_seqlens,
+                   int64_t seqs, const float* old_logp, const float* ref_logp, const float* adv,
+                   int adv_by_seq, double clip_low, double clip_high, double kl_coef,
+                   int per_sequence, float* loss, float* statistics, float* logp, float* stats,
+                   float* g_row, void* dlogits, float grad_scale, int64_t S, int64_t T, int64_t V,
+                   int64_t ss, int64_t st, int64_t dss, int64_t dst, int dtype, void* workspace,
+                   size_t ws_bytes, void* stream);
 
 /* ---- Global gradient norm and clipping ---------------------------------------
  * n tensors as host arrays of device pointers (element-aligned), element counts (each

@@ -90,15 +90,15 @@ TRAIN_SIGNATURES = {
                               [ctypes.c_void_p] * 10 +
                               [ctypes.c_size_t, _c_i64, _c_i64, ctypes.c_void_p]),
     # token log-probabilities and the losses on them
-    "sqb_logp_fwd": (ctypes.c_int, [_vp] * 5 + [_c_i64] * 5 + [ctypes.c_int, _vp]),
+    "sqb_logp_fwd": (ctypes.c_int, [_vp] * 4 + [_c_i64] * 5 + [ctypes.c_int, _vp]),
     "sqb_logp_bwd": (ctypes.c_int, [_vp] * 6 + [_c_i64] * 7 + [ctypes.c_int, _vp]),
-    "sqb_preference_finish": (ctypes.c_int, [_vp] * 3 + [_c_i64] * 3 + [ctypes.c_double] * 2 +
-                              [_vp] * 5),
-    "sqb_policy_weights": (ctypes.c_int, [_vp] * 2 + [_c_i64] * 3 + [ctypes.c_int] + [_vp] * 4),
-    "sqb_policy_rows": (ctypes.c_int, [_vp] * 5 + [ctypes.c_int] + [_vp] * 2 +
-                        [ctypes.c_double] * 3 + [_vp] * 5 + [ctypes.c_float] + [_c_i64] * 7 +
-                        [ctypes.c_int, _vp]),
-    "sqb_policy_finish": (ctypes.c_int, [_vp] * 2 + [_c_i64, ctypes.c_double] + [_vp] * 3),
+    "sqb_preference_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 2),
+    "sqb_preference_fwd": (ctypes.c_int, [_vp] * 4 + [_c_i64] + [ctypes.c_double] * 2 +
+                           [_vp] * 4 + [_c_i64] * 5 + [ctypes.c_int, _vp, ctypes.c_size_t, _vp]),
+    "sqb_policy_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 2),
+    "sqb_policy_fwd": (ctypes.c_int, [_vp] * 3 + [_c_i64] + [_vp] * 3 + [ctypes.c_int] +
+                       [ctypes.c_double] * 3 + [ctypes.c_int] + [_vp] * 6 + [ctypes.c_float] +
+                       [_c_i64] * 7 + [ctypes.c_int, _vp, ctypes.c_size_t, _vp]),
     # gradient norm and clipping
     "sqb_grad_norm_workspace_bytes": (ctypes.c_size_t, [_c_i64]),
     "sqb_grad_norm": (ctypes.c_int, [_vp] * 3 + [_c_i64, _vp, ctypes.c_size_t, _vp, _vp]),
@@ -122,6 +122,15 @@ def on_device(device):
     if device.index is None or device.index == torch.cuda.current_device():
         return contextlib.nullcontext()
     return torch.cuda.device(device)
+
+
+def plain(x) -> bool:
+    """Whether `x` is an ordinary tensor in an ordinary eager call.  The post-training ops
+    then run without the dispatcher, whose custom-op layers cost 100 us a call; a traced,
+    fake or otherwise intercepted call goes through the registered custom op."""
+    return (type(x) in (torch.Tensor, torch.nn.Parameter) and not torch.compiler.is_compiling()
+            and torch._C._len_torch_dispatch_stack() == 0
+            and not torch._C._are_functorch_transforms_active())
 
 
 def library_path() -> str:

@@ -2,21 +2,36 @@
 // (include/sqb_train.h): a preference loss over pairs of answers and a clipped
 // policy loss with a KL term, forward and backward.
 //
-// A row of V logits x with target t:  m = max x,  s = sum exp(x - m),
-//   logp = (x_t - m) - log s,   d logp / d x_c = [c == t] - exp(x_c - m) / s.
-// (m, s) is kept for the backward instead of log-sum-exp: exp(x - m) / s has the
-// rounding of one subtraction of nearby numbers, exp(x - lse) that of lse itself.
-// The row's sum is fp32 over at most a few hundred terms a thread and a tree over
-// threads; logp, and everything per token or per sequence above it, is computed in
-// 64 bits by one thread, since a sequence's sum of logps is hundreds to thousands
-// and the losses are made of small differences of such sums.
+// A row of V logits x with target t, m a number near its maximum:
+//   s = sum exp(x - m),  logp = x_t - m - log s,  d logp / d x_c = [c == t] - exp(x_c - m) / s.
+// (m, s) is kept for the backward.  A sequence's log-probability is a sum of hundreds
+// to thousands of logps and the losses are made of small differences of such sums, so
+// an error that all rows share grows with the length: everything above s is computed
+// in 64 bits by one thread, and s itself is summed without such an error (below).
 //
-// All kernels over logits are bound by HBM: they read each row once, all of its
-// loads independent, and rows whose target is ignored are not read at all.
+// The kernels over logits are bound by HBM: they read each row once, with independent
+// 16-byte loads, and rows whose target is ignored are not read at all.  The exponentials
+// come next (one special-function result for each logit, 16 a clock and SM, against 11.7
+// bf16 logits a clock and SM at 6.56 TB/s), which is why the sum is shaped around them.
+//
+// Sum of exponentials: of 2^(x log2(e) - c), c a whole number no smaller than the largest
+// x log2(e), so that a new maximum rescales by an exact power of two.  The arguments must
+// not be rounded either: rounding them, or rescaling by an approximate exponential, costs
+// as much and leaves 1e-7 of s in every row, the same sign in all - 5e-5 of a 512-token
+// answer's log-probability, against 1e-6 this way.
+//   bf16: with H = log2(e) cut to 15 bits, x H has at most 23 bits and x H - c is exact in
+//     one fused multiply-add.  What H lacks, exp(x) = 2^(x H) exp(x d) with
+//     d = 1 - H ln 2 (5e-6), is made up for once a row: sum e (1 + (x - x0) d) from the sums
+//     of e and of e x (the next term, ((x - x0) d)^2 / 2, is below 1e-8 where e counts).
+//   fp32: h = fl(x L), h - c is exact, and the rest of x log2(e), an fma's residual and the
+//     constant's low part, is summed as e r beside e.
+// Rows whose maximum is beyond 2800 are summed again by one warp, with rounded arguments.
 
 #include <cuda_bf16.h>
 #include <math.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "sqb_train.h"
 
@@ -25,14 +40,24 @@ namespace logits {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2eLow = (float)(1.4426950408889634 - (double)kLog2e);
+constexpr double kLn2 = 0.6931471805599453;
+// log2(e) cut to 15 bits, and 1 - H ln 2 (4.9e-6)
+constexpr float kH = 23637.0f / 16384.0f;
+constexpr double kLack = 1.0 - (double)kH * kLn2;
+constexpr int kBound = 4096;  // of c in the exact form
+// ex2.approx of arguments below 0 falls short by 5.06e-8 in the mean (measured on B200 over
+// 2^20 arguments a binade, the same for all of [-16, 0)), about a third of its largest error.
+// All of a row's terms share it, and all rows: it is made up for in the sum.
+constexpr double kExp2Short = 5.06e-8;
 
 struct View {  // (S, T, V) logits, unit stride on V; strides in elements
   int64_t T, V, ss, st;
 };
 
-__device__ __forceinline__ int64_t row_offset(int64_t r, int64_t T, int64_t ss, int64_t st) {
-  const int64_t s = r / T;
-  return s * ss + (r - s * T) * st;
+__device__ __forceinline__ int64_t row_offset(uint32_t r, int64_t T, int64_t ss, int64_t st) {
+  const uint32_t s = r / (uint32_t)T;
+  return s * ss + (r - s * (uint32_t)T) * st;
 }
 
 __device__ __forceinline__ float to_f(float x) { return x; }
@@ -53,155 +78,323 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// max that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 
-// exp(x - m): the difference first, so that no rounding of m * log2(e) is shared by
-// the whole row.
 __device__ __forceinline__ float exp_diff(float x, float m) {
   return exp2_approx((x - m) * kLog2e);
 }
 
-// The max a running sum is taken against: 0 while every element so far is -inf
+// The number a running sum is taken against: 0 while every element so far is -inf
 // (their exponentials are then 0, and a NaN still shows).
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }
 
-// Adds a sum over another part of the row, (m2, s2), to (m, s).
-__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
-  const float top = fmaxf(m, m2), ref = finite_ref(top);
-  s = s * exp_diff(m, ref) + s2 * exp_diff(m2, ref);
-  m = top;
-}
-
 // Elements before the first 16-byte boundary of `p`, at most V.
 template <typename T>
-__device__ __forceinline__ int64_t head_of(const T* p, int64_t V) {
-  const int64_t h = ((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T);
+__device__ __forceinline__ int head_of(const T* p, int V) {
+  const int h = (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / (int)sizeof(T);
   return h < V ? h : V;
 }
 
-// (max, sum of exp(x - max)) over a row, the same in every thread of the CTA.
-// red: 2 * 32 floats of shared memory.
-template <typename T, int kThreads>
-__device__ void row_stats(const T* row, int64_t V, float* red, float& m_out, float& s_out) {
-  constexpr int kN = 16 / sizeof(T);
-  const int64_t head = head_of(row, V), nvec = (V - head) / kN;
-  float m = -INFINITY, s = 0.f;
-  auto one = [&](float x) { join(m, s, x, 1.f); };
-  if (threadIdx.x < head) one(to_f(row[threadIdx.x]));
-  const T* body = row + head;
-  for (int64_t i = threadIdx.x; i < nvec; i += kThreads) {
-    const uint4 u = *reinterpret_cast<const uint4*>(body + i * kN);
-    const T* e = reinterpret_cast<const T*>(&u);
-    float x[kN], top = m;
-#pragma unroll
-    for (int j = 0; j < kN; ++j) {
-      x[j] = to_f(e[j]);
-      top = fmaxf(top, x[j]);
-    }
-    const float ref = finite_ref(top);
-    s *= exp_diff(m, ref);
-#pragma unroll
-    for (int j = 0; j < kN; ++j) s += exp_diff(x[j], ref);
-    m = top;
-  }
-  const int64_t tail = head + nvec * kN + threadIdx.x;
-  if (tail < V) one(to_f(row[tail]));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    join(m, s, m2, s2);
-  }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) {
-    red[warp] = m;
-    red[32 + warp] = s;
-  }
-  __syncthreads();
-  m = lane < kThreads / 32 ? red[lane] : -INFINITY;
-  s = lane < kThreads / 32 ? red[32 + lane] : 0.f;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    join(m, s, m2, s2);
-  }
-  m_out = m;
-  s_out = s;
+// A group of kThreads threads works on a row: a CTA of kThreads, or (32) one of its warps.
+template <int kThreads>
+__device__ __forceinline__ int rank() {
+  return kThreads == 32 ? (threadIdx.x & 31) : threadIdx.x;
+}
+template <int kThreads>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (kThreads == 32)
+    __syncwarp();
+  else
+    __syncthreads();
 }
 
-// drow[c] = g * ([c == t] - exp(row[c] - m) / s) for c < V, by the whole CTA.
+// Part of a row's sum: e = 2^(x log2(e) - ref) and its correction (e x for bf16, e r for fp32).
+// e is added up in fp32 over a group of up to 32 elements and from there in 64 bits: next to a
+// longer fp32 sum, what is below 2^-25 of it is lost, 1e-7 of s in all for logits whose
+// standard deviation is 4.
+struct Part {
+  int ref;
+  double a;
+  float b;
+};
+constexpr int kNone = -65536;  // ref before the first element
+
+// 2^k for k <= 0
+__device__ __forceinline__ float power_of_2(int k) {
+  return __int_as_float((max(k, -127) + 127) << 23);
+}
+
+__device__ __forceinline__ void rescale(Part& p, int ref) {
+  const float f = power_of_2(p.ref - ref);
+  p.a *= f;
+  p.b *= f;
+  p.ref = ref;
+}
+
+// The sum of the warp's parts, in all its lanes.
+__device__ __forceinline__ void join_warp(Part& p) {
+  rescale(p, __reduce_max_sync(0xffffffffu, p.ref));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    p.a += __shfl_xor_sync(0xffffffffu, p.a, o);
+    p.b += __shfl_xor_sync(0xffffffffu, p.b, o);
+  }
+}
+
+// Stand for -inf and below: their exponentials are 0 as well, and their corrections finite.
+constexpr float kLowestBf16 = -3.3e38f, kLowest = -1e30f;
+
+// Makes p's ref no smaller than top's.
+template <typename T>
+__device__ __forceinline__ void raise(Part& p, float top) {
+  const int c = min(__float2int_ru(top * (sizeof(T) == 2 ? kH : kLog2e)), -kNone);
+  if (c > p.ref) rescale(p, c);
+}
+
+template <typename T>
+__device__ __forceinline__ void add(Part& p, float& a, float c, float x) {
+  if constexpr (sizeof(T) == 2) {
+    const float e = exp2_approx(fmaf(x, kH, -c));
+    a += e;
+    p.b = fmaf(e, x, p.b);
+  } else {
+    const float h = x * kLog2e, e = exp2_approx(h - c);
+    a += e;
+    p.b = fmaf(e, fmaf(x, kLog2eLow, fmaf(x, kLog2e, -h)), p.b);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void add_one(Part& p, T v) {
+  const float x = max_nan(to_f(v), sizeof(T) == 2 ? kLowestBf16 : kLowest);
+  float a = 0.f;
+  raise<T>(p, x);
+  add<T>(p, a, (float)p.ref, x);
+  p.a += a;
+}
+
+// Adds the n 16-byte vectors u.
+template <typename T, int n>
+__device__ __forceinline__ void add_vectors(Part& p, uint4 (&u)[n]) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(u);
+  float a = 0.f;
+  if constexpr (sizeof(T) == 4) {
+    float top = kLowest;
+#pragma unroll
+    for (int j = 0; j < 4 * n; ++j) {
+      w[j] = __float_as_uint(max_nan(__uint_as_float(w[j]), kLowest));
+      top = fmaxf(top, __uint_as_float(w[j]));
+    }
+    raise<T>(p, top);
+    const float c = (float)p.ref;
+#pragma unroll
+    for (int j = 0; j < 4 * n; ++j) add<T>(p, a, c, __uint_as_float(w[j]));
+  } else {
+    const __nv_bfloat162 low = __float2bfloat162_rn(kLowestBf16);
+    __nv_bfloat162 top = low;
+#pragma unroll
+    for (int j = 0; j < 4 * n; ++j) {
+      const __nv_bfloat162 v = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&w[j]), low);
+      top = __hmax2(top, v);
+      w[j] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    raise<T>(p, fmaxf(__low2float(top), __high2float(top)));
+    const float c = (float)p.ref;
+#pragma unroll
+    for (int j = 0; j < 4 * n; ++j) {
+      add<T>(p, a, c, __uint_as_float(w[j] << 16));
+      add<T>(p, a, c, __uint_as_float(w[j] & 0xffff0000u));
+    }
+  }
+  p.a += a;
+}
+
+constexpr int kUnroll = 4;
+
+// (m, s) of a row whose maximum is out of the exact form's range, by one warp: rounded
+// arguments, 64-bit sums.
+template <typename T>
+__device__ void far_stats(const T* row, int V, float& m, double& s) {
+  const int lane = threadIdx.x & 31;
+  float top = -INFINITY;
+  for (int c = lane; c < V; c += 32) top = fmaxf(top, to_f(row[c]));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float ref = finite_ref(top);
+  s = 0.0;
+  for (int c = lane; c < V; c += 32) s += exp_diff(to_f(row[c]), ref);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  m = top;
+}
+
+// A row's (m, s), by its group of threads; in the lanes of the group's first warp alone.
+// red: shared memory of a CTA's warps.
 template <typename T, int kThreads>
-__device__ void write_grad(const T* row, T* drow, int64_t V, int64_t t, float m, float s,
-                           float g) {
+__device__ void row_stats(const T* row, int V, Part* red, float& m, double& s) {
   constexpr int kN = 16 / sizeof(T);
-  const float k = -g / s;
-  auto grad = [&](float x, int64_t c) {
+  Part p{kNone, 0.0, 0.f};
+  const int head = head_of(row, V), nvec = (V - head) / kN, me = rank<kThreads>();
+  const uint4* body = reinterpret_cast<const uint4*>(row + head);
+  int i = me;
+  for (; i + (kUnroll - 1) * kThreads < nvec; i += kUnroll * kThreads) {
+    uint4 u[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) u[k] = body[i + k * kThreads];
+    add_vectors<T>(p, u);
+  }
+  for (; i < nvec; i += kThreads) {
+    uint4 u[1] = {body[i]};
+    add_vectors<T>(p, u);
+  }
+  if (me < head) add_one<T>(p, row[me]);
+  const int tail = head + nvec * kN + me;
+  if (tail < V) add_one<T>(p, row[tail]);
+  join_warp(p);
+  if constexpr (kThreads > 32) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) red[warp] = p;
+    __syncthreads();
+    if (warp) return;
+    p = lane < kThreads / 32 ? red[lane] : Part{kNone, 0.0, 0.f};
+    join_warp(p);
+  }
+  if (abs(p.ref) >= kBound) {
+    far_stats(row, V, m, s);
+    return;
+  }
+  const double x0 = p.ref * kLn2;
+  m = (float)x0;
+  double y = x0 - (double)m;  // sum e^x = 2^ref sum = e^(m + y) sum
+  if constexpr (sizeof(T) == 2) {
+    s = p.a + kLack * ((double)p.b - x0 * p.a);  // sum e^(x lack) e = e^(x0 lack) s
+    y += x0 * kLack;                             // below 0.02
+  } else {
+    s = p.a + kLn2 * (double)p.b;
+  }
+  s *= 1.0 + kExp2Short + y * (1.0 + y * (0.5 + y * (1.0 / 6 + y / 24)));
+}
+
+// drow[c] = g [c == t] + k exp(row[c] - m) for c < V, k = -g / s, by the group.
+template <typename T, int kThreads>
+__device__ void write_grad(const T* row, T* drow, int V, int64_t t, float m, float k, float g) {
+  constexpr int kN = 16 / sizeof(T);
+  const int me = rank<kThreads>();
+  auto grad = [&](float x, int c) {
     const float p = k * exp_diff(x, m);
     return from_f<T>(c == t ? g + p : p);
   };
   if (((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(drow)) & 15) != 0) {
-    for (int64_t c = threadIdx.x; c < V; c += kThreads) drow[c] = grad(to_f(row[c]), c);
+    for (int c = me; c < V; c += kThreads) drow[c] = grad(to_f(row[c]), c);
     return;
   }
-  const int64_t head = head_of(row, V), nvec = (V - head) / kN;
-  if (threadIdx.x < head) drow[threadIdx.x] = grad(to_f(row[threadIdx.x]), threadIdx.x);
-  for (int64_t i = threadIdx.x; i < nvec; i += kThreads) {
-    const int64_t c = head + i * kN;
-    const uint4 u = *reinterpret_cast<const uint4*>(row + c);
+  const int head = head_of(row, V), nvec = (V - head) / kN;
+  if (me < head) drow[me] = grad(to_f(row[me]), me);
+  const uint4* body = reinterpret_cast<const uint4*>(row + head);
+  uint4* out = reinterpret_cast<uint4*>(drow + head);
+  auto vector = [&](uint4 u) {
     const T* e = reinterpret_cast<const T*>(&u);
     uint4 o;
     T* d = reinterpret_cast<T*>(&o);
 #pragma unroll
-    for (int j = 0; j < kN; ++j) d[j] = grad(to_f(e[j]), c + j);
-    *reinterpret_cast<uint4*>(drow + c) = o;
+    for (int j = 0; j < kN; ++j) d[j] = from_f<T>(k * exp_diff(to_f(e[j]), m));
+    return o;
+  };
+  int i = me;
+  for (; i + (kUnroll - 1) * kThreads < nvec; i += kUnroll * kThreads) {
+    uint4 u[kUnroll];
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) u[j] = body[i + j * kThreads];
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) out[i + j * kThreads] = vector(u[j]);
   }
-  const int64_t tail = head + nvec * kN + threadIdx.x;
+  for (; i < nvec; i += kThreads) out[i] = vector(body[i]);
+  const int tail = head + nvec * kN + me;
   if (tail < V) drow[tail] = grad(to_f(row[tail]), tail);
+  // the target's element, by the thread that wrote its vector
+  const int at = (int)(t - head);
+  if (t >= head && at < nvec * kN && (at / kN) % kThreads == me)
+    drow[t] = grad(to_f(row[t]), (int)t);
 }
 
 template <typename T, int kThreads>
-__device__ void write_zeros(T* drow, int64_t V) {
+__device__ void write_zeros(T* drow, int V) {
   constexpr int kN = 16 / sizeof(T);
-  const int64_t head = head_of(drow, V), nvec = (V - head) / kN;
-  if (threadIdx.x < head) drow[threadIdx.x] = from_f<T>(0.f);
-  for (int64_t i = threadIdx.x; i < nvec; i += kThreads)
-    *reinterpret_cast<uint4*>(drow + head + i * kN) = make_uint4(0, 0, 0, 0);
-  const int64_t tail = head + nvec * kN + threadIdx.x;
+  const int head = head_of(drow, V), nvec = (V - head) / kN, me = rank<kThreads>();
+  if (me < head) drow[me] = from_f<T>(0.f);
+  uint4* out = reinterpret_cast<uint4*>(drow + head);
+  for (int i = me; i < nvec; i += kThreads) out[i] = make_uint4(0, 0, 0, 0);
+  const int tail = head + nvec * kN + me;
   if (tail < V) drow[tail] = from_f<T>(0.f);
 }
 
 // Log-probability of target t in 64 bits (NaN for a t past the vocabulary).
 template <typename T>
-__device__ __forceinline__ double logp_of(const T* row, int64_t V, int64_t t, float m, float s) {
+__device__ __forceinline__ double logp_of(const T* row, int V, int64_t t, float m, double s) {
   if (t >= V) return NAN;
-  return ((double)to_f(row[t]) - (double)m) - log((double)s);
+  return ((double)to_f(row[t]) - (double)m) - log(s);
 }
 
-constexpr int kThreads = 512;
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    logp_fwd_kernel(const T* x, const int64_t* targets, float* logp, double* logp64,
-                    float2* stats, View v) {
-  __shared__ float red[64];
-  const int64_t r = blockIdx.x, t = targets[r];
-  float m = 0.f, s = 1.f;
-  double lp = 0.0;
+// ---- rows -------------------------------------------------------------------------
+
+constexpr int kRowThreads = 512;   // a CTA for each row
+constexpr int kWarpRows = 8;       // or a warp, eight rows to a CTA
+// Rows up to this many bytes take a warp.
+constexpr int64_t kWarpRowBytes = 8192;
+
+template <int kThreads>
+constexpr int block_of() {
+  return kThreads == 32 ? 32 * kWarpRows : kThreads;
+}
+// The group's row; >= N for a warp that has none.
+template <int kThreads>
+__device__ __forceinline__ uint32_t row_of() {
+  return kThreads == 32 ? blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
+}
+
+// Per-row outputs: logp (either or both), stats = (m, s), and a zero for g_row.
+struct RowOut {
+  float* logp;
+  double* logp64;
+  float2* stats;
+  float* g_row;
+};
+
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(block_of<kThreads>())
+    logp_fwd_kernel(const T* x, const int64_t* targets, RowOut out, View v, uint32_t N) {
+  __shared__ Part red[32];
+  const uint32_t r = row_of<kThreads>();
+  if (kThreads == 32 && r >= N) return;
+  const int64_t t = targets[r];
+  float m = 0.f;
+  double s = 1.0, lp = 0.0;
   if (t >= 0) {
     const T* row = x + row_offset(r, v.T, v.ss, v.st);
-    row_stats<T, kThreads>(row, v.V, red, m, s);
-    if (threadIdx.x == 0) lp = logp_of(row, v.V, t, m, s);
+    row_stats<T, kThreads>(row, (int)v.V, red, m, s);
+    if (rank<kThreads>() == 0) lp = logp_of(row, (int)v.V, t, m, s);
   }
-  if (threadIdx.x == 0) {
-    stats[r] = make_float2(m, s);
-    if (logp) logp[r] = (float)lp;
-    if (logp64) logp64[r] = lp;
+  if (rank<kThreads>() == 0) {
+    out.stats[r] = make_float2(m, (float)s);
+    if (out.logp) out.logp[r] = (float)lp;
+    if (out.logp64) out.logp64[r] = lp;
+    if (out.g_row) out.g_row[r] = 0.f;
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(block_of<kThreads>())
     logp_bwd_kernel(const T* x, const int64_t* targets, const float2* stats, const float* g_row,
-                    const float* scale, T* dx, View v, int64_t dss, int64_t dst) {
-  const int64_t r = blockIdx.x, t = targets[r];
+                    const float* scale, T* dx, View v, int64_t dss, int64_t dst, uint32_t N) {
+  const uint32_t r = row_of<kThreads>();
+  if (kThreads == 32 && r >= N) return;
+  const int64_t t = targets[r];
   T* drow = dx + row_offset(r, v.T, dss, dst);
   const float2 ms = stats[r];
   float g = t < 0 ? 0.f : g_row[r];
@@ -210,9 +403,10 @@ __global__ void __launch_bounds__(kThreads)
   // a zero factor (an ignored token, a clipped one) makes a zero row, which needs no
   // logits - unless they hold a NaN or an infinity, which the sum then shows
   if (t < 0 || (g == 0.f && isfinite(ms.x) && isfinite(ms.y)))
-    write_zeros<T, kThreads>(drow, v.V);
+    write_zeros<T, kThreads>(drow, (int)v.V);
   else
-    write_grad<T, kThreads>(x + row_offset(r, v.T, v.ss, v.st), drow, v.V, t, ms.x, ms.y, g);
+    write_grad<T, kThreads>(x + row_offset(r, v.T, v.ss, v.st), drow, (int)v.V, t, ms.x,
+                            -g / ms.y, g);
 }
 
 // Per-row terms of the policy loss.  In all of it NaN arguments give NaN results.
@@ -227,8 +421,8 @@ struct Policy {
 };
 
 // term: {-min(ratio A, held A), KL, 1 if the held one counts}; returns d loss / d logp.
-__device__ double policy_terms(const Policy& p, int64_t r, int64_t T, double lp, double* term) {
-  const int64_t a = p.by_seq ? (p.seq ? p.seq[r] : r / T) : r;
+__device__ double policy_terms(const Policy& p, uint32_t r, int64_t T, double lp, double* term) {
+  const uint32_t a = p.by_seq ? (p.seq ? (uint32_t)p.seq[r] : r / (uint32_t)T) : r;
   const double A = p.adv[a];
   const double ratio = p.old_logp ? exp(lp - (double)p.old_logp[r]) : exp(lp - lp);
   const double kept = ratio < p.lo ? p.lo : ratio > p.hi ? p.hi : ratio;
@@ -246,50 +440,63 @@ __device__ double policy_terms(const Policy& p, int64_t r, int64_t T, double lp,
   return d;
 }
 
-// One row of the policy loss: log-probability, terms and d loss / d logp; with dx,
-// also the row's gradient times `scale`, the row read again where it is still in L2.
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    policy_kernel(const T* x, const int64_t* targets, Policy p, float* logp, float2* stats,
-                  float* g_row, double* terms, T* dx, float scale, View v, int64_t dss,
-                  int64_t dst, int64_t N) {
-  __shared__ float red[64];
-  __shared__ float bcast;
-  const int64_t r = blockIdx.x, t = targets[r];
+
+// One row of the policy loss: log-probability, terms and d loss / d logp; with dx, also the
+// row's gradient times `scale`, the row read again where it is still in L2.
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(block_of<kThreads>())
+    policy_kernel(const T* x, const int64_t* targets, Policy p, RowOut out, double* terms, T* dx,
+                  float scale, View v, int64_t dss, int64_t dst, uint32_t N) {
+  __shared__ Part red[32];
+  __shared__ float3 known;
+  const uint32_t r = row_of<kThreads>();
+  if (kThreads == 32 && r >= N) return;
+  const int64_t t = targets[r];
+  const int me = rank<kThreads>(), V = (int)v.V;
   const float w = p.weight[r];
   T* drow = dx ? dx + row_offset(r, v.T, dss, dst) : nullptr;
   if (t < 0 || w == 0.f) {
-    if (threadIdx.x == 0) {
-      if (logp) logp[r] = 0.f;
-      if (stats) stats[r] = make_float2(0.f, 1.f);
-      if (g_row) g_row[r] = 0.f;
-      terms[r] = terms[N + r] = terms[2 * N + r] = 0.0;
+    if (me == 0) {
+      out.logp[r] = 0.f;
+      if (out.stats) out.stats[r] = make_float2(0.f, 1.f);
+      if (out.g_row) out.g_row[r] = 0.f;
+      terms[r] = terms[(size_t)N + r] = terms[2 * (size_t)N + r] = 0.0;
     }
-    if (dx) write_zeros<T, kThreads>(drow, v.V);
+    if (dx) write_zeros<T, kThreads>(drow, V);
     return;
   }
   const T* row = x + row_offset(r, v.T, v.ss, v.st);
-  float m, s;
-  row_stats<T, kThreads>(row, v.V, red, m, s);
-  if (threadIdx.x == 0) {
+  float m = 0.f;
+  double s = 1.0;
+  row_stats<T, kThreads>(row, V, red, m, s);
+  float3 f;  // m, -g / s (0: a zero row) and g
+  if (me == 0) {
     double term[3];
-    const double lp = logp_of(row, v.V, t, m, s);
+    const double lp = logp_of(row, V, t, m, s);
     const float g = (float)(policy_terms(p, r, v.T, lp, term) * (double)w);
-    if (logp) logp[r] = (float)lp;
-    if (stats) stats[r] = make_float2(m, s);
-    if (g_row) g_row[r] = g;
+    out.logp[r] = (float)lp;
+    if (out.stats) out.stats[r] = make_float2(m, (float)s);
+    if (out.g_row) out.g_row[r] = g;
     terms[r] = term[0];
-    terms[N + r] = term[1];
-    terms[2 * N + r] = term[2];
-    bcast = g * scale;
+    terms[(size_t)N + r] = term[1];
+    terms[2 * (size_t)N + r] = term[2];
+    const float gs = g * scale;
+    f = make_float3(m, gs == 0.f && isfinite(m) && isfinite(s) ? 0.f : -gs / (float)s, gs);
+    if (kThreads > 32) known = f;
   }
   if (!dx) return;
-  __syncthreads();
-  const float g = bcast;
-  if (g == 0.f && isfinite(m) && isfinite(s))
-    write_zeros<T, kThreads>(drow, v.V);
+  if constexpr (kThreads == 32) {
+    f.x = __shfl_sync(0xffffffffu, f.x, 0);
+    f.y = __shfl_sync(0xffffffffu, f.y, 0);
+    f.z = __shfl_sync(0xffffffffu, f.z, 0);
+  } else {
+    __syncthreads();
+    f = known;
+  }
+  if (f.y == 0.f && f.z == 0.f)
+    write_zeros<T, kThreads>(drow, V);
   else
-    write_grad<T, kThreads>(row, drow, v.V, t, m, s, g);
+    write_grad<T, kThreads>(row, drow, V, t, f.x, f.y, f.z);
 }
 
 // ---- sequences ------------------------------------------------------------------
@@ -374,76 +581,109 @@ constexpr int kWeightThreads = 1024;
 // batch (-1 for a row outside every sequence).  One CTA: the counts of all sequences
 // are needed before the first weight, and 64K targets are 512 KB.
 __global__ void __launch_bounds__(kWeightThreads)
-    policy_weights_kernel(const int64_t* targets, const int64_t* cu, int64_t S, int64_t T,
-                          int64_t N, bool per_sequence, int32_t* counts, float* weight,
+    policy_weights_kernel(const int64_t* targets, const int64_t* cu, uint32_t S, uint32_t T,
+                          uint32_t N, bool per_sequence, uint32_t* counts, float* weight,
                           int32_t* seq) {
   __shared__ double red[32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int64_t s = warp; s < S; s += kWeightThreads / 32) {
-    int64_t a, b;
-    rows_of(cu, s, T, N, a, b);
-    int n = 0;
-    for (int64_t r = a + lane; r < b; r += 32) n += targets[r] >= 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    if (lane == 0) counts[s] = n;
+  for (uint32_t s = threadIdx.x; s < S; s += kWeightThreads) counts[s] = 0;
+  __syncthreads();
+  auto sequence = [&](uint32_t r) -> uint32_t {  // S for none
+    if (!cu) return r / T;
+    uint32_t lo = 0, hi = S;  // the first s with cu[s + 1] > r
+    while (lo < hi) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (cu[mid + 1] <= (int64_t)r)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    return lo < S && cu[lo] <= (int64_t)r ? lo : S;
+  };
+  for (uint32_t base = 0; base < N; base += kWeightThreads) {
+    const uint32_t r = base + threadIdx.x;
+    const uint32_t s = r < N ? sequence(r) : S;
+    if (seq && r < N) seq[r] = s < S ? (int32_t)s : -1;
+    const bool counted = s < S && targets[r] >= 0;
+    // whole numbers: their order does not show.  Most warps lie in one sequence.
+    const uint32_t s0 = __shfl_sync(0xffffffffu, s, 0);
+    if (__all_sync(0xffffffffu, s == s0)) {
+      const uint32_t n = __popc(__ballot_sync(0xffffffffu, counted));
+      if ((threadIdx.x & 31) == 0 && n) atomicAdd(&counts[s0], n);
+    } else if (counted) {
+      atomicAdd(&counts[s], 1u);
+    }
   }
   __syncthreads();
   double total = 0.0;
-  for (int64_t s = threadIdx.x; s < S; s += kWeightThreads)
-    total += per_sequence ? (counts[s] > 0 ? 1.0 : 0.0) : (double)counts[s];
-  total = block_sum(total, red);  // whole numbers: exact
-  for (int64_t r = threadIdx.x; r < N; r += kWeightThreads) {
-    int64_t s = r / (T > 0 ? T : 1);
-    bool inside = true;
-    if (cu) {  // the last s with cu[s] <= r
-      int64_t lo = 0, hi = S;
-      while (lo < hi) {
-        const int64_t mid = (lo + hi) / 2;
-        if (cu[mid + 1] <= r)
-          lo = mid + 1;
-        else
-          hi = mid;
-      }
-      s = lo;
-      inside = s < S && cu[s] <= r;
-      seq[r] = inside ? (int32_t)s : -1;
-    }
+  for (uint32_t s = threadIdx.x; s < S; s += kWeightThreads) {
+    const uint32_t n = *reinterpret_cast<volatile uint32_t*>(&counts[s]);
+    total += per_sequence ? (n > 0 ? 1.0 : 0.0) : (double)n;
+  }
+  total = block_sum(total, red);
+  for (uint32_t r = threadIdx.x; r < N; r += kWeightThreads) {
+    const uint32_t s = seq ? (uint32_t)seq[r] : r / T;  // -1 is beyond S
     float w = 0.f;
-    if (inside && targets[r] >= 0)
-      w = (float)(1.0 / (per_sequence ? total * (double)counts[s] : total));
+    if (s < S && targets[r] >= 0)
+      w = (float)(1.0 / (per_sequence
+                             ? total * (double)*reinterpret_cast<volatile uint32_t*>(&counts[s])
+                             : total));
     weight[r] = w;
   }
 }
 
-// loss = sum of weight * (policy term + kl_coef * KL); stats: policy term, KL and
+// loss = sum of weight * (policy term + kl_coef * KL); statistics: policy term, KL and
 // clipped share, each so weighted.
 __global__ void __launch_bounds__(kWeightThreads)
-    policy_sum_kernel(const double* terms, const float* weight, int64_t N, double kl_coef,
-                      float* loss, float* stats) {
+    policy_sum_kernel(const double* terms, const float* weight, uint32_t N, double kl_coef,
+                      float* loss, float* statistics) {
   __shared__ double red[32];
   double v[3] = {0.0, 0.0, 0.0};
-  for (int64_t r = threadIdx.x; r < N; r += kWeightThreads) {
+  for (uint32_t r = threadIdx.x; r < N; r += kWeightThreads) {
     const double w = weight[r];
     if (w != 0.0)
 #pragma unroll
-      for (int k = 0; k < 3; ++k) v[k] += w * terms[k * N + r];
+      for (int k = 0; k < 3; ++k) v[k] += w * terms[k * (size_t)N + r];
   }
 #pragma unroll
   for (int k = 0; k < 3; ++k) v[k] = block_sum(v[k], red);
   if (threadIdx.x == 0) {
     *loss = (float)(v[0] + (kl_coef != 0.0 ? kl_coef * v[1] : 0.0));
-    for (int k = 0; k < 3; ++k) stats[k] = (float)v[k];
+    for (int k = 0; k < 3; ++k) statistics[k] = (float)v[k];
   }
 }
 
 int elt_of(int dtype) { return dtype == SQB_BF16 ? 2 : dtype == SQB_F32 ? 4 : 0; }
 
 bool dims_ok(int64_t S, int64_t T, int64_t V) {
-  return S > 0 && T > 0 && V > 0 && S <= INT32_MAX && T <= INT32_MAX / S;
+  return S > 0 && T > 0 && V > 0 && V <= (1 << 30) && S <= INT32_MAX && T <= INT32_MAX / S;
 }
 
 int launched() { return cudaGetLastError() == cudaSuccess ? SQB_OK : SQB_ERR_LAUNCH; }
+
+// Calls f(type, threads, grid) for the rows' type and width.
+template <typename F>
+void dispatch(int dtype, int64_t N, int64_t V, F&& f) {
+  const unsigned rows = (unsigned)N, packed = (unsigned)((N + kWarpRows - 1) / kWarpRows);
+  const bool warp = V * elt_of(dtype) <= kWarpRowBytes;
+  using W = std::integral_constant<int, 32>;
+  using B = std::integral_constant<int, kRowThreads>;
+  if (dtype == SQB_BF16)
+    warp ? f(__nv_bfloat16(), W(), packed) : f(__nv_bfloat16(), B(), rows);
+  else
+    warp ? f(float(), W(), packed) : f(float(), B(), rows);
+}
+
+void launch_logp(const void* x, const int64_t* targets, const RowOut& out, int64_t S, int64_t T,
+                 int64_t V, int64_t ss, int64_t st, int dtype, cudaStream_t q) {
+  dispatch(dtype, S * T, V, [&](auto type, auto threads, unsigned grid) {
+    using X = decltype(type);
+    constexpr int kThreads = decltype(threads)::value;
+    logp_fwd_kernel<X, kThreads><<<grid, block_of<kThreads>(), 0, q>>>(
+        static_cast<const X*>(x), targets, out, View{T, V, ss, st}, (uint32_t)(S * T));
+  });
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
 }  // namespace logits
@@ -451,21 +691,13 @@ int launched() { return cudaGetLastError() == cudaSuccess ? SQB_OK : SQB_ERR_LAU
 
 using namespace sqb::logits;
 
-extern "C" int sqb_logp_fwd(const void* logits, const int64_t* targets, float* logp,
-                            double* logp_double, float* stats, int64_t S, int64_t T, int64_t V,
-                            int64_t ss, int64_t st, int dtype, void* stream) {
-  if (!logits || !targets || !stats || !dims_ok(S, T, V)) return SQB_ERR_ARG;
+extern "C" int sqb_logp_fwd(const void* logits, const int64_t* targets, float* logp, float* stats,
+                            int64_t S, int64_t T, int64_t V, int64_t ss, int64_t st, int dtype,
+                            void* stream) {
+  if (!logits || !targets || !logp || !stats || !dims_ok(S, T, V)) return SQB_ERR_ARG;
   if (!elt_of(dtype)) return SQB_ERR_DTYPE;
-  cudaStream_t q = static_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)(S * T);
-  const View v{T, V, ss, st};
-  float2* ms = reinterpret_cast<float2*>(stats);
-  if (dtype == SQB_BF16)
-    logp_fwd_kernel<<<grid, kThreads, 0, q>>>(static_cast<const __nv_bfloat16*>(logits), targets,
-                                              logp, logp_double, ms, v);
-  else
-    logp_fwd_kernel<<<grid, kThreads, 0, q>>>(static_cast<const float*>(logits), targets, logp,
-                                              logp_double, ms, v);
+  const RowOut out{logp, nullptr, reinterpret_cast<float2*>(stats), nullptr};
+  launch_logp(logits, targets, out, S, T, V, ss, st, dtype, static_cast<cudaStream_t>(stream));
   return launched();
 }
 
@@ -476,79 +708,91 @@ extern "C" int sqb_logp_bwd(const void* logits, const int64_t* targets, const fl
   if (!logits || !targets || !stats || !g_row || !dlogits || !dims_ok(S, T, V))
     return SQB_ERR_ARG;
   if (!elt_of(dtype)) return SQB_ERR_DTYPE;
-  cudaStream_t q = static_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)(S * T);
-  const View v{T, V, ss, st};
-  const float2* ms = reinterpret_cast<const float2*>(stats);
-  if (dtype == SQB_BF16)
-    logp_bwd_kernel<<<grid, kThreads, 0, q>>>(static_cast<const __nv_bfloat16*>(logits), targets,
-                                              ms, g_row, scale,
-                                              static_cast<__nv_bfloat16*>(dlogits), v, dss, dst);
-  else
-    logp_bwd_kernel<<<grid, kThreads, 0, q>>>(static_cast<const float*>(logits), targets, ms,
-                                              g_row, scale, static_cast<float*>(dlogits), v, dss,
-                                              dst);
+  dispatch(dtype, S * T, V, [&](auto type, auto threads, unsigned grid) {
+    using X = decltype(type);
+    constexpr int kThreads = decltype(threads)::value;
+    logp_bwd_kernel<X, kThreads>
+        <<<grid, block_of<kThreads>(), 0, static_cast<cudaStream_t>(stream)>>>(
+            static_cast<const X*>(logits), targets, reinterpret_cast<const float2*>(stats), g_row,
+            scale, static_cast<X*>(dlogits), View{T, V, ss, st}, dss, dst, (uint32_t)(S * T));
+  });
   return launched();
 }
 
-extern "C" int sqb_preference_finish(const double* logp, const int64_t* cu_seqlens,
-                                     const float* ref_logps, int64_t P, int64_t T, int64_t N,
-                                     double beta, double label_smoothing, double* pair_loss,
-                                     float* loss, float* rewards, float* g_row, void* stream) {
-  if (!pair_loss || !loss || !rewards || P <= 0 || P > INT32_MAX / 2 || N < 0 || T < 0)
+extern "C" size_t sqb_preference_workspace_bytes(int64_t N, int64_t P) {
+  if (N < 0 || P <= 0) return 0;
+  return align256((size_t)N * sizeof(double)) + (size_t)P * sizeof(double);
+}
+
+extern "C" int sqb_preference_fwd(const void* logits, const int64_t* targets,
+                                  const int64_t* cu_seqlens, const float* ref_logps, int64_t P,
+                                  double beta, double label_smoothing, float* loss,
+                                  float* rewards, float* stats, float* g_row, int64_t S,
+                                  int64_t T, int64_t V, int64_t ss, int64_t st, int dtype,
+                                  void* workspace, size_t ws_bytes, void* stream) {
+  if (!loss || !rewards || P <= 0 || P > INT32_MAX / 2 || S <= 0 || T < 0) return SQB_ERR_ARG;
+  if (T > 0 && (!logits || !targets || !stats || !g_row || !dims_ok(S, T, V)))
     return SQB_ERR_ARG;
-  if (N > 0 && (!logp || !g_row)) return SQB_ERR_ARG;
-  if (!cu_seqlens && (T == 0 ? N != 0 : N / T != 2 * P || N % T != 0)) return SQB_ERR_ARG;
+  if (cu_seqlens ? S != 1 : S != 2 * P) return SQB_ERR_ARG;
+  if (!elt_of(dtype)) return SQB_ERR_DTYPE;
+  const int64_t N = S * T;
+  if (!workspace || ws_bytes < sqb_preference_workspace_bytes(N, P)) return SQB_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) % sizeof(double)) return SQB_ERR_ALIGN;
   cudaStream_t q = static_cast<cudaStream_t>(stream);
-  preference_pair_kernel<<<(unsigned)P, kSeqThreads, 0, q>>>(
-      logp, cu_seqlens, ref_logps, P, T, N, beta, label_smoothing, pair_loss, rewards, g_row);
+  double* logp = static_cast<double*>(workspace);
+  double* pair_loss = logp + align256((size_t)N * sizeof(double)) / sizeof(double);
+  // rows of a packed batch that belong to no sequence keep the zero written here
+  const RowOut out{nullptr, logp, reinterpret_cast<float2*>(stats), cu_seqlens ? g_row : nullptr};
+  if (N > 0) launch_logp(logits, targets, out, S, T, V, ss, st, dtype, q);
+  preference_pair_kernel<<<(unsigned)P, kSeqThreads, 0, q>>>(logp, cu_seqlens, ref_logps, P, T, N,
+                                                             beta, label_smoothing, pair_loss,
+                                                             rewards, g_row);
   preference_mean_kernel<<<1, kSeqThreads, 0, q>>>(pair_loss, P, loss);
   return launched();
 }
 
-extern "C" int sqb_policy_weights(const int64_t* targets, const int64_t* cu_seqlens, int64_t S,
-                                  int64_t T, int64_t N, int per_sequence, int32_t* counts,
-                                  float* weight, int32_t* row_seq, void* stream) {
-  if (!targets || !counts || !weight || S <= 0 || S > INT32_MAX || N <= 0 || N > INT32_MAX ||
-      T < 0 || (cu_seqlens && !row_seq))
+extern "C" size_t sqb_policy_workspace_bytes(int64_t N, int64_t seqs) {
+  if (N <= 0 || seqs <= 0) return 0;
+  return align256((size_t)N * 3 * sizeof(double)) +
+         ((size_t)N * 2 + (size_t)seqs) * sizeof(float);
+}
+
+extern "C" int sqb_policy_fwd(const void* logits, const int64_t* targets,
+                              const int64_t* cu_seqlens, int64_t seqs, const float* old_logp,
+                              const float* ref_logp, const float* adv, int adv_by_seq,
+                              double clip_low, double clip_high, double kl_coef,
+                              int per_sequence, float* loss, float* statistics, float* logp,
+                              float* stats, float* g_row, void* dlogits, float grad_scale,
+                              int64_t S, int64_t T, int64_t V, int64_t ss, int64_t st,
+                              int64_t dss, int64_t dst, int dtype, void* workspace,
+                              size_t ws_bytes, void* stream) {
+  if (!logits || !targets || !adv || !loss || !statistics || !logp || !dims_ok(S, T, V) ||
+      seqs <= 0 || seqs > INT32_MAX || (cu_seqlens ? S != 1 : S != seqs))
     return SQB_ERR_ARG;
-  if (!cu_seqlens && (T == 0 || N / T != S || N % T != 0)) return SQB_ERR_ARG;
-  policy_weights_kernel<<<1, kWeightThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-      targets, cu_seqlens, S, T, N, per_sequence != 0, counts, weight, row_seq);
-  return launched();
-}
-
-extern "C" int sqb_policy_rows(const void* logits, const int64_t* targets, const float* old_logp,
-                               const float* ref_logp, const float* adv, int adv_by_seq,
-                               const int32_t* row_seq, const float* weight, double clip_low,
-                               double clip_high, double kl_coef, float* logp, float* stats,
-                               float* g_row, double* terms, void* dlogits, float grad_scale,
-                               int64_t S, int64_t T, int64_t V, int64_t ss, int64_t st,
-                               int64_t dss, int64_t dst, int dtype, void* stream) {
-  if (!logits || !targets || !adv || !weight || !terms || !dims_ok(S, T, V)) return SQB_ERR_ARG;
   if (!elt_of(dtype)) return SQB_ERR_DTYPE;
-  cudaStream_t q = static_cast<cudaStream_t>(stream);
   const int64_t N = S * T;
-  const View v{T, V, ss, st};
-  const Policy p{old_logp, ref_logp,       adv,           row_seq,        weight,
+  if (!workspace || ws_bytes < sqb_policy_workspace_bytes(N, seqs)) return SQB_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) % sizeof(double)) return SQB_ERR_ALIGN;
+  cudaStream_t q = static_cast<cudaStream_t>(stream);
+  double* terms = static_cast<double*>(workspace);
+  float* weight = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                           align256((size_t)N * 3 * sizeof(double)));
+  int32_t* seq = reinterpret_cast<int32_t*>(weight + N);
+  uint32_t* counts = reinterpret_cast<uint32_t*>(seq + N);
+  policy_weights_kernel<<<1, kWeightThreads, 0, q>>>(targets, cu_seqlens, (uint32_t)seqs,
+                                                     (uint32_t)T, (uint32_t)N, per_sequence != 0,
+                                                     counts, weight, cu_seqlens ? seq : nullptr);
+  const Policy p{old_logp,        ref_logp,       adv,    cu_seqlens ? seq : nullptr, weight,
                  adv_by_seq != 0, 1.0 - clip_low, 1.0 + clip_high, kl_coef};
-  float2* ms = reinterpret_cast<float2*>(stats);
-  if (dtype == SQB_BF16)
-    policy_kernel<<<(unsigned)N, kThreads, 0, q>>>(
-        static_cast<const __nv_bfloat16*>(logits), targets, p, logp, ms, g_row, terms,
-        static_cast<__nv_bfloat16*>(dlogits), grad_scale, v, dss, dst, N);
-  else
-    policy_kernel<<<(unsigned)N, kThreads, 0, q>>>(static_cast<const float*>(logits), targets, p,
-                                                   logp, ms, g_row, terms,
-                                                   static_cast<float*>(dlogits), grad_scale, v,
-                                                   dss, dst, N);
-  return launched();
-}
-
-extern "C" int sqb_policy_finish(const double* terms, const float* weight, int64_t N,
-                                 double kl_coef, float* loss, float* stats, void* stream) {
-  if (!terms || !weight || !loss || !stats || N <= 0 || N > INT32_MAX) return SQB_ERR_ARG;
-  policy_sum_kernel<<<1, kWeightThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-      terms, weight, N, kl_coef, loss, stats);
+  const RowOut out{logp, nullptr, reinterpret_cast<float2*>(stats), g_row};
+  dispatch(dtype, N, V, [&](auto type, auto threads, unsigned grid) {
+    using X = decltype(type);
+    constexpr int kThreads = decltype(threads)::value;
+    policy_kernel<X, kThreads><<<grid, block_of<kThreads>(), 0, q>>>(
+        static_cast<const X*>(logits), targets, p, out, terms, static_cast<X*>(dlogits),
+        grad_scale, View{T, V, ss, st}, dss, dst, (uint32_t)N);
+  });
+  policy_sum_kernel<<<1, kWeightThreads, 0, q>>>(terms, weight, (uint32_t)N, kl_coef, loss,
+                                                 statistics);
   return launched();
 }

@@ -24,6 +24,7 @@ from . import _lib
 __all__ = ["token_log_probs", "preference_loss", "policy_loss", "policy_loss_and_grad"]
 
 _DTYPES = {torch.float32: _lib.SQB_F32, torch.bfloat16: _lib.SQB_BF16}
+_INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 
 def _ptr(t):
@@ -46,52 +47,74 @@ def _grad_like(x):
     return buf.as_strided(x.shape, x.stride(), phase)
 
 
-# ---- custom ops: x (S, T, V), t (S, T) int64 contiguous -----------------------------
+# ---- the operators --------------------------------------------------------------------
+# x is (S, T, V), or (N, V) as one sequence; t int64, contiguous, one target a row.  Each
+# has a function that launches it, registered as a custom op for traced calls and wrapped in
+# an autograd function, with the same backward, for eager ones.
 
 
-def _launch_logp(x, t, logp, logp64, stats):
-    S, T, V = x.shape
-    if S * T == 0:
-        return
-    _lib.check("sqb_logp_fwd", _lib.lib().sqb_logp_fwd(
-        x.data_ptr(), t.data_ptr(), _ptr(logp), _ptr(logp64), stats.data_ptr(), S, T, V,
-        x.stride(0), x.stride(1), _DTYPES[x.dtype], _stream(x)))
+def _dims(x):
+    """(S, T, V, sequence stride, token stride)"""
+    if x.dim() == 2:
+        return (1, *x.shape, 0, x.stride(0))
+    return (*x.shape, x.stride(0), x.stride(1))
 
 
-@torch.library.custom_op("sqrtblock::logp_fwd", mutates_args=())
-def _logp_fwd(x: torch.Tensor, t: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """(logp (S, T), row statistics (S, T, 2): max and sum of exp(x - max))."""
+def _run(raw, op, function, x, *args):
+    if not _lib.plain(x):
+        return op(x, *args)
+    if x.requires_grad and torch.is_grad_enabled():
+        return function.apply(x, *args)
+    return raw(x, *args)
+
+
+def _logp_fwd_raw(x: torch.Tensor, t: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(logp in t's shape, row statistics (2 S T,))."""
+    S, T, V, ss, st = _dims(x)
     logp = torch.empty(t.shape, dtype=torch.float32, device=x.device)
-    stats = torch.empty((*t.shape, 2), dtype=torch.float32, device=x.device)
-    with _lib.on_device(x.device):
-        _launch_logp(x, t, logp, None, stats)
+    stats = torch.empty(2 * S * T, dtype=torch.float32, device=x.device)
+    if S * T:
+        with _lib.on_device(x.device):
+            _lib.check("sqb_logp_fwd", _lib.lib().sqb_logp_fwd(
+                x.data_ptr(), t.data_ptr(), logp.data_ptr(), stats.data_ptr(), S, T, V, ss, st,
+                _DTYPES[x.dtype], _stream(x)))
     return logp, stats
+
+
+_logp_fwd = torch.library.custom_op("sqrtblock::logp_fwd", _logp_fwd_raw, mutates_args=())
 
 
 @_logp_fwd.register_fake
 def _(x, t):
     return (x.new_empty(t.shape, dtype=torch.float32),
-            x.new_empty((*t.shape, 2), dtype=torch.float32))
+            x.new_empty(2 * t.numel(), dtype=torch.float32))
 
 
-@torch.library.custom_op("sqrtblock::logp_bwd", mutates_args=())
-def _logp_bwd(x: torch.Tensor, t: torch.Tensor, stats: torch.Tensor, g_row: torch.Tensor,
-              scale: Optional[torch.Tensor]) -> torch.Tensor:
-    """g_row[r] * scale * ([c == t] - softmax) in x's dtype and strides."""
-    S, T, V = x.shape
+def _logp_bwd_raw(x: torch.Tensor, t: torch.Tensor, stats: torch.Tensor,
+                  g_row: Optional[torch.Tensor], scale: Optional[torch.Tensor]) -> torch.Tensor:
+    """g_row[r] * scale * ([c == t] - softmax) in x's dtype and strides; without a g_row the
+    factors follow the row statistics."""
+    S, T, V, ss, st = _dims(x)
     dx = _grad_like(x)
     if S * T:
+        g = g_row.data_ptr() if g_row is not None else stats.data_ptr() + 8 * S * T
         with _lib.on_device(x.device):
             _lib.check("sqb_logp_bwd", _lib.lib().sqb_logp_bwd(
-                x.data_ptr(), t.data_ptr(), stats.data_ptr(), g_row.data_ptr(), _ptr(scale),
-                dx.data_ptr(), S, T, V, x.stride(0), x.stride(1), dx.stride(0), dx.stride(1),
-                _DTYPES[x.dtype], _stream(x)))
+                x.data_ptr(), t.data_ptr(), stats.data_ptr(), g, _ptr(scale), dx.data_ptr(), S,
+                T, V, ss, st, ss, st, _DTYPES[x.dtype], _stream(x)))
     return dx
+
+
+_logp_bwd = torch.library.custom_op("sqrtblock::logp_bwd", _logp_bwd_raw, mutates_args=())
 
 
 @_logp_bwd.register_fake
 def _(x, t, stats, g_row, scale):
     return torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=x.device)
+
+
+def _rows_grad(x, *args):
+    return (_logp_bwd_raw if _lib.plain(x) else _logp_bwd)(x, *args)
 
 
 def _logp_setup(ctx, inputs, output):
@@ -101,163 +124,188 @@ def _logp_setup(ctx, inputs, output):
 
 def _logp_grad(ctx, dlogp, _dstats):
     x, t, stats = ctx.saved_tensors
-    return _logp_bwd(x, t, stats, dlogp.to(torch.float32).contiguous(), None), None
+    return _rows_grad(x, t, stats, dlogp.to(torch.float32).contiguous(), None), None
 
 
 _logp_fwd.register_autograd(_logp_grad, setup_context=_logp_setup)
 
 
-@torch.library.custom_op("sqrtblock::preference_fwd", mutates_args=())
-def _preference_fwd(x: torch.Tensor, t: torch.Tensor, ref: Optional[torch.Tensor],
+class _LogP(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *args):
+        out = _logp_fwd_raw(*args)
+        _logp_setup(ctx, args, out)
+        return out
+
+    backward = staticmethod(_logp_grad)
+
+
+def _preference_raw(x: torch.Tensor, t: torch.Tensor, ref: Optional[torch.Tensor],
                     cu: Optional[torch.Tensor], pairs: int, beta: float, label_smoothing: float
-                    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(loss, rewards (2, P), row statistics, d loss / d logp of each row)."""
-    S, T, V = x.shape
-    dev = x.device
-    f32, f64 = torch.float32, torch.float64
-    logp = torch.empty(t.shape, dtype=f64, device=dev)
-    stats = torch.empty((*t.shape, 2), dtype=f32, device=dev)
-    # rows of a packed batch that belong to no sequence keep a zero
-    g_row = (torch.empty if cu is None else torch.zeros)(t.shape, dtype=f32, device=dev)
+                    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(loss, rewards (2, P), row statistics and d loss / d logp of each row (3 S T,))."""
+    S, T, V, ss, st = _dims(x)
+    dev, N, f32 = x.device, S * T, torch.float32
     loss = torch.empty((), dtype=f32, device=dev)
     rewards = torch.empty((2, pairs), dtype=f32, device=dev)
-    pair_loss = torch.empty(pairs, dtype=f64, device=dev)
+    rows = torch.empty(3 * N, dtype=f32, device=dev)
+    lib = _lib.lib()
+    nbytes = lib.sqb_preference_workspace_bytes(N, pairs)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    at = rows.data_ptr()
     with _lib.on_device(dev):
-        _launch_logp(x, t, None, logp, stats)
-        _lib.check("sqb_preference_finish", _lib.lib().sqb_preference_finish(
-            _ptr(logp), _ptr(cu), _ptr(ref), pairs, T, S * T, beta, label_smoothing,
-            pair_loss.data_ptr(), loss.data_ptr(), rewards.data_ptr(), _ptr(g_row), _stream(x)))
-    return loss, rewards, stats, g_row
+        _lib.check("sqb_preference_fwd", lib.sqb_preference_fwd(
+            x.data_ptr(), t.data_ptr(), _ptr(cu), _ptr(ref), pairs, beta, label_smoothing,
+            loss.data_ptr(), rewards.data_ptr(), at, at + 8 * N, S, T, V, ss, st,
+            _DTYPES[x.dtype], ws.data_ptr(), nbytes, _stream(x)))
+    return loss, rewards, rows
+
+
+_preference_fwd = torch.library.custom_op("sqrtblock::preference_fwd", _preference_raw,
+                                          mutates_args=())
 
 
 @_preference_fwd.register_fake
 def _(x, t, ref, cu, pairs, beta, label_smoothing):
     f32 = torch.float32
     return (x.new_empty((), dtype=f32), x.new_empty((2, pairs), dtype=f32),
-            x.new_empty((*t.shape, 2), dtype=f32), x.new_empty(t.shape, dtype=f32))
-
-
-def _preference_setup(ctx, inputs, output):
-    x, t = inputs[:2]
-    _, rewards, stats, g_row = output
-    ctx.save_for_backward(x, t, stats, g_row)
-    ctx.mark_non_differentiable(rewards, stats, g_row)
+            x.new_empty(3 * t.numel(), dtype=f32))
 
 
 def _loss_grad(ctx, dloss):
-    x, t, stats, g_row = ctx.saved_tensors
-    return _logp_bwd(x, t, stats, g_row, dloss.to(torch.float32).reshape(1))
+    x, t, rows = ctx.saved_tensors
+    return _rows_grad(x, t, rows, None, dloss.to(torch.float32))
+
+
+def _preference_setup(ctx, inputs, output):
+    _, rewards, rows = output
+    ctx.save_for_backward(*inputs[:2], rows)
+    ctx.mark_non_differentiable(rewards, rows)
+    ctx.set_materialize_grads(False)
 
 
 def _preference_grad(ctx, dloss, *_):
-    return _loss_grad(ctx, dloss), None, None, None, None, None, None
+    if dloss is None:
+        return (None,) * 7
+    return (_loss_grad(ctx, dloss),) + (None,) * 6
 
 
 _preference_fwd.register_autograd(_preference_grad, setup_context=_preference_setup)
 
 
-@torch.library.custom_op("sqrtblock::policy_fwd", mutates_args=())
-def _policy_fwd(x: torch.Tensor, t: torch.Tensor, adv: torch.Tensor,
+class _Preference(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *args):
+        out = _preference_raw(*args)
+        _preference_setup(ctx, args, out)
+        return out
+
+    backward = staticmethod(_preference_grad)
+
+
+def _policy_raw(x: torch.Tensor, t: torch.Tensor, adv: torch.Tensor,
                 old: Optional[torch.Tensor], ref: Optional[torch.Tensor],
                 cu: Optional[torch.Tensor], seqs: int, adv_by_seq: bool, per_seq: bool,
                 clip_low: float, clip_high: float, kl_coef: float, grad_scale: Optional[float]
-                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
-                           torch.Tensor]:
-    """(loss, logps, (policy term, KL, clipped share), row statistics, d loss / d logp of
-    each row, the logits' gradient times grad_scale - empty for None)."""
-    S, T, V = x.shape
-    dev, N = x.device, S * T
-    f32, i32 = torch.float32, torch.int32
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(loss, logps, (policy term, KL, clipped share), last): `last` is the logits' gradient
+    times grad_scale, or for None the row statistics and d loss / d logp (3 S T,)."""
+    S, T, V, ss, st = _dims(x)
+    dev, N, f32 = x.device, S * T, torch.float32
     logps = torch.empty(t.shape, dtype=f32, device=dev)
-    rowstats = torch.empty((*t.shape, 2), dtype=f32, device=dev)
-    g_row = torch.empty(t.shape, dtype=f32, device=dev)
     loss = torch.empty((), dtype=f32, device=dev)
-    stats = torch.empty(3, dtype=f32, device=dev)
-    dx = _grad_like(x) if grad_scale is not None else torch.empty(0, dtype=x.dtype, device=dev)
+    statistics = torch.empty(3, dtype=f32, device=dev)
+    fused = grad_scale is not None
+    last = _grad_like(x) if fused else torch.empty(3 * N, dtype=f32, device=dev)
     if N == 0:
-        return loss.zero_(), logps, stats.zero_(), rowstats, g_row, dx
-    terms = torch.empty((3, N), dtype=torch.float64, device=dev)
-    weight = torch.empty(N, dtype=f32, device=dev)
-    counts = torch.empty(seqs, dtype=i32, device=dev)
-    row_seq = torch.empty(N, dtype=i32, device=dev) if cu is not None else None
-    lib, stream = _lib.lib(), _stream(x)
+        return loss.zero_(), logps, statistics.zero_(), last
+    lib = _lib.lib()
+    nbytes = lib.sqb_policy_workspace_bytes(N, seqs)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    at = last.data_ptr()
     with _lib.on_device(dev):
-        _lib.check("sqb_policy_weights", lib.sqb_policy_weights(
-            t.data_ptr(), _ptr(cu), seqs, T, N, int(per_seq), counts.data_ptr(),
-            weight.data_ptr(), _ptr(row_seq), stream))
-        _lib.check("sqb_policy_rows", lib.sqb_policy_rows(
-            x.data_ptr(), t.data_ptr(), _ptr(old), _ptr(ref), adv.data_ptr(), int(adv_by_seq),
-            _ptr(row_seq), weight.data_ptr(), clip_low, clip_high, kl_coef, logps.data_ptr(),
-            rowstats.data_ptr(), g_row.data_ptr(), terms.data_ptr(),
-            dx.data_ptr() if grad_scale is not None else None,
-            1.0 if grad_scale is None else grad_scale, S, T, V, x.stride(0), x.stride(1),
-            x.stride(0), x.stride(1), _DTYPES[x.dtype], stream))
-        _lib.check("sqb_policy_finish", lib.sqb_policy_finish(
-            terms.data_ptr(), weight.data_ptr(), N, kl_coef, loss.data_ptr(), stats.data_ptr(),
-            stream))
-    return loss, logps, stats, rowstats, g_row, dx
+        _lib.check("sqb_policy_fwd", lib.sqb_policy_fwd(
+            x.data_ptr(), t.data_ptr(), _ptr(cu), seqs, _ptr(old), _ptr(ref), adv.data_ptr(),
+            adv_by_seq, clip_low, clip_high, kl_coef, per_seq, loss.data_ptr(),
+            statistics.data_ptr(), logps.data_ptr(), None if fused else at,
+            None if fused else at + 8 * N, at if fused else None, grad_scale if fused else 1.0,
+            S, T, V, ss, st, ss, st, _DTYPES[x.dtype], ws.data_ptr(), nbytes, _stream(x)))
+    return loss, logps, statistics, last
+
+
+_policy_fwd = torch.library.custom_op("sqrtblock::policy_fwd", _policy_raw, mutates_args=())
 
 
 @_policy_fwd.register_fake
 def _(x, t, adv, old, ref, cu, seqs, adv_by_seq, per_seq, clip_low, clip_high, kl_coef,
       grad_scale):
     f32 = torch.float32
-    dx = (torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=x.device)
-          if grad_scale is not None else x.new_empty(0))
+    last = (torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=x.device)
+            if grad_scale is not None else x.new_empty(3 * t.numel(), dtype=f32))
     return (x.new_empty((), dtype=f32), x.new_empty(t.shape, dtype=f32),
-            x.new_empty(3, dtype=f32), x.new_empty((*t.shape, 2), dtype=f32),
-            x.new_empty(t.shape, dtype=f32), dx)
+            x.new_empty(3, dtype=f32), last)
 
 
 def _policy_setup(ctx, inputs, output):
-    x, t = inputs[:2]
-    _, logps, stats, rowstats, g_row, dx = output
-    ctx.save_for_backward(x, t, rowstats, g_row)
-    ctx.mark_non_differentiable(logps, stats, rowstats, g_row, dx)
+    _, logps, statistics, last = output
+    ctx.save_for_backward(*inputs[:2], last)
+    ctx.mark_non_differentiable(logps, statistics, last)
+    ctx.set_materialize_grads(False)
 
 
 def _policy_grad(ctx, dloss, *_):
+    if dloss is None:
+        return (None,) * 13
     return (_loss_grad(ctx, dloss),) + (None,) * 12
 
 
 _policy_fwd.register_autograd(_policy_grad, setup_context=_policy_setup)
 
 
+class _Policy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *args):
+        out = _policy_raw(*args)
+        _policy_setup(ctx, args, out)
+        return out
+
+    backward = staticmethod(_policy_grad)
+
+
 # ---- public entry points --------------------------------------------------------------
 
 
 def _disjoint(x):
-    """Whether the rows of x (S, T, V), unit stride on V, occupy different memory."""
-    (S, T, V), (ss, st, _) = x.shape, x.stride()
+    """Whether the rows of x, unit stride on V, occupy different memory."""
+    S, T, V, ss, st = _dims(x)
     if S <= 1 or T <= 1:
         return (S <= 1 or ss >= V) and (T <= 1 or st >= V)
     return (st >= V and ss >= (T - 1) * st + V) or (ss >= V and st >= (S - 1) * ss + V)
 
 
 def _rows(fn, logits, targets):
-    """Logits as (S, T, V) and targets as (S, T) int64, checked."""
+    """Logits as (S, T, V) or (N, V) and int64 targets, checked."""
     if not logits.is_cuda:
         raise RuntimeError(f"{fn}: logits must be a CUDA tensor (the op has no CPU "
                            "implementation)")
     if logits.dtype not in _DTYPES:
         raise TypeError(f"{fn} supports float32 and bfloat16 logits, got {logits.dtype}")
-    if logits.dim() < 2 or logits.shape[-1] == 0:
-        raise ValueError(f"{fn}: logits must be (..., tokens, V), got {tuple(logits.shape)}")
-    if targets.shape != logits.shape[:-1] or targets.device != logits.device:
+    shape = logits.shape
+    if len(shape) < 2 or shape[-1] == 0:
+        raise ValueError(f"{fn}: logits must be (..., tokens, V), got {tuple(shape)}")
+    if targets.shape != shape[:-1] or targets.device != logits.device:
         raise ValueError(f"{fn}: one target per row of logits on their device, got targets "
-                         f"{tuple(targets.shape)} for logits {tuple(logits.shape)}")
-    if targets.dtype.is_floating_point or targets.dtype.is_complex or targets.dtype == torch.bool:
+                         f"{tuple(targets.shape)} for logits {tuple(shape)}")
+    if targets.dtype not in _INTEGERS:
         raise TypeError(f"{fn}: targets must be integers, got {targets.dtype}")
-    V = logits.shape[-1]
-    x = logits
-    if x.dim() != 3:
-        x = (x.unsqueeze(0) if x.dim() == 2
-             else x.reshape(math.prod(x.shape[:-2]), x.shape[-2], V))
-    if x.shape[0] * x.shape[1] > 2**31 - 1:
-        raise ValueError(f"{fn}: at most 2**31 - 1 rows of logits")
-    if (x.stride(2) != 1 and V > 1) or not _disjoint(x):
+    x, t = logits, targets
+    if len(shape) > 3:
+        x = x.reshape(math.prod(shape[:-2]), *shape[-2:])
+    if t.numel() > 2**31 - 1 or shape[-1] > 2**30:
+        raise ValueError(f"{fn}: at most 2**31 - 1 rows of at most 2**30 logits")
+    if (x.stride(-1) != 1 and shape[-1] > 1) or not _disjoint(x):
         x = x.contiguous()
-    return x, targets.to(torch.int64).reshape(x.shape[:2]).contiguous()
+    return x, t.to(torch.int64).contiguous()
 
 
 def _sequences(fn, logits, targets, cu_seqlens):
@@ -306,7 +354,7 @@ def token_log_probs(logits, targets):
     (``sqrtblock::logp_fwd/bwd``): one read of the logits forward, and one read and one
     write backward, with no softmax kept in between."""
     x, t = _rows("token_log_probs", logits, targets)
-    return _logp_fwd(x, t)[0].view(targets.shape)
+    return _run(_logp_fwd_raw, _logp_fwd, _LogP, x, t)[0]
 
 
 def preference_loss(logits, targets, ref_logps=None, *, beta=0.1, label_smoothing=0.0,
@@ -330,8 +378,9 @@ def preference_loss(logits, targets, ref_logps=None, *, beta=0.1, label_smoothin
     ref = _given(fn, "ref_logps", ref_logps, [(seqs,)], x.device)
     beta = _number(fn, "beta", beta, most=1e30)
     label_smoothing = _number(fn, "label_smoothing", label_smoothing, most=1.0)
-    loss, rewards, _, _ = _preference_fwd(x, t, ref, cu, seqs // 2, beta, label_smoothing)
-    return loss, rewards[0], rewards[1]
+    loss, rewards, _ = _run(_preference_raw, _preference_fwd, _Preference, x, t, ref, cu,
+                            seqs // 2, beta, label_smoothing)
+    return (loss, *rewards.unbind(0))
 
 
 def _policy_args(fn, logits, targets, advantages, old_logps, ref_logps, clip, clip_high, kl_coef,
@@ -381,8 +430,8 @@ def policy_loss(logits, targets, advantages, old_logps=None, ref_logps=None, *, 
     loss - are for logging and for the next step's ``old_logps``, not differentiable."""
     args = _policy_args("policy_loss", logits, targets, advantages, old_logps, ref_logps, clip,
                         clip_high, kl_coef, reduction, cu_seqlens)
-    loss, logps, stats, _, _, _ = _policy_fwd(*args, None)
-    return loss, logps.view(targets.shape), stats
+    loss, logps, stats, _ = _run(_policy_raw, _policy_fwd, _Policy, *args, None)
+    return loss, logps, stats
 
 
 def policy_loss_and_grad(logits, targets, advantages, old_logps=None, ref_logps=None, *,
@@ -401,5 +450,5 @@ def policy_loss_and_grad(logits, targets, advantages, old_logps=None, ref_logps=
     grad_scale = float(grad_scale)
     if not math.isfinite(grad_scale):
         raise ValueError(f"{fn}: grad_scale must be finite, got {grad_scale}")
-    loss, logps, stats, _, _, dx = _policy_fwd(*args, grad_scale)
-    return loss, dx[0] if logits.dim() == 2 else dx, logps.view(targets.shape), stats
+    loss, logps, stats, dx = _run(_policy_raw, _policy_fwd, _Policy, *args, grad_scale)
+    return loss, dx, logps, stats

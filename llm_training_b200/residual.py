@@ -20,54 +20,55 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-@torch.library.custom_op("sqrtblock::residual_norm_fwd", mutates_args=())
-def _fwd(x: torch.Tensor, h: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor],
-         wp: Optional[torch.Tensor], bp: Optional[torch.Tensor], gate: Optional[torch.Tensor],
-         scale: float, eps: float, rms: bool, out_dtype: torch.dtype
-         ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """Rows x, h (N, C), gate (G, C) or None -> (x' (N, C), y (N, C), row statistics)."""
-    N, C = x.shape
+def _fwd_raw(x: torch.Tensor, h: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor],
+             wp: Optional[torch.Tensor], bp: Optional[torch.Tensor],
+             gate: Optional[torch.Tensor], scale: float, eps: float, rms: bool,
+             out_dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Contiguous x, h (..., C) and gate (... , C), each of its rows shared by as many rows
+    of x in turn -> (x', y, row statistics)."""
+    C = x.shape[-1]
+    N = x.numel() // C
     xo = torch.empty_like(x)
-    y = torch.empty((N, C), dtype=out_dtype, device=x.device)
-    stats = torch.empty((N, 4), dtype=torch.float32, device=x.device)
+    y = torch.empty_like(x, dtype=out_dtype)
+    stats = torch.empty(4 * N, dtype=torch.float32, device=x.device)
     if N:
         with _lib.on_device(x.device):
             _lib.check("sqb_residual_norm_fwd", _lib.lib().sqb_residual_norm_fwd(
                 x.data_ptr(), _DTYPES[x.dtype], h.data_ptr(), _DTYPES[h.dtype], w.data_ptr(),
-                _ptr(b), _ptr(wp), _ptr(bp), _ptr(gate), gate.shape[0] if gate is not None else 0,
-                scale, eps, int(rms), xo.data_ptr(), y.data_ptr(), _DTYPES[out_dtype],
-                stats.data_ptr(), N, C, torch.cuda.current_stream(x.device).cuda_stream))
+                _ptr(b), _ptr(wp), _ptr(bp), _ptr(gate),
+                gate.numel() // C if gate is not None else 0, scale, eps, rms, xo.data_ptr(),
+                y.data_ptr(), _DTYPES[out_dtype], stats.data_ptr(), N, C,
+                torch.cuda.current_stream(x.device).cuda_stream))
     return xo, y, stats
+
+
+_fwd = torch.library.custom_op("sqrtblock::residual_norm_fwd", _fwd_raw, mutates_args=())
 
 
 @_fwd.register_fake
 def _(x, h, w, b, wp, bp, gate, scale, eps, rms, out_dtype):
-    N, C = x.shape
-    return (x.new_empty((N, C)), x.new_empty((N, C), dtype=out_dtype),
-            x.new_empty((N, 4), dtype=torch.float32))
+    return (torch.empty_like(x), torch.empty_like(x, dtype=out_dtype),
+            x.new_empty(4 * (x.numel() // x.shape[-1]), dtype=torch.float32))
 
 
-@torch.library.custom_op("sqrtblock::residual_norm_bwd", mutates_args=())
-def _bwd(dy: torch.Tensor, dxo: Optional[torch.Tensor], x: torch.Tensor, h: torch.Tensor,
-         w: torch.Tensor, b: Optional[torch.Tensor], wp: Optional[torch.Tensor],
-         bp: Optional[torch.Tensor], gate: Optional[torch.Tensor], scale: float, eps: float,
-         rms: bool, stats: torch.Tensor
-         ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
-                    torch.Tensor, torch.Tensor]:
-    """(dx, dh, dw, db, dwp, dbp, dgate), empty for a parameter that is not there."""
-    N, C = x.shape
-    gates = gate.shape[0] if gate is not None else 0
+def _bwd_raw(dy: torch.Tensor, dxo: Optional[torch.Tensor], x: torch.Tensor, h: torch.Tensor,
+             w: torch.Tensor, b: Optional[torch.Tensor], wp: Optional[torch.Tensor],
+             bp: Optional[torch.Tensor], gate: Optional[torch.Tensor], scale: float, eps: float,
+             rms: bool, stats: torch.Tensor
+             ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dh, the gradients of w, b, wp, bp and gate - those that are there - end to end)."""
+    C = x.shape[-1]
+    N = x.numel() // C
+    sizes = [p.numel() if p is not None else 0 for p in (w, b, wp, bp, gate)]
     dx, dh = torch.empty_like(x), torch.empty_like(h)
-
-    def grad_of(p, *shape):
-        return torch.empty(shape if p is not None else 0, dtype=torch.float32, device=x.device)
-
-    dw, db, dwp, dbp = grad_of(w, C), grad_of(b, C), grad_of(wp, C), grad_of(bp, C)
-    dgate = grad_of(gate, gates, C)
+    dp = torch.empty(sum(sizes), dtype=torch.float32, device=x.device)
     if N == 0:
-        for g in (dw, db, dwp, dbp, dgate):
-            g.zero_()
-        return dx, dh, dw, db, dwp, dbp, dgate
+        return dx, dh, dp.zero_()
+    at, ptrs = dp.data_ptr(), []
+    for n in sizes:
+        ptrs.append(at if n else None)
+        at += 4 * n
+    gates = sizes[4] // C
     lib = _lib.lib()
     nbytes = lib.sqb_residual_norm_workspace_bytes(N, C, gates)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
@@ -75,26 +76,25 @@ def _bwd(dy: torch.Tensor, dxo: Optional[torch.Tensor], x: torch.Tensor, h: torc
         _lib.check("sqb_residual_norm_bwd", lib.sqb_residual_norm_bwd(
             dy.data_ptr(), _DTYPES[dy.dtype], _ptr(dxo), x.data_ptr(), _DTYPES[x.dtype],
             h.data_ptr(), _DTYPES[h.dtype], w.data_ptr(), _ptr(b), _ptr(wp), _ptr(bp),
-            _ptr(gate), gates, scale, eps, int(rms), stats.data_ptr(), dx.data_ptr(),
-            dh.data_ptr(), dw.data_ptr(), _ptr(db), _ptr(dwp), _ptr(dbp), _ptr(dgate),
-            ws.data_ptr(), nbytes, N, C, torch.cuda.current_stream(x.device).cuda_stream))
-    return dx, dh, dw, db, dwp, dbp, dgate
+            _ptr(gate), gates, scale, eps, rms, stats.data_ptr(), dx.data_ptr(), dh.data_ptr(),
+            *ptrs, ws.data_ptr(), nbytes, N, C,
+            torch.cuda.current_stream(x.device).cuda_stream))
+    return dx, dh, dp
+
+
+_bwd = torch.library.custom_op("sqrtblock::residual_norm_bwd", _bwd_raw, mutates_args=())
 
 
 @_bwd.register_fake
 def _(dy, dxo, x, h, w, b, wp, bp, gate, scale, eps, rms, stats):
-    def grad_of(p):
-        return x.new_empty(p.shape if p is not None else 0, dtype=torch.float32)
-
-    return (torch.empty_like(x), torch.empty_like(h), grad_of(w), grad_of(b), grad_of(wp),
-            grad_of(bp), grad_of(gate))
+    n = sum(p.numel() for p in (w, b, wp, bp, gate) if p is not None)
+    return torch.empty_like(x), torch.empty_like(h), x.new_empty(n, dtype=torch.float32)
 
 
 def _setup(ctx, inputs, output):
-    x, h, w, b, wp, bp, gate, scale, eps, rms, _ = inputs
-    xo, y, stats = output
-    ctx.save_for_backward(x, h, w, b, wp, bp, gate, stats)
-    ctx.cfg = (scale, eps, rms)
+    _, y, stats = output
+    ctx.save_for_backward(*inputs[:7], stats)
+    ctx.cfg = inputs[7:10]
     ctx.y_dtype = y.dtype
     ctx.mark_non_differentiable(stats)
     ctx.set_materialize_grads(False)
@@ -107,14 +107,40 @@ def _grad(ctx, dxo, dy, _dstats):
     if dy is None:
         dy = torch.zeros(x.shape, dtype=ctx.y_dtype, device=x.device)
     dxo = dxo.contiguous() if dxo is not None else None
-    dx, dh, dw, db, dwp, dbp, dgate = _bwd(dy.contiguous(), dxo, x, h, w, b, wp, bp, gate,
-                                           *ctx.cfg, stats)
-    given = (dw, db if b is not None else None, dwp if wp is not None else None,
-             dbp if bp is not None else None, dgate if gate is not None else None)
+    dx, dh, dp = (_bwd_raw if _lib.plain(x) else _bwd)(
+        dy.contiguous(), dxo, x, h, w, b, wp, bp, gate, *ctx.cfg, stats)
+    given, at = [], 0
+    for p in (w, b, wp, bp, gate):
+        if p is None:
+            given.append(None)
+        else:
+            given.append(dp[at:at + p.numel()])
+            at += p.numel()
+    if gate is not None and gate.dim() > 1:
+        given[4] = given[4].view(gate.shape)
     return (dx, dh, *given, None, None, None, None)
 
 
 _fwd.register_autograd(_grad, setup_context=_setup)
+
+
+class _Residual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *args):
+        out = _fwd_raw(*args)
+        _setup(ctx, args, out)
+        return out
+
+    backward = staticmethod(_grad)
+
+
+def _run(*args):
+    """An eager call skips the dispatcher, a traced one is the custom op."""
+    if not _lib.plain(args[0]):
+        return _fwd(*args)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:7]):
+        return _Residual.apply(*args)
+    return _fwd_raw(*args)
 
 
 def _param(name, p, shape, device):
@@ -127,21 +153,19 @@ def _param(name, p, shape, device):
 
 
 def _gates(gate, x):
-    """The gate as (G, C) rows, each shared by N / G rows of x in turn."""
     if gate is None:
         return None
-    C = x.shape[-1]
+    C, B = x.shape[-1], x.shape[0]
     if gate.device != x.device or gate.dtype not in _DTYPES:
         raise ValueError("residual_norm: gate must be float32 or bfloat16 on x's device, got "
                          f"{gate.dtype}")
-    if tuple(gate.shape) == (C,):
-        return gate.float().reshape(1, C).contiguous()
-    one_per_sample = [(x.shape[0], *(1,) * (x.dim() - 2), C), (x.shape[0], C)]
-    if x.dim() >= 2 and tuple(gate.shape) in one_per_sample and 0 < x.shape[0] <= MAX_GATES:
-        return gate.float().reshape(x.shape[0], C).contiguous()
-    raise ValueError(f"residual_norm: gate must be (C,) or one row for each of the first "
-                     f"dimension's entries (at most {MAX_GATES}), got {tuple(gate.shape)} for x "
-                     f"{tuple(x.shape)}")
+    shape = tuple(gate.shape)
+    if shape != (C,) and (x.dim() < 2 or not 0 < B <= MAX_GATES
+                          or shape not in ((B, *(1,) * (x.dim() - 2), C), (B, C))):
+        raise ValueError(f"residual_norm: gate must be (C,) or one row for each of the first "
+                         f"dimension's entries (at most {MAX_GATES}), got {shape} for x "
+                         f"{tuple(x.shape)}")
+    return gate.float().contiguous()
 
 
 def residual_norm(x, h, weight, bias=None, *, post_weight=None, post_bias=None, gate=None,
@@ -186,6 +210,6 @@ def residual_norm(x, h, weight, bias=None, *, post_weight=None, post_bias=None, 
     w, b = (_param(n, p, (C,), x.device) for n, p in (("weight", weight), ("bias", bias)))
     wp, bp = (_param(n, p, (C,), x.device) for n, p in (("post_weight", post_weight),
                                                         ("post_bias", post_bias)))
-    xo, y, _ = _fwd(x.reshape(-1, C).contiguous(), h.reshape(-1, C).contiguous(), w, b, wp, bp,
-                    _gates(gate, x), scale, eps, kind == "rms", out_dtype)
-    return xo.view(x.shape), y.view(x.shape)
+    xo, y, _ = _run(x.contiguous(), h.contiguous(), w, b, wp, bp, _gates(gate, x), scale, eps,
+                    kind == "rms", out_dtype)
+    return xo, y

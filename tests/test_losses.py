@@ -4,11 +4,11 @@ CPU: refusals, argument checks of the C entry points, fake implementations.  GPU
 and gradients against the definition in 64 bits (log_softmax and autograd in float64),
 with bounds that count the roundings:
 
-* a row's sum s of exp(x - max) is added up in fp32 over V / threads terms a thread (at
+* a row's sum s of exp(x - m) is added up in fp32 over V / threads terms a thread (at
   most V / 32 + 8) and a tree of at most 10 levels; each exponential is off by two units
-  (2^-22) and by the rounding of its argument, |x - max| * 2^-23.  Terms further than 30
-  below the max weigh nothing, so relative error of s <= rel(V) below, and log s is off
-  by as much;
+  (2^-22) and by at most the rounding of its argument, |x - m| * 2^-23.  Terms further
+  than 30 below the maximum weigh nothing, so relative error of s <= rel(V) below, and
+  log s is off by as much;
 * a log-probability stored in fp32 is off by 2^-24 of itself more;
 * a gradient element g ([c == t] - exp / s) is off by rel(V) of g p, 2^-23 of g at the
   target (the sum) and, rounded to its type, by half a step: finfo.eps / 2."""
@@ -22,7 +22,7 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 
 from llm_training_b200 import _lib, ops
 
-ERR_ARG, ERR_DTYPE = 1, 2  # include/sqrtblock.h
+ERR_ARG, ERR_DTYPE, ERR_ALIGN, ERR_WORKSPACE = 1, 2, 3, 5  # include/sqrtblock.h
 U = 2.0**-24  # half a step of fp32, relative
 
 
@@ -92,19 +92,33 @@ def test_bad_arguments_are_refused():
 
 def test_c_entry_points_reject_bad_arguments_without_a_device():
     lib, p = _lib.lib(), ctypes.c_void_p(16)
-    assert lib.sqb_logp_fwd(None, p, p, p, p, 1, 4, 8, 32, 8, 1, None) == ERR_ARG
-    assert lib.sqb_logp_fwd(p, p, p, p, p, 0, 4, 8, 32, 8, 1, None) == ERR_ARG
-    assert lib.sqb_logp_fwd(p, p, p, p, p, 2**20, 2**12, 8, 32, 8, 1, None) == ERR_ARG
-    assert lib.sqb_logp_fwd(p, p, p, p, p, 1, 4, 8, 32, 8, 7, None) == ERR_DTYPE
+    assert lib.sqb_logp_fwd(None, p, p, p, 1, 4, 8, 32, 8, 1, None) == ERR_ARG
+    assert lib.sqb_logp_fwd(p, p, p, p, 0, 4, 8, 32, 8, 1, None) == ERR_ARG
+    assert lib.sqb_logp_fwd(p, p, p, p, 2**20, 2**12, 8, 32, 8, 1, None) == ERR_ARG
+    assert lib.sqb_logp_fwd(p, p, p, p, 1, 4, 2**31, 32, 8, 1, None) == ERR_ARG
+    assert lib.sqb_logp_fwd(p, p, p, p, 1, 4, 8, 32, 8, 7, None) == ERR_DTYPE
     assert lib.sqb_logp_bwd(p, p, p, None, p, p, 1, 4, 8, 32, 8, 32, 8, 1, None) == ERR_ARG
     assert lib.sqb_logp_bwd(p, p, p, p, p, p, 1, 4, 8, 32, 8, 32, 8, 9, None) == ERR_DTYPE
-    assert lib.sqb_preference_finish(p, None, p, 2, 4, 15, .1, 0., p, p, p, p, None) == ERR_ARG
-    assert lib.sqb_preference_finish(p, None, p, 0, 4, 0, .1, 0., p, p, p, p, None) == ERR_ARG
-    assert lib.sqb_policy_weights(p, p, 2, 0, 8, 0, p, p, None, None) == ERR_ARG
-    assert lib.sqb_policy_weights(p, None, 2, 3, 8, 0, p, p, None, None) == ERR_ARG
-    assert lib.sqb_policy_rows(p, p, None, None, None, 0, None, p, .2, .2, 0., p, p, p, p, None,
-                               1., 1, 4, 8, 32, 8, 32, 8, 1, None) == ERR_ARG
-    assert lib.sqb_policy_finish(p, p, 0, 0., p, p, None) == ERR_ARG
+
+    def preference(x=p, cu=None, P=2, S=4, T=3, dtype=1, ws=p, nbytes=1 << 20, loss=p):
+        return lib.sqb_preference_fwd(x, p, cu, p, P, .1, 0., loss, p, p, p, S, T, 8, 24, 8, dtype,
+                                      ws, nbytes, None)
+
+    assert preference(x=None) == ERR_ARG and preference(loss=None) == ERR_ARG
+    assert preference(P=0) == ERR_ARG and preference(P=3) == ERR_ARG and preference(T=-1) == ERR_ARG
+    assert preference(cu=p) == ERR_ARG and preference(dtype=4) == ERR_DTYPE
+    assert preference(ws=None) == ERR_WORKSPACE and preference(nbytes=64) == ERR_WORKSPACE
+    assert preference(ws=ctypes.c_void_p(20)) == ERR_ALIGN
+
+    def policy(adv=p, cu=None, seqs=4, S=4, dtype=1, ws=p, nbytes=1 << 20, logp=p):
+        return lib.sqb_policy_fwd(p, p, cu, seqs, None, None, adv, 1, .2, .2, 0., 0, p, p, logp, p,
+                                  p, None, 1., S, 3, 8, 24, 8, 24, 8, dtype, ws, nbytes, None)
+
+    assert policy(adv=None) == ERR_ARG and policy(logp=None) == ERR_ARG
+    assert policy(seqs=3) == ERR_ARG and policy(cu=p) == ERR_ARG and policy(seqs=0) == ERR_ARG
+    assert policy(dtype=4) == ERR_DTYPE
+    assert policy(ws=None) == ERR_WORKSPACE and policy(nbytes=64) == ERR_WORKSPACE
+    assert policy(ws=ctypes.c_void_p(20)) == ERR_ALIGN
 
 
 def test_fakes_keep_shapes_dtypes_and_strides():
