@@ -178,7 +178,7 @@ size_t sqb_residual_norm_workspace_bytes(int64_t N, int64_t C, int64_t gates);
 
 /* Backward from x, h and the forward's stats: dy (y_dtype), dx_out (x's dtype; NULL: 0)
  * -> dx, dh in x's and h's dtypes and the gradient of every parameter given (fp32,
- * overwritten; dgate (gates, C)), summed in a fixed order.  At most 65531 gates. */
+ * overwritten; dgate (gates, C)), summed in a fixed order.  At most 65530 gates. */
 int sqb_residual_norm_bwd(const void* dy, int y_dtype, const void* dx_out, const void* x,
                           int x_dtype, const void* h, int h_dtype, const float* weight,
                           const float* bias, const float* post_weight, const float* post_bias,

@@ -12,18 +12,17 @@
 //   d weight = sum dy x^, d bias = sum dy, d post weight = sum dn h^, d post bias = sum dn,
 //   d gate = sum scale D n over the rows that share the gate
 //
-// One CTA per row, the row in registers (E elements a thread).  Both norms' statistics
-// are saved; the backward forms x' again from x and h in fp32, so that a stream kept
-// in bf16 is not rounded between the two passes.  Variances are of differences from
-// the mean (two sweeps over registers), never E[v^2] - mean^2.  The backward's CTAs
-// each take a run of rows, keep their columns' sums in registers and write one partial
-// row; a second kernel adds the partials in a fixed order (bit-reproducible).
+// Both norms' statistics are saved; the backward forms x' again from x and h in fp32, so
+// that a stream kept in bf16 is not rounded between the two passes.  Variances are of
+// differences from the mean (two sweeps over registers), never E[v^2] - mean^2.
 // Bound by HBM for large batches: forward reads x, h and writes x', y; backward reads
 // x, h, dy, dx' and writes dx, dh.
 
 #include <cuda_bf16.h>
 #include <math.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "sqb_train.h"
 
@@ -32,301 +31,430 @@ namespace resnorm {
 namespace {
 
 constexpr int kMaxC = 4096;
-constexpr int kParts = 4;  // d weight, d bias, d post weight, d post bias
+constexpr int kParts = 5;  // d weight, d bias, d post weight, d post bias, d gate (if one)
 
 struct Args {
   const void *x, *h;
   const float *w, *b, *wp, *bp, *gate;
   float scale, eps;
-  int64_t N, T;  // rows, rows that share a gate (N for one gate)
+  uint32_t N, T;  // rows, rows that share a gate (N for one gate)
   int C;
-  bool rms, x_bf16, h_bf16, y_bf16;
+  bool rms;
 };
 
-// W consecutive elements of a row of either type, and their stores.
+template <typename T, int W>
+struct Raw;  // W elements as they lie in memory
+template <>
+struct Raw<float, 4> {
+  float4 v;
+};
+template <>
+struct Raw<__nv_bfloat16, 4> {
+  uint2 v;
+};
+template <>
+struct Raw<float, 1> {
+  float v;
+};
+template <>
+struct Raw<__nv_bfloat16, 1> {
+  __nv_bfloat16 v;
+};
+
+template <typename T, int W>
+__device__ __forceinline__ Raw<T, W> fetch(const T* p) {
+  return *reinterpret_cast<const Raw<T, W>*>(p);
+}
+__device__ __forceinline__ void unpack(Raw<float, 4> r, float* v) {
+  v[0] = r.v.x, v[1] = r.v.y, v[2] = r.v.z, v[3] = r.v.w;
+}
+__device__ __forceinline__ void unpack(Raw<__nv_bfloat16, 4> r, float* v) {
+  v[0] = __uint_as_float(r.v.x << 16), v[1] = __uint_as_float(r.v.x & 0xffff0000u);
+  v[2] = __uint_as_float(r.v.y << 16), v[3] = __uint_as_float(r.v.y & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack(Raw<float, 1> r, float* v) { v[0] = r.v; }
+__device__ __forceinline__ void unpack(Raw<__nv_bfloat16, 1> r, float* v) {
+  v[0] = __bfloat162float(r.v);
+}
+
 template <int W>
-__device__ __forceinline__ void load(const void* p, bool bf16, int64_t i, float* v) {
+__device__ __forceinline__ void store(float* p, const float* v) {
+  if constexpr (W == 4)
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else
+    p[0] = v[0];
+}
+template <int W>
+__device__ __forceinline__ void store(__nv_bfloat16* p, const float* v) {
   if constexpr (W == 4) {
-    if (bf16) {
-      const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + i);
-      const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
-      const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
-      v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
-    } else {
-      const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-    }
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]);
+    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a),
+                                              *reinterpret_cast<const uint32_t*>(&b));
   } else {
-    v[0] = bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i])
-                : static_cast<const float*>(p)[i];
+    p[0] = __float2bfloat16_rn(v[0]);
   }
 }
 
+// W parameters of columns c.., or `none` for a null p.
 template <int W>
-__device__ __forceinline__ void store(void* p, bool bf16, int64_t i, const float* v) {
-  if constexpr (W == 4) {
-    if (bf16) {
-      const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]);
-      const __nv_bfloat162 b = __floats2bfloat162_rn(v[2], v[3]);
-      uint2 u;
-      u.x = *reinterpret_cast<const uint32_t*>(&a);
-      u.y = *reinterpret_cast<const uint32_t*>(&b);
-      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p) + i) = u;
-    } else {
-      *reinterpret_cast<float4*>(static_cast<float*>(p) + i) =
-          make_float4(v[0], v[1], v[2], v[3]);
-    }
-  } else {
-    if (bf16)
-      static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v[0]);
-    else
-      static_cast<float*>(p)[i] = v[0];
+__device__ __forceinline__ void param(const float* p, int c, float none, float* v) {
+  if (p)
+    unpack(fetch<float, W>(p + c), v);
+  else
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[j] = none;
+}
+
+// ---- forward ------------------------------------------------------------------------
+//
+// kThreads threads hold a row, E = K * W elements each; a CTA of 256 threads takes
+// 256 / kThreads rows.  A warp for rows up to 1024 columns: its sums need no barrier, and
+// enough rows are in flight on an SM to keep HBM busy.
+
+constexpr int kFwdThreads = 256;
+
+// Sum over the row's threads, the same in all of them.  red: one float for each warp of the
+// CTA; each use of a buffer is followed by another's before its next.
+template <int kThreads>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (kThreads > 32) {
+    constexpr int kWarps = kThreads / 32;
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) red[warp] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) v += red[warp / kWarps * kWarps + i];
   }
+  return v;
 }
 
-// Column of the thread's k-th group of W elements.
-template <int W>
-__device__ __forceinline__ int column(int k) {
-  return (k * (int)blockDim.x + (int)threadIdx.x) * W;
-}
-
-// Sums of K values over the CTA, the same in every thread.  red: K * 32 floats; the
-// caller alternates two such buffers, so one barrier separates a buffer's uses.
-template <int K>
-__device__ __forceinline__ void block_sums(float* v, float* red) {
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-  const int warps = blockDim.x >> 5;
-  if (warps == 1) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0)
-#pragma unroll
-    for (int k = 0; k < K; ++k) red[k * 32 + warp] = v[k];
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    v[k] = lane < warps ? red[k * 32 + lane] : 0.f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-  }
-}
-
-// Mean (0 for RMS) and 1/std of a row held as v[E], columns past C excluded.
-template <int E, int W>
-__device__ __forceinline__ void moments(const float* v, const Args& a, float* red0, float* red1,
+template <int K, int W, int kThreads>
+__device__ __forceinline__ void moments(const float (&v)[K * W], const Args& a, int me, float* red,
                                         float& mean, float& rstd) {
   mean = 0.f;
   if (!a.rms) {
     float s = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += v[e];  // columns past C hold 0
-    block_sums<1>(&s, red0);
-    mean = s / a.C;
+    for (int e = 0; e < K * W; ++e) s += v[e];  // columns past C hold 0
+    mean = row_sum<kThreads>(s, red) / a.C;
   }
   float q = 0.f;
 #pragma unroll
-  for (int k = 0; k < E / W; ++k)
-    if (column<W>(k) < a.C)
+  for (int k = 0; k < K; ++k)
+    if ((k * kThreads + me) * W < a.C)
 #pragma unroll
       for (int j = 0; j < W; ++j) {
         const float d = v[k * W + j] - mean;
-        q += d * d;
+        q = fmaf(d, d, q);
       }
-  block_sums<1>(&q, red1);
-  rstd = rsqrtf(q / a.C + a.eps);
+  rstd = rsqrtf(row_sum<kThreads>(q, red + 8) / a.C + a.eps);
 }
 
-// scale * gate and the post norm's weight and bias for the thread's columns.
-template <int W>
-__device__ __forceinline__ void gate_of(const Args& a, const float* gate, int c, float* g) {
-  if (gate)
-    load<W>(gate, false, c, g);
-  else
+template <typename X, typename H, typename Y, int K, int W, int kThreads>
+__global__ void __launch_bounds__(kFwdThreads)
+    fwd_kernel(const Args a, X* xo, Y* y, float4* stats) {
+  __shared__ float red[32];
+  constexpr int kRows = kFwdThreads / kThreads;
+  const int me = threadIdx.x % kThreads;
+  const uint32_t r = blockIdx.x * kRows + threadIdx.x / kThreads;
+  const bool live = r < a.N;  // a row of the CTA may be past the end: it only takes barriers
+  if (kThreads == 32 && !live) return;
+  const size_t base = (size_t)(live ? r : 0) * a.C;
+  const X* xr = static_cast<const X*>(a.x) + base;
+  const H* hr = static_cast<const H*>(a.h) + base;
+  const float* gate = a.gate ? a.gate + (size_t)((live ? r : 0) / a.T) * a.C : nullptr;
+  Raw<X, W> xw[K];
+  Raw<H, W> hw[K];
 #pragma unroll
-    for (int j = 0; j < W; ++j) g[j] = 1.f;
-#pragma unroll
-  for (int j = 0; j < W; ++j) g[j] *= a.scale;
-}
-
-template <int E, int W>
-__global__ void __launch_bounds__(E == 4 ? 256 : 512) fwd_kernel(Args a, void* xo, void* y, float4* stats) {
-  __shared__ float red[4][32];
-  const int64_t r = blockIdx.x, base = r * a.C;
-  const float* gate = a.gate ? a.gate + (r / a.T) * a.C : nullptr;
-  float h[E], x[E];
-#pragma unroll
-  for (int k = 0; k < E / W; ++k) {
-    const int c = column<W>(k);
+  for (int k = 0; k < K; ++k) {
+    const int c = (k * kThreads + me) * W;
     if (c < a.C) {
-      load<W>(a.h, a.h_bf16, base + c, h + k * W);
-      load<W>(a.x, a.x_bf16, base + c, x + k * W);
+      hw[k] = fetch<H, W>(hr + c);
+      xw[k] = fetch<X, W>(xr + c);
+    }
+  }
+  float h[K * W], x[K * W];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if ((k * kThreads + me) * W < a.C) {
+      unpack(hw[k], h + k * W);
+      unpack(xw[k], x + k * W);
     } else {
 #pragma unroll
       for (int j = 0; j < W; ++j) h[k * W + j] = x[k * W + j] = 0.f;
     }
   }
   float mh = 0.f, rh = 1.f, mx, rx;
-  if (a.wp) moments<E, W>(h, a, red[0], red[1], mh, rh);
+  if (a.wp) moments<K, W, kThreads>(h, a, me, red, mh, rh);
 #pragma unroll
-  for (int k = 0; k < E / W; ++k) {
-    const int c = column<W>(k);
+  for (int k = 0; k < K; ++k) {
+    const int c = (k * kThreads + me) * W;
     if (c >= a.C) continue;
     float g[W], w[W], b[W];
-    gate_of<W>(a, gate, c, g);
-    if (a.wp) load<W>(a.wp, false, c, w);
-    if (a.bp) load<W>(a.bp, false, c, b);
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      float n = h[k * W + j];
-      if (a.wp) n = (n - mh) * rh * w[j] + (a.bp ? b[j] : 0.f);
-      x[k * W + j] += g[j] * n;
-    }
-    store<W>(xo, a.x_bf16, base + c, x + k * W);
-  }
-  moments<E, W>(x, a, red[2], red[3], mx, rx);
-#pragma unroll
-  for (int k = 0; k < E / W; ++k) {
-    const int c = column<W>(k);
-    if (c >= a.C) continue;
-    float w[W], b[W], o[W];
-    load<W>(a.w, false, c, w);
-    if (a.b) load<W>(a.b, false, c, b);
+    param<W>(gate, c, 1.f, g);
+    param<W>(a.wp, c, 1.f, w);
+    param<W>(a.bp, c, 0.f, b);
 #pragma unroll
     for (int j = 0; j < W; ++j)
-      o[j] = (x[k * W + j] - mx) * rx * w[j] + (a.b ? b[j] : 0.f);
-    store<W>(y, a.y_bf16, base + c, o);
+      x[k * W + j] += a.scale * g[j] * fmaf((h[k * W + j] - mh) * rh, w[j], b[j]);
+    if (live) store<W>(xo + base + c, x + k * W);
   }
-  if (threadIdx.x == 0) stats[r] = make_float4(mh, rh, mx, rx);
+  moments<K, W, kThreads>(x, a, me, red + 16, mx, rx);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (k * kThreads + me) * W;
+    if (c >= a.C) continue;
+    float w[W], b[W], o[W];
+    param<W>(a.w, c, 1.f, w);
+    param<W>(a.b, c, 0.f, b);
+#pragma unroll
+    for (int j = 0; j < W; ++j) o[j] = fmaf((x[k * W + j] - mx) * rx, w[j], b[j]);
+    if (live) store<W>(y + base + c, o);
+  }
+  if (live && me == 0) stats[r] = make_float4(mh, rh, mx, rx);
 }
 
-// CTA i takes rows [i * rows, (i + 1) * rows).  parts: (kParts, grid, C) column sums of
-// the CTAs; gate_parts: one row of C for each (CTA, gate) that meet, at slot
-// CTA + gate (each step along the rows raises one of the two, so no slot is shared).
-template <int E, int W>
-__global__ void __launch_bounds__(E == 4 ? 256 : 512) bwd_kernel(Args a, const void* dy, const void* dxo, const float4* stats, void* dx,
-                           void* dh, float* parts, float* gate_parts, int64_t rows) {
-  __shared__ float red[2][64];
-  const int64_t first = (int64_t)blockIdx.x * rows, last = min(first + rows, a.N);
-  float sw[E], sb[E], swp[E], sbp[E], sg[E];
+// ---- backward -----------------------------------------------------------------------
+//
+// G warps (1 to 8) hold a row, E columns a lane, each warp 32 E consecutive ones, and walk a
+// run of consecutive rows; the columns' sums (d weight and so on) stay in their registers
+// over the run.  A CTA is one such group, or eight groups of one warp; each CTA writes one
+// partial row of each (parts: (kParts, grid, pitch)), which a second kernel adds in a fixed
+// order (bit-reproducible).  A gate for each sample has its sums written where the gate
+// changes: one row for each (run, gate) that meet, at slot run + gate (each step along the
+// rows raises one of the two, so no slot is shared).
+// What binds it first is the issue of instructions, with 16 warps an SM to cover their
+// latencies: 25 for each element are the mathematics.  So a warp whose columns all exist
+// takes a path without a comparison for each, and no more is kept in registers than 16
+// warps of 128 have room for.
+
+constexpr int kBwdThreads = 256;  // at most
+
+// Sums of a pair over the G warps of a row, the same in all of them.  red: the group's,
+// member: this warp's place in it.
+__device__ __forceinline__ void pair_sums(float& u, float& v, float2* red, int G, int member) {
+  const int lane = threadIdx.x & 31;
+  const bool upper = lane & 16;  // the upper lanes go on with v
+  const float send = upper ? u : v;
+  float t = (upper ? v : u) + __shfl_xor_sync(0xffffffffu, send, 16);
 #pragma unroll
-  for (int e = 0; e < E; ++e) sw[e] = sb[e] = swp[e] = sbp[e] = sg[e] = 0.f;
-  for (int64_t r = first; r < last; ++r) {
-    const int64_t base = r * a.C, grp = r / a.T;
-    const float* gate = a.gate ? a.gate + grp * a.C : nullptr;
-    const float4 st = stats[r];
-    // D starts as u; hh and xh are the normalised rows
-    float D[E], xh[E], hh[E];
-    float s[2] = {0.f, 0.f};
+  for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if (G == 1) {
+    u = __shfl_sync(0xffffffffu, t, 0);
+    v = __shfl_sync(0xffffffffu, t, 16);
+    return;
+  }
+  if ((lane & 15) == 0) reinterpret_cast<float*>(red + member)[lane >> 4] = t;
+  // the CTA's barrier: its warps arrive from two places in the code
+  asm volatile("bar.sync 0;" ::: "memory");
+  u = v = 0.f;
+  for (int i = 0; i < G; ++i) {
+    const float2 p = red[i];
+    u += p.x, v += p.y;
+  }
+}
+
+template <int E>
+struct ColumnSums {
+  float w[E], b[E], wp[E], bp[E], g[E];
+};
+
+struct BwdArgs {
+  const float4* stats;
+  float *parts, *gate_parts;
+  int pitch, G;
+  uint32_t rows;
+};
+
+// Rows [first, last) of one warp, whose lanes' columns start at c0.  kFull: all of them exist.
+template <typename X, typename H, typename Y, int E, int W, bool kBias, bool kFull>
+__device__ __forceinline__ void bwd_rows(const Args& a, const BwdArgs& p, const Y* dy,
+                                         const X* dxo, X* dx, H* dh, ColumnSums<E>& sum,
+                                         float2* red, uint32_t run, uint32_t first, uint32_t last,
+                                         int c0, int member) {
+  constexpr int K = E / W, kStep = 32 * W;
+  constexpr bool kKeep = E == 8 && !kBias;  // the gate and post weight in registers
+  const int C = a.C;
+  auto on = [&](int k) { return kFull || c0 + k * kStep < C; };
+  const float inv = 1.f / C, mean_inv = a.rms ? 0.f : inv;
+  float w[W], bp[W], wp[kKeep ? E : W], gw[kKeep ? E : W];
+  auto load_wp = [&](int k, int i) { param<W>(on(k) ? a.wp : nullptr, c0 + k * kStep, 1.f, wp + i); };
+  auto load_gate = [&](const float* gate, int k, int i) {
+    param<W>(on(k) ? gate : nullptr, c0 + k * kStep, 1.f, gw + i);
 #pragma unroll
-    for (int k = 0; k < E / W; ++k) {
-      const int c = column<W>(k);
-      if (c < a.C) {
-        float g[W], w[W], wp[W], bp[W];
-        load<W>(a.h, a.h_bf16, base + c, hh + k * W);
-        load<W>(a.x, a.x_bf16, base + c, xh + k * W);
-        load<W>(dy, a.y_bf16, base + c, D + k * W);
-        load<W>(a.w, false, c, w);
-        gate_of<W>(a, gate, c, g);
-        if (a.wp) load<W>(a.wp, false, c, wp);
-        if (a.bp) load<W>(a.bp, false, c, bp);
+    for (int j = 0; j < W; ++j) gw[i + j] *= a.scale;
+  };
+  uint32_t grp = first / a.T, turn = (grp + 1) * a.T;  // the gate, and the row where it ends
+  const float* gate = a.gate ? a.gate + (size_t)grp * C : nullptr;
+  if (kKeep)
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-          const int e = k * W + j;
-          float n = hh[e];
-          if (a.wp) {
-            hh[e] = (n - st.x) * st.y;
-            n = hh[e] * wp[j] + (a.bp ? bp[j] : 0.f);
-          }
-          xh[e] = (xh[e] + g[j] * n - st.z) * st.w;
-          sw[e] += D[e] * xh[e];
-          sb[e] += D[e];
-          D[e] *= w[j];
-          s[0] += D[e];
-          s[1] += D[e] * xh[e];
-        }
-      } else {
+    for (int k = 0; k < K; ++k) {
+      load_wp(k, k * W);
+      load_gate(gate, k, k * W);
+    }
+  int flip = 0;
+  for (uint32_t r = first; r < last; ++r) {
+    const size_t base = (size_t)r * C + c0;
+    const X* xr = static_cast<const X*>(a.x) + base;
+    const H* hr = static_cast<const H*>(a.h) + base;
+    const Y* yr = dy + base;
+    const X* ur = dxo + base;
+    Raw<X, W> xw[K], uw[K];
+    Raw<H, W> hw[K];
+    Raw<Y, W> yw[K];
 #pragma unroll
-        for (int j = 0; j < W; ++j) D[k * W + j] = xh[k * W + j] = hh[k * W + j] = 0.f;
+    for (int k = 0; k < K; ++k) {
+      const int i = on(k) ? k * kStep : -c0;  // a column that is not there: the row's first
+      hw[k] = fetch<H, W>(hr + i);
+      xw[k] = fetch<X, W>(xr + i);
+      yw[k] = fetch<Y, W>(yr + i);
+      if (dxo) uw[k] = fetch<X, W>(ur + i);
+    }
+    const float4 st = p.stats[r];
+    if (r == turn) {
+      ++grp, turn += a.T;
+      if (a.gate) {
+        gate += C;
+        if (kKeep)
+#pragma unroll
+          for (int k = 0; k < K; ++k) load_gate(gate, k, k * W);
       }
     }
-    block_sums<2>(s, red[0]);
-    const float mu = a.rms ? 0.f : s[0] / a.C, mux = s[1] / a.C;
-    float q[2] = {0.f, 0.f};
+    const float mh = -st.x * st.y, mx = -st.z * st.w;
+    float D[E], xh[E], hh[E], s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;  // D is u
 #pragma unroll
-    for (int k = 0; k < E / W; ++k) {
-      const int c = column<W>(k);
-      if (c >= a.C) continue;
-      float up[W], g[W], wp[W], bp[W];
+    for (int k = 0; k < K; ++k) {
+      const int i = kKeep ? k * W : 0;
+      if (!kKeep) load_wp(k, 0), load_gate(gate, k, 0);
+      param<W>(on(k) ? a.w : nullptr, c0 + k * kStep, 0.f, w);
+      param<W>(kBias && on(k) ? a.bp : nullptr, c0 + k * kStep, 0.f, bp);
+      unpack(hw[k], hh + k * W);
+      unpack(xw[k], xh + k * W);
+      unpack(yw[k], D + k * W);
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const int e = k * W + j;
+        hh[e] = fmaf(hh[e], st.y, mh);  // h itself without a post norm
+        xh[e] = fmaf(fmaf(gw[i + j], fmaf(hh[e], wp[i + j], bp[j]), xh[e]), st.w, mx);
+        if (!on(k)) D[e] = xh[e] = hh[e] = 0.f;
+        sum.w[e] = fmaf(D[e], xh[e], sum.w[e]);
+        if (kBias) sum.b[e] += D[e];
+        D[e] *= w[j];
+        (e & 1 ? t0 : s0) += D[e];
+        float& s = e & 1 ? t1 : s1;
+        s = fmaf(D[e], xh[e], s);
+      }
+    }
+    s0 += t0, s1 += t1;
+    pair_sums(s0, s1, red + flip * 8, p.G, member);
+    flip ^= 1;
+    const float k0 = -st.w * (s0 * mean_inv), k1 = -s1 * inv;
+    float q0 = 0.f, q1 = 0.f;
+    t0 = t1 = 0.f;
+    X* dxr = dx + base;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int i = kKeep ? k * W : 0;
+      float d[W];
       if (dxo)
-        load<W>(dxo, a.x_bf16, base + c, up);
+        unpack(uw[k], d);
       else
 #pragma unroll
-        for (int j = 0; j < W; ++j) up[j] = 0.f;
-      gate_of<W>(a, gate, c, g);
-      if (a.wp) load<W>(a.wp, false, c, wp);
-      if (a.bp) load<W>(a.bp, false, c, bp);
+        for (int j = 0; j < W; ++j) d[j] = 0.f;
+      if (!kKeep) load_wp(k, 0), load_gate(gate, k, 0);
+      param<W>(kBias && on(k) ? a.bp : nullptr, c0 + k * kStep, 0.f, bp);
 #pragma unroll
       for (int j = 0; j < W; ++j) {
         const int e = k * W + j;
-        up[j] += st.w * (D[e] - mu - xh[e] * mux);
-        const float n = a.wp ? hh[e] * wp[j] + (a.bp ? bp[j] : 0.f) : hh[e];
-        sg[e] += up[j] * n;
-        const float dn = up[j] * g[j];
-        swp[e] += dn * hh[e];
-        sbp[e] += dn;
-        D[e] = a.wp ? dn * wp[j] : dn;
-        q[0] += D[e];
-        q[1] += D[e] * hh[e];
+        d[j] += fmaf(st.w, fmaf(xh[e], k1, D[e]), k0);
+        if (!on(k)) d[j] = 0.f;
+        sum.g[e] = fmaf(d[j], fmaf(hh[e], wp[i + j], bp[j]), sum.g[e]);
+        const float dn = d[j] * gw[i + j];
+        sum.wp[e] = fmaf(dn, hh[e], sum.wp[e]);
+        if (kBias) sum.bp[e] += dn;
+        D[e] = dn * wp[i + j];
+        (e & 1 ? t0 : q0) += D[e];
+        float& q = e & 1 ? t1 : q1;
+        q = fmaf(D[e], hh[e], q);
       }
-      store<W>(dx, a.x_bf16, base + c, up);
+      if (on(k)) store<W>(dxr + k * kStep, d);
     }
-    float mv = 0.f, mvh = 0.f;
+    float l0 = 0.f, l1 = 0.f;
     if (a.wp) {
-      block_sums<2>(q, red[1]);
-      mv = a.rms ? 0.f : q[0] / a.C;
-      mvh = q[1] / a.C;
-    } else {
-      __syncthreads();  // red[0] is free for the next row
+      q0 += t0, q1 += t1;
+      pair_sums(q0, q1, red + flip * 8, p.G, member);
+      flip ^= 1;
+      l0 = -st.y * (q0 * mean_inv), l1 = -q1 * inv;
     }
+    H* dhr = dh + base;
 #pragma unroll
-    for (int k = 0; k < E / W; ++k) {
-      const int c = column<W>(k);
-      if (c >= a.C) continue;
+    for (int k = 0; k < K; ++k) {
       float o[W];
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const int e = k * W + j;
-        o[j] = a.wp ? st.y * (D[e] - mv - hh[e] * mvh) : D[e];
-      }
-      store<W>(dh, a.h_bf16, base + c, o);
+      for (int j = 0; j < W; ++j)  // 1/std is 1 without a post norm
+        o[j] = fmaf(st.y, fmaf(hh[k * W + j], l1, D[k * W + j]), l0);
+      if (on(k)) store<W>(dhr + k * kStep, o);
     }
-    if (gate_parts && (r + 1 == last || (r + 1) / a.T != grp)) {
-      float* out = gate_parts + ((int64_t)blockIdx.x + grp) * a.C;
+    if (p.gate_parts && (r + 1 == last || r + 1 == turn)) {
+      float* out = p.gate_parts + ((size_t)run + grp) * p.pitch + c0;
 #pragma unroll
-      for (int k = 0; k < E / W; ++k) {
-        const int c = column<W>(k);
-        if (c >= a.C) continue;
+      for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int j = 0; j < W; ++j) {
-          out[c + j] = a.scale * sg[k * W + j];
-          sg[k * W + j] = 0.f;
+          if (on(k)) out[k * kStep + j] = a.scale * sum.g[k * W + j];
+          sum.g[k * W + j] = 0.f;
         }
-      }
     }
   }
-  const int64_t plane = (int64_t)gridDim.x * a.C;
-  float* out = parts + (int64_t)blockIdx.x * a.C;
+}
+
+template <typename X, typename H, typename Y, int E, int W, bool kBias>
+__global__ void __launch_bounds__(kBwdThreads, E == 8 ? 2 : 1)
+    bwd_kernel(const Args a, const BwdArgs p, const Y* dy, const X* dxo, X* dx, H* dh) {
+  constexpr int K = E / W, kStep = 32 * W;
+  __shared__ float2 red[2 * 8];
+  __shared__ float sums[kBwdThreads * E];
+  const int C = a.C, warp = threadIdx.x >> 5, groups = p.G == 1 ? (int)blockDim.x >> 5 : 1;
+  const int group = p.G == 1 ? warp : 0, member = p.G == 1 ? 0 : warp;
+  const int c0 = member * 32 * E + (threadIdx.x & 31) * W;
+  const uint32_t run = blockIdx.x * groups + group;
+  const uint32_t first = min(run * p.rows, a.N), last = min(first + p.rows, a.N);
+  ColumnSums<E> sum;
 #pragma unroll
-  for (int k = 0; k < E / W; ++k) {
-    const int c = column<W>(k);
-    if (c >= a.C) continue;
-    store<W>(out, false, c, sw + k * W);
-    if (a.b) store<W>(out + plane, false, c, sb + k * W);
-    if (a.wp) store<W>(out + 2 * plane, false, c, swp + k * W);
-    if (a.bp) store<W>(out + 3 * plane, false, c, sbp + k * W);
+  for (int e = 0; e < E; ++e) sum.w[e] = sum.b[e] = sum.wp[e] = sum.bp[e] = sum.g[e] = 0.f;
+  if (first < last) {
+    if ((member + 1) * 32 * E <= C)
+      bwd_rows<X, H, Y, E, W, kBias, true>(a, p, dy, dxo, dx, dh, sum, red, run, first, last, c0,
+                                           member);
+    else
+      bwd_rows<X, H, Y, E, W, kBias, false>(a, p, dy, dxo, dx, dh, sum, red, run, first, last, c0,
+                                            member);
   }
+  // the groups' sums, added in order
+  auto total = [&](const float* v, float f, int part) {
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (c0 + k * kStep < C)
+#pragma unroll
+        for (int j = 0; j < W; ++j) sums[group * C + c0 + k * kStep + j] = v[k * W + j];
+    __syncthreads();
+    float* out = p.parts + ((size_t)part * gridDim.x + blockIdx.x) * p.pitch;
+    for (int c = threadIdx.x; c < C; c += blockDim.x) {
+      float t = 0.f;
+      for (int i = 0; i < groups; ++i) t += sums[i * C + c];
+      out[c] = f * t;
+    }
+  };
+  total(sum.w, 1.f, 0);
+  if (kBias && a.b) total(sum.b, 1.f, 1);
+  if (a.wp) total(sum.wp, 1.f, 2);
+  if (kBias && a.bp) total(sum.bp, 1.f, 3);
+  if (a.gate && !p.gate_parts) total(sum.g, a.scale, 4);
 }
 
 struct Sums {
@@ -335,41 +463,50 @@ struct Sums {
   const float* gate_parts;
   float* dgate;
   int64_t N, T, rows;
-  int C, ctas;
+  int C, pitch, ctas;
 };
 
 // Column sums of the partial rows: blockIdx.y < kParts one parameter's gradient, else
-// the gate's gradient of group blockIdx.y - kParts.  A CTA of 8 x 32 threads takes 32
-// columns, thread (g, j) adds rows g, g + 8, ... of column j, then the eight are added.
-__global__ void __launch_bounds__(256) sums_kernel(Sums s) {
-  __shared__ float red[8][33];
-  const int j = threadIdx.x & 31, grp = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + j;
-  const int64_t y = blockIdx.y;
+// that of gate blockIdx.y - kParts from the rows of the runs it meets.  A CTA takes 32 columns: thread (g, j) of
+// 32 x 8 adds rows g, g + 32, ... of four columns, then the 32 are added in order.
+__global__ void __launch_bounds__(256) sums_kernel(const Sums s) {
+  __shared__ float red[32][33];
+  const int j = threadIdx.x & 7, grp = threadIdx.x >> 3;
+  const int c = blockIdx.x * 32 + j * 4;
+  const int y = blockIdx.y;
   const float* in;
   float* out;
-  int64_t count = s.ctas;
+  int count = s.ctas;
   if (y < kParts) {
-    in = s.parts + y * s.ctas * s.C;
+    in = s.parts + (size_t)y * s.ctas * s.pitch;
     out = s.out[y];
   } else {
     const int64_t g = y - kParts, first = g * s.T / s.rows;
     const int64_t end = min((g + 1) * s.T, s.N);
-    count = (end - 1) / s.rows - first + 1;
-    in = s.gate_parts + (first + g) * s.C;
+    count = (int)((end - 1) / s.rows - first + 1);
+    in = s.gate_parts + (first + g) * s.pitch;
     out = s.dgate ? s.dgate + g * s.C : nullptr;
   }
   if (!out) return;
-  float t = 0.f;
-  if (c < s.C)
-    for (int64_t r = grp; r < count; r += 8) t += in[r * s.C + c];
-  red[grp][j] = t;
+  float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (c < s.pitch) {
+#pragma unroll 8
+    for (int r = grp; r < count; r += 32) {
+      const float4 v = *reinterpret_cast<const float4*>(in + (size_t)r * s.pitch + c);
+      t.x += v.x, t.y += v.y, t.z += v.z, t.w += v.w;
+    }
+  }
+  red[grp][j * 4] = t.x, red[grp][j * 4 + 1] = t.y;
+  red[grp][j * 4 + 2] = t.z, red[grp][j * 4 + 3] = t.w;
   __syncthreads();
-  if (grp == 0 && c < s.C) {
-    float u = 0.f;
+  // column of warp w's k-th turn: its 32 sums are one in each lane
 #pragma unroll
-    for (int i = 0; i < 8; ++i) u += red[i][j];
-    out[c] = u;
+  for (int k = 0; k < 4; ++k) {
+    const int col = (threadIdx.x >> 5) * 4 + k, at = blockIdx.x * 32 + col;
+    float u = red[threadIdx.x & 31][col];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+    if ((threadIdx.x & 31) == 0 && at < s.C) out[at] = u;
   }
 }
 
@@ -379,49 +516,81 @@ bool aligned(const void* p, int bytes) {
 
 bool known(int dtype) { return dtype == SQB_BF16 || dtype == SQB_F32; }
 
-constexpr int kMaxCtas = 148 * 4;
+// How the backward deals out N rows of C columns: groups of G warps whose lanes hold E
+// columns (16 beyond 2048 columns, so that 8 warps do), as many CTAs of one group (or of eight
+// groups of one warp) on each of 148 SMs as their registers allow, runs of as many rows each.
+struct Plan {
+  int G, E, groups, ctas, runs, pitch;
+  uint32_t rows;
+};
 
-int ctas_of(int64_t N) { return (int)(N < kMaxCtas ? N : kMaxCtas); }
-int64_t rows_of(int64_t N) { return (N + ctas_of(N) - 1) / ctas_of(N); }
+constexpr int kMaxCtas = 148 * 8;
 
-// Elements a thread holds, and threads for C columns.
-int elements_of(int64_t C) { return C <= 1024 ? 4 : 8; }
-int threads_of(int64_t C) {
-  const int64_t e = elements_of(C);
-  return (int)(((C + e - 1) / e + 31) / 32 * 32);
+Plan plan_of(int64_t N, int64_t C) {
+  Plan p;
+  p.E = C <= 2048 ? 8 : 16;
+  p.G = (int)((C + 32 * p.E - 1) / (32 * p.E));
+  p.groups = p.G == 1 ? 8 : 1;
+  const int per_sm = (p.E == 8 ? 16 : 8) / (p.G * p.groups);
+  const int64_t all = (int64_t)148 * per_sm * p.groups;
+  p.rows = (uint32_t)((N + all - 1) / all);
+  p.runs = (int)((N + p.rows - 1) / p.rows);
+  p.ctas = (p.runs + p.groups - 1) / p.groups;
+  p.pitch = (int)((C + 3) / 4 * 4);
+  return p;
 }
 
-int check(const Args& a, int x_dtype, int h_dtype, int y_dtype, int64_t gates) {
-  if (!a.x || !a.h || !a.w || a.N <= 0 || a.N > INT32_MAX || (a.bp && !a.wp)) return SQB_ERR_ARG;
-  if (a.gate && (gates <= 0 || a.N % gates != 0)) return SQB_ERR_ARG;
+int check(const Args& a, int64_t N, int64_t C, int x_dtype, int h_dtype, int y_dtype,
+          int64_t gates) {
+  if (!a.x || !a.h || !a.w || N <= 0 || N > INT32_MAX || (a.bp && !a.wp)) return SQB_ERR_ARG;
+  if (a.gate && (gates <= 0 || N % gates != 0)) return SQB_ERR_ARG;
   if (!known(x_dtype) || !known(h_dtype) || !known(y_dtype)) return SQB_ERR_DTYPE;
-  if (a.C <= 0 || a.C > kMaxC) return SQB_ERR_UNSUPPORTED;
+  if (C <= 0 || C > kMaxC) return SQB_ERR_UNSUPPORTED;
   return SQB_OK;
 }
 
 // Whether every row can be read four elements at a time.
 bool wide(const Args& a, const void* const* more, int n) {
   if (a.C % 4) return false;
-  for (const void* p : {a.x, a.h, (const void*)a.w, (const void*)a.b, (const void*)a.wp,
-                        (const void*)a.bp, (const void*)a.gate})
+  const void* all[] = {a.x, a.h, a.w, a.b, a.wp, a.bp, a.gate};
+  for (const void* p : all)
     if (!aligned(p, 16)) return false;
   for (int i = 0; i < n; ++i)
     if (!aligned(more[i], 16)) return false;
   return true;
 }
 
-Args make_args(const void* x, int x_dtype, const void* h, int h_dtype, int y_dtype,
-               const float* w, const float* b, const float* wp, const float* bp,
-               const float* gate, int64_t gates, float scale, float eps, int rms, int64_t N,
-               int64_t C) {
+Args make_args(const void* x, const void* h, const float* w, const float* b, const float* wp,
+               const float* bp, const float* gate, int64_t gates, float scale, float eps, int rms,
+               int64_t N, int64_t C) {
   Args a;
   a.x = x, a.h = h, a.w = w, a.b = b, a.wp = wp, a.bp = bp, a.gate = gate;
-  a.scale = scale, a.eps = eps, a.N = N, a.T = gate && gates > 0 ? N / gates : N;
-  if (a.T <= 0) a.T = 1;
-  a.C = C > kMaxC ? kMaxC + 1 : (int)C;
-  a.rms = rms != 0, a.x_bf16 = x_dtype == SQB_BF16, a.h_bf16 = h_dtype == SQB_BF16;
-  a.y_bf16 = y_dtype == SQB_BF16;
+  a.scale = scale, a.eps = eps, a.N = (uint32_t)N;
+  a.T = (uint32_t)(gate && gates > 0 && N >= gates ? N / gates : N);
+  a.C = (int)C;
+  a.rms = rms != 0;
   return a;
+}
+
+// Calls f(X(), H(), Y()) for the three dtypes.
+template <typename F>
+void by_type(int x, int h, int y, F&& f) {
+  auto second = [&](auto X) {
+    auto third = [&](auto H) {
+      if (y == SQB_BF16)
+        f(X, H, __nv_bfloat16());
+      else
+        f(X, H, float());
+    };
+    if (h == SQB_BF16)
+      third(__nv_bfloat16());
+    else
+      third(float());
+  };
+  if (x == SQB_BF16)
+    second(__nv_bfloat16());
+  else
+    second(float());
 }
 
 }  // namespace
@@ -436,35 +605,55 @@ extern "C" int sqb_residual_norm_fwd(const void* x, int x_dtype, const void* h, 
                                      const float* gate, int64_t gates, float scale, float eps,
                                      int rms, void* x_out, void* y, int y_dtype, float* stats,
                                      int64_t N, int64_t C, void* stream) {
-  const Args a = make_args(x, x_dtype, h, h_dtype, y_dtype, weight, bias, post_weight, post_bias,
-                           gate, gates, scale, eps, rms, N, C);
-  if (const int rc = check(a, x_dtype, h_dtype, y_dtype, gates)) return rc;
+  const Args a = make_args(x, h, weight, bias, post_weight, post_bias, gate, gates, scale, eps,
+                           rms, N, C);
+  if (const int rc = check(a, N, C, x_dtype, h_dtype, y_dtype, gates)) return rc;
   if (!x_out || !y || !stats) return SQB_ERR_ARG;
   if (!aligned(stats, 16)) return SQB_ERR_ALIGN;
   cudaStream_t q = static_cast<cudaStream_t>(stream);
   const void* more[] = {x_out, y};
   const bool w4 = wide(a, more, 2);
-  const int nt = threads_of(C);
-  const unsigned grid = (unsigned)N;
   float4* st = reinterpret_cast<float4*>(stats);
-  if (elements_of(C) == 4) {
-    if (w4)
-      fwd_kernel<4, 4><<<grid, nt, 0, q>>>(a, x_out, y, st);
-    else
-      fwd_kernel<4, 1><<<grid, nt, 0, q>>>(a, x_out, y, st);
-  } else {
-    if (w4)
-      fwd_kernel<8, 4><<<grid, nt, 0, q>>>(a, x_out, y, st);
-    else
-      fwd_kernel<8, 1><<<grid, nt, 0, q>>>(a, x_out, y, st);
-  }
+  by_type(x_dtype, h_dtype, y_dtype, [&](auto tx, auto th, auto ty) {
+    using X = decltype(tx);
+    using H = decltype(th);
+    using Y = decltype(ty);
+    X* xo = static_cast<X*>(x_out);
+    Y* yo = static_cast<Y*>(y);
+#define SQB_FWD(K, W, TH)                                                                     \
+  fwd_kernel<X, H, Y, K, W, TH>                                                               \
+      <<<(unsigned)((N + kFwdThreads / TH - 1) / (kFwdThreads / TH)), kFwdThreads, 0, q>>>( \
+          a, xo, yo, st)
+    if (w4) {
+      if (C <= 512)
+        SQB_FWD(4, 4, 32);
+      else if (C <= 768)
+        SQB_FWD(6, 4, 32);
+      else if (C <= 1024)
+        SQB_FWD(8, 4, 32);
+      else if (C <= 2048)
+        SQB_FWD(4, 4, 128);
+      else
+        SQB_FWD(4, 4, 256);
+    } else {
+      if (C <= 512)
+        SQB_FWD(16, 1, 32);
+      else if (C <= 2048)
+        SQB_FWD(16, 1, 128);
+      else
+        SQB_FWD(16, 1, 256);
+    }
+#undef SQB_FWD
+  });
   return cudaGetLastError() == cudaSuccess ? SQB_OK : SQB_ERR_LAUNCH;
 }
 
 extern "C" size_t sqb_residual_norm_workspace_bytes(int64_t N, int64_t C, int64_t gates) {
   if (N <= 0 || C <= 0 || gates < 0) return 0;
-  const int64_t rows = kParts * (int64_t)ctas_of(N) + (gates ? ctas_of(N) + gates : 0);
-  return (size_t)rows * (size_t)C * sizeof(float);
+  // partial rows of the CTAs, and of at most 16 runs on each SM
+  const int64_t ctas = N < kMaxCtas ? N : kMaxCtas, runs = N < 148 * 16 ? N : 148 * 16;
+  return (size_t)(kParts * ctas + (gates > 1 ? runs + gates : 0)) * (size_t)((C + 3) / 4 * 4) *
+         sizeof(float);
 }
 
 extern "C" int sqb_residual_norm_bwd(const void* dy, int y_dtype, const void* dx_out,
@@ -476,9 +665,9 @@ extern "C" int sqb_residual_norm_bwd(const void* dy, int y_dtype, const void* dx
                                      float* dweight, float* dbias, float* dpost_weight,
                                      float* dpost_bias, float* dgate, void* workspace,
                                      size_t ws_bytes, int64_t N, int64_t C, void* stream) {
-  const Args a = make_args(x, x_dtype, h, h_dtype, y_dtype, weight, bias, post_weight, post_bias,
-                           gate, gates, scale, eps, rms, N, C);
-  if (const int rc = check(a, x_dtype, h_dtype, y_dtype, gates)) return rc;
+  const Args a = make_args(x, h, weight, bias, post_weight, post_bias, gate, gates, scale, eps,
+                           rms, N, C);
+  if (const int rc = check(a, N, C, x_dtype, h_dtype, y_dtype, gates)) return rc;
   if (!dy || !stats || !dx || !dh || !dweight || (bias && !dbias) ||
       (post_weight && !dpost_weight) || (post_bias && !dpost_bias) || (gate && !dgate))
     return SQB_ERR_ARG;
@@ -488,31 +677,38 @@ extern "C" int sqb_residual_norm_bwd(const void* dy, int y_dtype, const void* dx
   if (!aligned(stats, 16) || !aligned(workspace, 16)) return SQB_ERR_ALIGN;
   cudaStream_t q = static_cast<cudaStream_t>(stream);
   const void* more[] = {dy, dx_out, dx, dh};
-  const bool w4 = wide(a, more, 4);
-  const int nt = threads_of(C), ctas = ctas_of(N);
-  const int64_t rows = rows_of(N);
+  const bool w4 = wide(a, more, 4), biased = bias || post_bias;
+  const Plan p = plan_of(N, C);
   float* parts = static_cast<float*>(workspace);
-  float* gate_parts = gate ? parts + (int64_t)kParts * ctas * C : nullptr;
-  const float4* st = reinterpret_cast<const float4*>(stats);
-  // rows are dealt out evenly, so the last CTAs may have none: they write zero sums
-  if (elements_of(C) == 4) {
-    if (w4)
-      bwd_kernel<4, 4><<<ctas, nt, 0, q>>>(a, dy, dx_out, st, dx, dh, parts, gate_parts, rows);
-    else
-      bwd_kernel<4, 1><<<ctas, nt, 0, q>>>(a, dy, dx_out, st, dx, dh, parts, gate_parts, rows);
-  } else {
-    if (w4)
-      bwd_kernel<8, 4><<<ctas, nt, 0, q>>>(a, dy, dx_out, st, dx, dh, parts, gate_parts, rows);
-    else
-      bwd_kernel<8, 1><<<ctas, nt, 0, q>>>(a, dy, dx_out, st, dx, dh, parts, gate_parts, rows);
-  }
+  float* gate_parts = gate && gates > 1 ? parts + (size_t)kParts * p.ctas * p.pitch : nullptr;
+  const BwdArgs more_args{reinterpret_cast<const float4*>(stats), parts, gate_parts, p.pitch, p.G,
+                          p.rows};
+  by_type(x_dtype, h_dtype, y_dtype, [&](auto tx, auto th, auto ty) {
+    using X = decltype(tx);
+    using H = decltype(th);
+    using Y = decltype(ty);
+    auto run = [&](auto kernel) {
+      kernel<<<p.ctas, 32 * p.G * p.groups, 0, q>>>(
+          a, more_args, static_cast<const Y*>(dy), static_cast<const X*>(dx_out),
+          static_cast<X*>(dx), static_cast<H*>(dh));
+    };
+    auto sized = [&](auto biased_) {
+      constexpr bool kb = decltype(biased_)::value;
+      if (p.E == 8)
+        w4 ? run(bwd_kernel<X, H, Y, 8, 4, kb>) : run(bwd_kernel<X, H, Y, 8, 1, kb>);
+      else
+        w4 ? run(bwd_kernel<X, H, Y, 16, 4, kb>) : run(bwd_kernel<X, H, Y, 16, 1, kb>);
+    };
+    biased ? sized(std::true_type()) : sized(std::false_type());
+  });
   Sums s;
   s.parts = parts;
   s.out[0] = dweight, s.out[1] = bias ? dbias : nullptr;
   s.out[2] = post_weight ? dpost_weight : nullptr, s.out[3] = post_bias ? dpost_bias : nullptr;
+  s.out[4] = gate && !gate_parts ? dgate : nullptr;
   s.gate_parts = gate_parts, s.dgate = dgate;
-  s.N = N, s.T = a.T, s.rows = rows, s.C = (int)C, s.ctas = ctas;
-  const dim3 grid((unsigned)((C + 31) / 32), (unsigned)(kParts + (gate ? gates : 0)));
+  s.N = N, s.T = a.T, s.rows = p.rows, s.C = (int)C, s.pitch = p.pitch, s.ctas = p.ctas;
+  const dim3 grid((unsigned)((C + 31) / 32), (unsigned)(kParts + (gate_parts ? gates : 0)));
   sums_kernel<<<grid, 256, 0, q>>>(s);
   return cudaGetLastError() == cudaSuccess ? SQB_OK : SQB_ERR_LAUNCH;
 }

@@ -13,7 +13,7 @@ __all__ = ["residual_norm"]
 
 _DTYPES = {torch.float32: _lib.SQB_F32, torch.bfloat16: _lib.SQB_BF16}
 MAX_WIDTH = 4096
-MAX_GATES = 65531
+MAX_GATES = 65530
 
 
 def _ptr(t):
