@@ -124,6 +124,12 @@ def on_device(device):
     return torch.cuda.device(device)
 
 
+def stream(device) -> int:
+    """The current stream of a CUDA device, as the library takes it."""
+    return torch._C._cuda_getCurrentRawStream(
+        torch.cuda.current_device() if device.index is None else device.index)
+
+
 def plain(x) -> bool:
     """Whether `x` is an ordinary tensor in an ordinary eager call.  The post-training ops
     then run without the dispatcher, whose custom-op layers cost 100 us a call; a traced,

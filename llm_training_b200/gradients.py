@@ -73,7 +73,7 @@ def grad_norm(tensors):
     with _lib.on_device(device):
         _lib.check("sqb_grad_norm", _lib.lib().sqb_grad_norm(
             ptrs, _numels(tensors), dtypes, len(tensors), ws.data_ptr(), nbytes,
-            norm.data_ptr(), torch.cuda.current_stream(device).cuda_stream))
+            norm.data_ptr(), _lib.stream(device)))
     return norm
 
 
@@ -86,7 +86,7 @@ def _clip(grads, outs, max_norm, device):
         _lib.check("sqb_grad_clip", _lib.lib().sqb_grad_clip(
             ptrs, out_ptrs, _numels(grads), dtypes, out_dtypes, len(grads), max_norm,
             ws.data_ptr(), nbytes, norm.data_ptr(),
-            torch.cuda.current_stream(device).cuda_stream))
+            _lib.stream(device)))
     return norm
 
 

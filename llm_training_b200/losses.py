@@ -31,10 +31,6 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
-
-
 def _grad_like(x):
     """An uninitialised tensor of x's shape, strides and 16-byte phase (the gradient is
     written with the vector stores the logits are read with)."""
@@ -60,6 +56,16 @@ def _dims(x):
     return (*x.shape, x.stride(0), x.stride(1))
 
 
+def _scratch(N):
+    """Where the scratch begins in a buffer that starts with 3 N floats, in bytes."""
+    return -(-12 * N // 256) * 256
+
+
+def _rows_and(nbytes, N):
+    """Floats of a buffer of 3 N floats and then `nbytes` of scratch."""
+    return (_scratch(N) + nbytes + 3) // 4
+
+
 def _run(raw, op, function, x, *args):
     if not _lib.plain(x):
         return op(x, *args)
@@ -77,7 +83,7 @@ def _logp_fwd_raw(x: torch.Tensor, t: torch.Tensor) -> tuple[torch.Tensor, torch
         with _lib.on_device(x.device):
             _lib.check("sqb_logp_fwd", _lib.lib().sqb_logp_fwd(
                 x.data_ptr(), t.data_ptr(), logp.data_ptr(), stats.data_ptr(), S, T, V, ss, st,
-                _DTYPES[x.dtype], _stream(x)))
+                _DTYPES[x.dtype], _lib.stream(x.device)))
     return logp, stats
 
 
@@ -101,7 +107,7 @@ def _logp_bwd_raw(x: torch.Tensor, t: torch.Tensor, stats: torch.Tensor,
         with _lib.on_device(x.device):
             _lib.check("sqb_logp_bwd", _lib.lib().sqb_logp_bwd(
                 x.data_ptr(), t.data_ptr(), stats.data_ptr(), g, _ptr(scale), dx.data_ptr(), S,
-                T, V, ss, st, ss, st, _DTYPES[x.dtype], _stream(x)))
+                T, V, ss, st, ss, st, _DTYPES[x.dtype], _lib.stream(x.device)))
     return dx
 
 
@@ -143,21 +149,21 @@ class _LogP(torch.autograd.Function):
 def _preference_raw(x: torch.Tensor, t: torch.Tensor, ref: Optional[torch.Tensor],
                     cu: Optional[torch.Tensor], pairs: int, beta: float, label_smoothing: float
                     ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(loss, rewards (2, P), row statistics and d loss / d logp of each row (3 S T,))."""
+    """(loss, rewards (2, P), row statistics and d loss / d logp of each row (3 S T floats, and
+    scratch))."""
     S, T, V, ss, st = _dims(x)
     dev, N, f32 = x.device, S * T, torch.float32
     loss = torch.empty((), dtype=f32, device=dev)
     rewards = torch.empty((2, pairs), dtype=f32, device=dev)
-    rows = torch.empty(3 * N, dtype=f32, device=dev)
     lib = _lib.lib()
     nbytes = lib.sqb_preference_workspace_bytes(N, pairs)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    rows = torch.empty(_rows_and(nbytes, N), dtype=f32, device=dev)
     at = rows.data_ptr()
     with _lib.on_device(dev):
         _lib.check("sqb_preference_fwd", lib.sqb_preference_fwd(
             x.data_ptr(), t.data_ptr(), _ptr(cu), _ptr(ref), pairs, beta, label_smoothing,
             loss.data_ptr(), rewards.data_ptr(), at, at + 8 * N, S, T, V, ss, st,
-            _DTYPES[x.dtype], ws.data_ptr(), nbytes, _stream(x)))
+            _DTYPES[x.dtype], at + _scratch(N), nbytes, _lib.stream(x.device)))
     return loss, rewards, rows
 
 
@@ -168,8 +174,10 @@ _preference_fwd = torch.library.custom_op("sqrtblock::preference_fwd", _preferen
 @_preference_fwd.register_fake
 def _(x, t, ref, cu, pairs, beta, label_smoothing):
     f32 = torch.float32
+    N = t.numel()
+    nbytes = -(-8 * N // 256) * 256 + 8 * pairs  # sqb_preference_workspace_bytes
     return (x.new_empty((), dtype=f32), x.new_empty((2, pairs), dtype=f32),
-            x.new_empty(3 * t.numel(), dtype=f32))
+            x.new_empty(_rows_and(nbytes, N), dtype=f32))
 
 
 def _loss_grad(ctx, dloss):
@@ -229,7 +237,7 @@ def _policy_raw(x: torch.Tensor, t: torch.Tensor, adv: torch.Tensor,
             adv_by_seq, clip_low, clip_high, kl_coef, per_seq, loss.data_ptr(),
             statistics.data_ptr(), logps.data_ptr(), None if fused else at,
             None if fused else at + 8 * N, at if fused else None, grad_scale if fused else 1.0,
-            S, T, V, ss, st, ss, st, _DTYPES[x.dtype], ws.data_ptr(), nbytes, _stream(x)))
+            S, T, V, ss, st, ss, st, _DTYPES[x.dtype], ws.data_ptr(), nbytes, _lib.stream(x.device)))
     return loss, logps, statistics, last
 
 

@@ -38,7 +38,7 @@ def _fwd_raw(x: torch.Tensor, h: torch.Tensor, w: torch.Tensor, b: Optional[torc
                 _ptr(b), _ptr(wp), _ptr(bp), _ptr(gate),
                 gate.numel() // C if gate is not None else 0, scale, eps, rms, xo.data_ptr(),
                 y.data_ptr(), _DTYPES[out_dtype], stats.data_ptr(), N, C,
-                torch.cuda.current_stream(x.device).cuda_stream))
+                _lib.stream(x.device)))
     return xo, y, stats
 
 
@@ -78,7 +78,7 @@ def _bwd_raw(dy: torch.Tensor, dxo: Optional[torch.Tensor], x: torch.Tensor, h: 
             h.data_ptr(), _DTYPES[h.dtype], w.data_ptr(), _ptr(b), _ptr(wp), _ptr(bp),
             _ptr(gate), gates, scale, eps, rms, stats.data_ptr(), dx.data_ptr(), dh.data_ptr(),
             *ptrs, ws.data_ptr(), nbytes, N, C,
-            torch.cuda.current_stream(x.device).cuda_stream))
+            _lib.stream(x.device)))
     return dx, dh, dp
 
 
@@ -109,14 +109,15 @@ def _grad(ctx, dxo, dy, _dstats):
     dxo = dxo.contiguous() if dxo is not None else None
     dx, dh, dp = (_bwd_raw if _lib.plain(x) else _bwd)(
         dy.contiguous(), dxo, x, h, w, b, wp, bp, gate, *ctx.cfg, stats)
-    given, at = [], 0
-    for p in (w, b, wp, bp, gate):
-        if p is None:
-            given.append(None)
-        else:
-            given.append(dp[at:at + p.numel()])
-            at += p.numel()
-    if gate is not None and gate.dim() > 1:
+    C = x.shape[-1]
+    rows = dp.view(-1, C)
+    if gate is not None and gate.numel() != C:  # its rows are the last
+        k = rows.shape[0] - gate.numel() // C
+        parts = iter((*rows[:k].unbind(0), rows[k:].view(gate.shape)))
+    else:
+        parts = iter(rows.unbind(0))
+    given = [next(parts) if p is not None else None for p in (w, b, wp, bp, gate)]
+    if gate is not None and given[4].shape != gate.shape:
         given[4] = given[4].view(gate.shape)
     return (dx, dh, *given, None, None, None, None)
 
