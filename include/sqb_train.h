@@ -145,8 +145,8 @@ int sqb_policy_fwd(const void* logits, const int64_t* targets, const int64_t* cu
                    size_t ws_bytes, void* stream);
 
 /* ---- Global gradient norm and clipping ---------------------------------------
- * n tensors as host arrays of device pointers (element-aligned), element counts (each
- * at most 2^34, 0 allowed) and dtypes; the arrays are read before the call returns.
+ * n tensors as host arrays of device pointers (element-aligned), element counts (0
+ * allowed) and dtypes; the arrays are read before the call returns.
  * norm: one fp32 on the device, sqrt of the sum of squares, summed in 64 bits in a
  * fixed order. */
 size_t sqb_grad_norm_workspace_bytes(int64_t n_tensors);
