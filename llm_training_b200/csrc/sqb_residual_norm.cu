@@ -106,133 +106,256 @@ __device__ __forceinline__ void param(const float* p, int c, float none, float* 
     for (int j = 0; j < W; ++j) v[j] = none;
 }
 
-// ---- forward ------------------------------------------------------------------------
+// ---- rows ---------------------------------------------------------------------------
 //
-// kThreads threads hold a row, E = K * W elements each; a CTA of 256 threads takes
-// 256 / kThreads rows.  A warp for rows up to 1024 columns: its sums need no barrier, and
-// enough rows are in flight on an SM to keep HBM busy.
+// G warps (1 to 8) hold a row, E columns a lane, each warp 32 E consecutive ones, and walk a
+// run of consecutive rows.  A CTA is one such group, or eight groups of one warp.  A warp
+// whose columns all exist takes a path without a comparison for each.
 
-constexpr int kFwdThreads = 256;
+constexpr int kMaxThreads = 256;
 
-// Sum over the row's threads, the same in all of them.  red: one float for each warp of the
-// CTA; each use of a buffer is followed by another's before its next.
-template <int kThreads>
-__device__ __forceinline__ float row_sum(float v, float* red) {
+// The CTA's barrier: its warps arrive from two places in the code.
+__device__ __forceinline__ void group_barrier() { asm volatile("bar.sync 0;" ::: "memory"); }
+
+__device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if constexpr (kThreads > 32) {
-    constexpr int kWarps = kThreads / 32;
-    const int warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) red[warp] = v;
-    __syncthreads();
-    v = 0.f;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) v += red[warp / kWarps * kWarps + i];
-  }
   return v;
 }
 
-template <int K, int W, int kThreads>
-__device__ __forceinline__ void moments(const float (&v)[K * W], const Args& a, int me, float* red,
-                                        float& mean, float& rstd) {
-  mean = 0.f;
+// ---- forward ------------------------------------------------------------------------
+
+// Mean (0 for RMS) and 1/std of a row over its G warps.  Each warp finds its own columns'
+// mean and squared differences (two sweeps over registers); the warps' are joined by
+//   M2 = sum M2_i + n_i (mean_i - mean)^2,  one barrier for both.
+// red: a pair for each warp; uses alternate between two.
+template <int E, int W, typename On>
+__device__ __forceinline__ void moments(const float (&v)[E], const Args& a, On on, int G,
+                                        int member, float2* red, float& mean, float& rstd) {
+  const int n = min(32 * E, a.C - member * 32 * E);
+  float m = 0.f, q = 0.f;
   if (!a.rms) {
-    float s = 0.f;
 #pragma unroll
-    for (int e = 0; e < K * W; ++e) s += v[e];  // columns past C hold 0
-    mean = row_sum<kThreads>(s, red) / a.C;
+    for (int e = 0; e < E; ++e) m += v[e];  // columns that are not there hold 0
+    m = warp_sum(m) / n;
   }
-  float q = 0.f;
 #pragma unroll
-  for (int k = 0; k < K; ++k)
-    if ((k * kThreads + me) * W < a.C)
-#pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const float d = v[k * W + j] - mean;
-        q = fmaf(d, d, q);
-      }
-  rstd = rsqrtf(row_sum<kThreads>(q, red + 8) / a.C + a.eps);
+  for (int e = 0; e < E; ++e) {
+    const float d = v[e] - m;
+    if (on(e / W)) q = fmaf(d, d, q);
+  }
+  q = warp_sum(q);
+  mean = m;
+  if (G > 1) {
+    if ((threadIdx.x & 31) == 0) red[member] = make_float2(m, q);
+    group_barrier();
+    if (!a.rms) {
+      mean = 0.f;
+      for (int i = 0; i < G; ++i) mean += red[i].x * min(32 * E, a.C - i * 32 * E);
+      mean /= a.C;
+    }
+    q = 0.f;
+    for (int i = 0; i < G; ++i) {
+      const float2 p = red[i];
+      const float d = p.x - mean;
+      q += p.y;
+      if (!a.rms) q += d * d * min(32 * E, a.C - i * 32 * E);
+    }
+  }
+  rstd = rsqrtf(q / a.C + a.eps);
 }
 
-template <typename X, typename H, typename Y, int K, int W, int kThreads>
-__global__ void __launch_bounds__(kFwdThreads)
-    fwd_kernel(const Args a, X* xo, Y* y, float4* stats) {
-  __shared__ float red[32];
-  constexpr int kRows = kFwdThreads / kThreads;
-  const int me = threadIdx.x % kThreads;
-  const uint32_t r = blockIdx.x * kRows + threadIdx.x / kThreads;
-  const bool live = r < a.N;  // a row of the CTA may be past the end: it only takes barriers
-  if (kThreads == 32 && !live) return;
-  const size_t base = (size_t)(live ? r : 0) * a.C;
-  const X* xr = static_cast<const X*>(a.x) + base;
-  const H* hr = static_cast<const H*>(a.h) + base;
-  const float* gate = a.gate ? a.gate + (size_t)((live ? r : 0) / a.T) * a.C : nullptr;
-  Raw<X, W> xw[K];
-  Raw<H, W> hw[K];
+template <typename X, typename H, typename Y, int E, int W, bool kBias, bool kFull>
+__device__ __forceinline__ void fwd_rows(const Args& a, X* xo, Y* y, float4* stats, float2* red,
+                                         uint32_t first, uint32_t last, int c0, int member,
+                                         int G) {
+  constexpr int K = E / W, kStep = 32 * W;
+  constexpr bool kKeep = E == 8 && !kBias;  // parameters in registers
+  const int C = a.C;
+  auto on = [&](int k) { return kFull || c0 + k * kStep < C; };
+  float w[kKeep ? E : W], wp[kKeep ? E : W], gw[kKeep ? E : W], b[W], bp[W];
+  auto load_post = [&](const float* gate, int k, int i) {
+    param<W>(on(k) ? a.wp : nullptr, c0 + k * kStep, 1.f, wp + i);
+    param<W>(on(k) ? gate : nullptr, c0 + k * kStep, 1.f, gw + i);
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = (k * kThreads + me) * W;
-    if (c < a.C) {
-      hw[k] = fetch<H, W>(hr + c);
-      xw[k] = fetch<X, W>(xr + c);
+    for (int j = 0; j < W; ++j) gw[i + j] *= a.scale;
+  };
+  uint32_t grp = first / a.T, turn = (grp + 1) * a.T;
+  const float* gate = a.gate ? a.gate + (size_t)grp * C : nullptr;
+  if (kKeep)
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      load_post(gate, k, k * W);
+      param<W>(on(k) ? a.w : nullptr, c0 + k * kStep, 1.f, w + k * W);
     }
-  }
-  float h[K * W], x[K * W];
+  for (uint32_t r = first; r < last; ++r) {
+    const size_t base = (size_t)r * C + c0;
+    const X* xr = static_cast<const X*>(a.x) + base;
+    const H* hr = static_cast<const H*>(a.h) + base;
+    Raw<X, W> xw[K];
+    Raw<H, W> hw[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if ((k * kThreads + me) * W < a.C) {
+    for (int k = 0; k < K; ++k) {
+      const int i = on(k) ? k * kStep : -c0;  // a column that is not there: the row's first
+      hw[k] = fetch<H, W>(hr + i);
+      xw[k] = fetch<X, W>(xr + i);
+    }
+    if (r == turn) {
+      turn += a.T;
+      if (a.gate) {
+        gate += C;
+        if (kKeep)
+#pragma unroll
+          for (int k = 0; k < K; ++k) load_post(gate, k, k * W);
+      }
+    }
+    float h[E], x[E];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
       unpack(hw[k], h + k * W);
       unpack(xw[k], x + k * W);
+      if (!on(k))
+#pragma unroll
+        for (int j = 0; j < W; ++j) h[k * W + j] = x[k * W + j] = 0.f;
+    }
+    float mh = 0.f, rh = 1.f, mx, rx;
+    if (a.wp) moments<E, W>(h, a, on, G, member, red, mh, rh);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int i = kKeep ? k * W : 0;
+      if (!kKeep) load_post(gate, k, 0);
+      param<W>(kBias && on(k) ? a.bp : nullptr, c0 + k * kStep, 0.f, bp);
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const int e = k * W + j;
+        x[e] = fmaf(gw[i + j], fmaf((h[e] - mh) * rh, wp[i + j], bp[j]), x[e]);
+        if (!on(k)) x[e] = 0.f;
+      }
+      if (on(k)) store<W>(xo + base + k * kStep, x + k * W);
+    }
+    moments<E, W>(x, a, on, G, member, red + 8, mx, rx);
+    if (G > 1 && !a.wp) group_barrier();  // red + 8 is written again before another barrier
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int i = kKeep ? k * W : 0;
+      float o[W];
+      if (!kKeep) param<W>(on(k) ? a.w : nullptr, c0 + k * kStep, 1.f, w);
+      param<W>(kBias && on(k) ? a.b : nullptr, c0 + k * kStep, 0.f, b);
+#pragma unroll
+      for (int j = 0; j < W; ++j) o[j] = fmaf((x[k * W + j] - mx) * rx, w[i + j], b[j]);
+      if (on(k)) store<W>(y + base + k * kStep, o);
+    }
+    if (member == 0 && (threadIdx.x & 31) == 0) stats[r] = make_float4(mh, rh, mx, rx);
+  }
+}
+
+template <typename X, typename H, typename Y, int E, int W, bool kBias>
+__global__ void __launch_bounds__(kMaxThreads, E == 8 ? 3 : 2)
+    fwd_kernel(const Args a, X* xo, Y* y, float4* stats, int G, uint32_t rows) {
+  __shared__ float2 red[2 * 8];
+  const int warp = threadIdx.x >> 5, groups = G == 1 ? (int)blockDim.x >> 5 : 1;
+  const int group = G == 1 ? warp : 0, member = G == 1 ? 0 : warp;
+  const int c0 = member * 32 * E + (threadIdx.x & 31) * W;
+  const uint32_t run = blockIdx.x * groups + group;
+  const uint32_t first = min(run * rows, a.N), last = min(first + rows, a.N);
+  if (first >= last) return;  // the whole group
+  if ((member + 1) * 32 * E <= a.C)
+    fwd_rows<X, H, Y, E, W, kBias, true>(a, xo, y, stats, red, first, last, c0, member, G);
+  else
+    fwd_rows<X, H, Y, E, W, kBias, false>(a, xo, y, stats, red, first, last, c0, member, G);
+}
+
+// A warp for a row of up to 1024 columns, K * 4 a lane, when they can be read four at a time:
+// no barriers, and rows enough in flight (16384 rows of 768: 31 us, against 41 us with three
+// warps a row; wider rows would leave too few registers, single elements too many
+// instructions: 9006 x 1999 53 us with eight warps a row, 89 us with four and more columns
+// a lane).
+template <typename X, typename H, typename Y, int K>
+__global__ void __launch_bounds__(kMaxThreads)
+    fwd_warp_kernel(const Args a, X* xo, Y* y, float4* stats) {
+  const int lane = threadIdx.x & 31, C = a.C;
+  const uint32_t r = blockIdx.x * (kMaxThreads / 32) + (threadIdx.x >> 5);
+  if (r >= a.N) return;
+  const size_t base = (size_t)r * C;
+  const X* xr = static_cast<const X*>(a.x) + base;
+  const H* hr = static_cast<const H*>(a.h) + base;
+  const float* gate = a.gate ? a.gate + (size_t)(r / a.T) * C : nullptr;
+  auto column = [&](int k) { return (k * 32 + lane) * 4; };
+  auto on = [&](int k) { return column(k) < C; };
+  Raw<X, 4> xw[K];
+  Raw<H, 4> hw[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (on(k)) {
+      hw[k] = fetch<H, 4>(hr + column(k));
+      xw[k] = fetch<X, 4>(xr + column(k));
+    }
+  float h[K * 4], x[K * 4];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (on(k)) {
+      unpack(hw[k], h + k * 4);
+      unpack(xw[k], x + k * 4);
     } else {
 #pragma unroll
-      for (int j = 0; j < W; ++j) h[k * W + j] = x[k * W + j] = 0.f;
+      for (int j = 0; j < 4; ++j) h[k * 4 + j] = x[k * 4 + j] = 0.f;
     }
   }
+  auto moments = [&](const float* v, float& mean, float& rstd) {
+    mean = 0.f;
+    if (!a.rms) {
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < K * 4; ++e) s += v[e];
+      mean = warp_sum(s) / C;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int e = 0; e < K * 4; ++e) {
+      const float d = v[e] - mean;
+      if (on(e / 4)) q = fmaf(d, d, q);
+    }
+    rstd = rsqrtf(warp_sum(q) / C + a.eps);
+  };
   float mh = 0.f, rh = 1.f, mx, rx;
-  if (a.wp) moments<K, W, kThreads>(h, a, me, red, mh, rh);
+  if (a.wp) moments(h, mh, rh);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int c = (k * kThreads + me) * W;
-    if (c >= a.C) continue;
-    float g[W], w[W], b[W];
-    param<W>(gate, c, 1.f, g);
-    param<W>(a.wp, c, 1.f, w);
-    param<W>(a.bp, c, 0.f, b);
+    if (!on(k)) continue;
+    float g[4], w[4], b[4];
+    param<4>(gate, column(k), 1.f, g);
+    param<4>(a.wp, column(k), 1.f, w);
+    param<4>(a.bp, column(k), 0.f, b);
 #pragma unroll
-    for (int j = 0; j < W; ++j)
-      x[k * W + j] += a.scale * g[j] * fmaf((h[k * W + j] - mh) * rh, w[j], b[j]);
-    if (live) store<W>(xo + base + c, x + k * W);
+    for (int j = 0; j < 4; ++j)
+      x[k * 4 + j] =
+          fmaf(a.scale * g[j], fmaf((h[k * 4 + j] - mh) * rh, w[j], b[j]), x[k * 4 + j]);
+    store<4>(xo + base + column(k), x + k * 4);
   }
-  moments<K, W, kThreads>(x, a, me, red + 16, mx, rx);
+  moments(x, mx, rx);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int c = (k * kThreads + me) * W;
-    if (c >= a.C) continue;
-    float w[W], b[W], o[W];
-    param<W>(a.w, c, 1.f, w);
-    param<W>(a.b, c, 0.f, b);
+    if (!on(k)) continue;
+    float w[4], b[4], o[4];
+    param<4>(a.w, column(k), 1.f, w);
+    param<4>(a.b, column(k), 0.f, b);
 #pragma unroll
-    for (int j = 0; j < W; ++j) o[j] = fmaf((x[k * W + j] - mx) * rx, w[j], b[j]);
-    if (live) store<W>(y + base + c, o);
+    for (int j = 0; j < 4; ++j) o[j] = fmaf((x[k * 4 + j] - mx) * rx, w[j], b[j]);
+    store<4>(y + base + column(k), o);
   }
-  if (live && me == 0) stats[r] = make_float4(mh, rh, mx, rx);
+  if (lane == 0) stats[r] = make_float4(mh, rh, mx, rx);
 }
 
 // ---- backward -----------------------------------------------------------------------
 //
-// G warps (1 to 8) hold a row, E columns a lane, each warp 32 E consecutive ones, and walk a
-// run of consecutive rows; the columns' sums (d weight and so on) stay in their registers
-// over the run.  A CTA is one such group, or eight groups of one warp; each CTA writes one
-// partial row of each (parts: (kParts, grid, pitch)), which a second kernel adds in a fixed
-// order (bit-reproducible).  A gate for each sample has its sums written where the gate
+// The columns' sums (d weight and so on) stay in registers over a run of rows; each CTA
+// writes one partial row of each (parts: (kParts, grid, pitch)), which a second kernel adds
+// in a fixed order (bit-reproducible).  A gate for each sample has its sums written where the gate
 // changes: one row for each (run, gate) that meet, at slot run + gate (each step along the
 // rows raises one of the two, so no slot is shared).
 // What binds it first is the issue of instructions, with 16 warps an SM to cover their
-// latencies: 25 for each element are the mathematics.  So a warp whose columns all exist
-// takes a path without a comparison for each, and no more is kept in registers than 16
+// latencies: 25 for each element are the mathematics.  No more is kept in registers than 16
 // warps of 128 have room for.
-
-constexpr int kBwdThreads = 256;  // at most
 
 // Sums of a pair over the G warps of a row, the same in all of them.  red: the group's,
 // member: this warp's place in it.
@@ -249,8 +372,7 @@ __device__ __forceinline__ void pair_sums(float& u, float& v, float2* red, int G
     return;
   }
   if ((lane & 15) == 0) reinterpret_cast<float*>(red + member)[lane >> 4] = t;
-  // the CTA's barrier: its warps arrive from two places in the code
-  asm volatile("bar.sync 0;" ::: "memory");
+  group_barrier();
   u = v = 0.f;
   for (int i = 0; i < G; ++i) {
     const float2 p = red[i];
@@ -413,11 +535,11 @@ __device__ __forceinline__ void bwd_rows(const Args& a, const BwdArgs& p, const 
 }
 
 template <typename X, typename H, typename Y, int E, int W, bool kBias>
-__global__ void __launch_bounds__(kBwdThreads, E == 8 ? 2 : 1)
+__global__ void __launch_bounds__(kMaxThreads, E == 8 ? 2 : 1)
     bwd_kernel(const Args a, const BwdArgs p, const Y* dy, const X* dxo, X* dx, H* dh) {
   constexpr int K = E / W, kStep = 32 * W;
   __shared__ float2 red[2 * 8];
-  __shared__ float sums[kBwdThreads * E];
+  __shared__ float sums[kMaxThreads * E];
   const int C = a.C, warp = threadIdx.x >> 5, groups = p.G == 1 ? (int)blockDim.x >> 5 : 1;
   const int group = p.G == 1 ? warp : 0, member = p.G == 1 ? 0 : warp;
   const int c0 = member * 32 * E + (threadIdx.x & 31) * W;
@@ -466,11 +588,12 @@ struct Sums {
   int C, pitch, ctas;
 };
 
-// Column sums of the partial rows: blockIdx.y < kParts one parameter's gradient, else
-// that of gate blockIdx.y - kParts from the rows of the runs it meets.  A CTA takes 32 columns: thread (g, j) of
-// 32 x 8 adds rows g, g + 32, ... of four columns, then the 32 are added in order.
-__global__ void __launch_bounds__(256) sums_kernel(const Sums s) {
-  __shared__ float red[32][33];
+// Column sums of the partial rows: blockIdx.y < kParts one parameter's gradient, else that of
+// gate blockIdx.y - kParts from the rows of the runs it meets.  A CTA takes 32 columns: thread
+// (g, j) of 64 x 8 adds rows g, g + 64, ... of four columns, then the 64 are added in order.
+__global__ void __launch_bounds__(512) sums_kernel(const Sums s) {
+  constexpr int kGroups = 64;
+  __shared__ float red[kGroups][33];
   const int j = threadIdx.x & 7, grp = threadIdx.x >> 3;
   const int c = blockIdx.x * 32 + j * 4;
   const int y = blockIdx.y;
@@ -491,7 +614,7 @@ __global__ void __launch_bounds__(256) sums_kernel(const Sums s) {
   float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
   if (c < s.pitch) {
 #pragma unroll 8
-    for (int r = grp; r < count; r += 32) {
+    for (int r = grp; r < count; r += kGroups) {
       const float4 v = *reinterpret_cast<const float4*>(in + (size_t)r * s.pitch + c);
       t.x += v.x, t.y += v.y, t.z += v.z, t.w += v.w;
     }
@@ -499,14 +622,12 @@ __global__ void __launch_bounds__(256) sums_kernel(const Sums s) {
   red[grp][j * 4] = t.x, red[grp][j * 4 + 1] = t.y;
   red[grp][j * 4 + 2] = t.z, red[grp][j * 4 + 3] = t.w;
   __syncthreads();
-  // column of warp w's k-th turn: its 32 sums are one in each lane
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;  // two columns a warp
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int col = (threadIdx.x >> 5) * 4 + k, at = blockIdx.x * 32 + col;
-    float u = red[threadIdx.x & 31][col];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-    if ((threadIdx.x & 31) == 0 && at < s.C) out[at] = u;
+  for (int k = 0; k < 2; ++k) {
+    const int col = warp * 2 + k, at = blockIdx.x * 32 + col;
+    const float u = warp_sum(red[lane][col] + red[lane + 32][col]);
+    if (lane == 0 && at < s.C) out[at] = u;
   }
 }
 
@@ -516,22 +637,23 @@ bool aligned(const void* p, int bytes) {
 
 bool known(int dtype) { return dtype == SQB_BF16 || dtype == SQB_F32; }
 
-// How the backward deals out N rows of C columns: groups of G warps whose lanes hold E
-// columns (16 beyond 2048 columns, so that 8 warps do), as many CTAs of one group (or of eight
-// groups of one warp) on each of 148 SMs as their registers allow, runs of as many rows each.
+// How N rows of C columns are dealt out: groups of G warps whose lanes hold E columns (16
+// beyond 2048 columns, so that 8 warps do), as many CTAs of one group (or of eight groups of
+// one warp) on each of 148 SMs as `warps` (for E = 8) allow, runs of as many rows each.
 struct Plan {
   int G, E, groups, ctas, runs, pitch;
   uint32_t rows;
 };
 
+constexpr int kBwdWarps = 16, kFwdWarps = 24;
 constexpr int kMaxCtas = 148 * 8;
 
-Plan plan_of(int64_t N, int64_t C) {
+Plan plan_of(int64_t N, int64_t C, int warps) {
   Plan p;
   p.E = C <= 2048 ? 8 : 16;
   p.G = (int)((C + 32 * p.E - 1) / (32 * p.E));
   p.groups = p.G == 1 ? 8 : 1;
-  const int per_sm = (p.E == 8 ? 16 : 8) / (p.G * p.groups);
+  const int per_sm = (p.E == 8 ? warps : warps * 2 / 3 / 8 * 8) / (p.G * p.groups);
   const int64_t all = (int64_t)148 * per_sm * p.groups;
   p.rows = (uint32_t)((N + all - 1) / all);
   p.runs = (int)((N + p.rows - 1) / p.rows);
@@ -612,38 +734,36 @@ extern "C" int sqb_residual_norm_fwd(const void* x, int x_dtype, const void* h, 
   if (!aligned(stats, 16)) return SQB_ERR_ALIGN;
   cudaStream_t q = static_cast<cudaStream_t>(stream);
   const void* more[] = {x_out, y};
-  const bool w4 = wide(a, more, 2);
+  const bool w4 = wide(a, more, 2), biased = bias || post_bias;
+  const Plan p = plan_of(N, C, kFwdWarps);
   float4* st = reinterpret_cast<float4*>(stats);
   by_type(x_dtype, h_dtype, y_dtype, [&](auto tx, auto th, auto ty) {
     using X = decltype(tx);
     using H = decltype(th);
     using Y = decltype(ty);
-    X* xo = static_cast<X*>(x_out);
-    Y* yo = static_cast<Y*>(y);
-#define SQB_FWD(K, W, TH)                                                                     \
-  fwd_kernel<X, H, Y, K, W, TH>                                                               \
-      <<<(unsigned)((N + kFwdThreads / TH - 1) / (kFwdThreads / TH)), kFwdThreads, 0, q>>>( \
-          a, xo, yo, st)
-    if (w4) {
-      if (C <= 512)
-        SQB_FWD(4, 4, 32);
-      else if (C <= 768)
-        SQB_FWD(6, 4, 32);
-      else if (C <= 1024)
-        SQB_FWD(8, 4, 32);
-      else if (C <= 2048)
-        SQB_FWD(4, 4, 128);
+    auto run = [&](auto kernel) {
+      kernel<<<p.ctas, 32 * p.G * p.groups, 0, q>>>(a, static_cast<X*>(x_out),
+                                                    static_cast<Y*>(y), st, p.G, p.rows);
+    };
+    auto sized = [&](auto biased_) {
+      constexpr bool kb = decltype(biased_)::value;
+      if (p.E == 8)
+        w4 ? run(fwd_kernel<X, H, Y, 8, 4, kb>) : run(fwd_kernel<X, H, Y, 8, 1, kb>);
       else
-        SQB_FWD(4, 4, 256);
-    } else {
-      if (C <= 512)
-        SQB_FWD(16, 1, 32);
-      else if (C <= 2048)
-        SQB_FWD(16, 1, 128);
-      else
-        SQB_FWD(16, 1, 256);
-    }
-#undef SQB_FWD
+        w4 ? run(fwd_kernel<X, H, Y, 16, 4, kb>) : run(fwd_kernel<X, H, Y, 16, 1, kb>);
+    };
+    auto one_warp = [&](auto kernel) {
+      kernel<<<(unsigned)((N + 7) / 8), kMaxThreads, 0, q>>>(a, static_cast<X*>(x_out),
+                                                             static_cast<Y*>(y), st);
+    };
+    if (w4 && C <= 512)
+      one_warp(fwd_warp_kernel<X, H, Y, 4>);
+    else if (w4 && C <= 768)
+      one_warp(fwd_warp_kernel<X, H, Y, 6>);
+    else if (w4 && C <= 1024)
+      one_warp(fwd_warp_kernel<X, H, Y, 8>);
+    else
+      biased ? sized(std::true_type()) : sized(std::false_type());
   });
   return cudaGetLastError() == cudaSuccess ? SQB_OK : SQB_ERR_LAUNCH;
 }
@@ -678,7 +798,7 @@ extern "C" int sqb_residual_norm_bwd(const void* dy, int y_dtype, const void* dx
   cudaStream_t q = static_cast<cudaStream_t>(stream);
   const void* more[] = {dy, dx_out, dx, dh};
   const bool w4 = wide(a, more, 4), biased = bias || post_bias;
-  const Plan p = plan_of(N, C);
+  const Plan p = plan_of(N, C, kBwdWarps);
   float* parts = static_cast<float*>(workspace);
   float* gate_parts = gate && gates > 1 ? parts + (size_t)kParts * p.ctas * p.pitch : nullptr;
   const BwdArgs more_args{reinterpret_cast<const float4*>(stats), parts, gate_parts, p.pitch, p.G,
@@ -709,6 +829,6 @@ extern "C" int sqb_residual_norm_bwd(const void* dy, int y_dtype, const void* dx
   s.gate_parts = gate_parts, s.dgate = dgate;
   s.N = N, s.T = a.T, s.rows = p.rows, s.C = (int)C, s.pitch = p.pitch, s.ctas = p.ctas;
   const dim3 grid((unsigned)((C + 31) / 32), (unsigned)(kParts + (gate_parts ? gates : 0)));
-  sums_kernel<<<grid, 256, 0, q>>>(s);
+  sums_kernel<<<grid, 512, 0, q>>>(s);
   return cudaGetLastError() == cudaSuccess ? SQB_OK : SQB_ERR_LAUNCH;
 }
