@@ -333,20 +333,29 @@ __device__ void write_zeros(T* drow, int V) {
   if (tail < V) drow[tail] = from_f<T>(0.f);
 }
 
-// Log-probability of target t in 64 bits (NaN for a t past the vocabulary).
+// Log-probability of a target whose logit is x (NaN for one past the vocabulary).  In 64
+// bits, and never inlined, like the policy's terms: one thread of a row calls them, and what
+// registers they need is not to be taken from all the others.
+__device__ __noinline__ double logp_of(double x, float m, double s) {
+  return (x - (double)m) - log(s);
+}
 template <typename T>
 __device__ __forceinline__ double logp_of(const T* row, int V, int64_t t, float m, double s) {
-  if (t >= V) return NAN;
-  return ((double)to_f(row[t]) - (double)m) - log(s);
+  return logp_of(t < V ? (double)to_f(row[t]) : (double)NAN, m, s);
 }
 
 
 // ---- rows -------------------------------------------------------------------------
 
-constexpr int kRowThreads = 512;   // a CTA for each row
+// Threads of a row's CTA: of the kernels that only read it (4685 of 8192 rows of 50304 bf16:
+// 88 us, 92 with 512), and of those that write its gradient (193 us, 201 with 256).
+constexpr int kReadThreads = 256, kWriteThreads = 512;
 constexpr int kWarpRows = 8;       // or a warp, eight rows to a CTA
-// Rows up to this many bytes take a warp.
-constexpr int64_t kWarpRowBytes = 8192;
+// A warp takes a row of at most 2 KB, and one of up to 16 KB when there are rows for eight
+// warps on every SM.  Forward and backward, warp against CTA: 32768 rows of 1024 bf16 21 + 26
+// us, 59 + 121; 4096 of 8192 bf16 16 + 22, 17 + 31; 4096 of 16384 bf16 30 + 51, 28 + 43; 64
+// rows of 4096 bf16 4.7 + 4.5, 3.1 + 2.7.
+constexpr int64_t kWarpRowBytes = 16384, kFewRowBytes = 2048, kFewRows = 148 * 8;
 
 template <int kThreads>
 constexpr int block_of() {
@@ -421,30 +430,34 @@ struct Policy {
 };
 
 // term: {-min(ratio A, held A), KL, 1 if the held one counts}; returns d loss / d logp.
-__device__ double policy_terms(const Policy& p, uint32_t r, int64_t T, double lp, double* term) {
-  const uint32_t a = p.by_seq ? (p.seq ? (uint32_t)p.seq[r] : r / (uint32_t)T) : r;
-  const double A = p.adv[a];
-  const double ratio = p.old_logp ? exp(lp - (double)p.old_logp[r]) : exp(lp - lp);
-  const double kept = ratio < p.lo ? p.lo : ratio > p.hi ? p.hi : ratio;
+__device__ __noinline__ double policy_terms(double A, bool has_old, double old_logp,
+                                            bool has_ref, double ref_logp, double lo, double hi,
+                                            double kl_coef, double lp, double* term) {
+  const double ratio = has_old ? exp(lp - old_logp) : exp(lp - lp);
+  const double kept = ratio < lo ? lo : ratio > hi ? hi : ratio;
   const double open = ratio * A, held = kept * A;
   const bool clipped = held < open;
   term[0] = clipped ? -held : -open;
   term[2] = clipped ? 1.0 : 0.0;
   double d = clipped ? 0.0 : -open;
   term[1] = 0.0;
-  if (p.ref_logp) {
-    const double gap = (double)p.ref_logp[r] - lp;
-    term[1] = expm1(gap) - gap;
-    d -= p.kl_coef * expm1(gap);
+  if (has_ref) {
+    const double gap = ref_logp - lp, e = expm1(gap);
+    term[1] = e - gap;
+    d -= kl_coef * e;
   }
   return d;
 }
 
 
 // One row of the policy loss: log-probability, terms and d loss / d logp; with dx, also the
-// row's gradient times `scale`, the row read again where it is still in L2.
+// row's gradient times `scale`, the row read again where it is still in L2.  Launched while
+// the weights are still being counted: it waits for them once it has its sum.
+// Three CTAs of 512 threads an SM: 8192 rows of 50304 bf16, 4975 of them counted, 250 us, 5.3
+// TB/s.  Measured: four, 272 us (59 MB of rows between their two readings in L2); the row
+// kept in shared memory, two an SM, 284 us.
 template <typename T, int kThreads>
-__global__ void __launch_bounds__(block_of<kThreads>())
+__global__ void __launch_bounds__(block_of<kThreads>(), kThreads == 32 ? 1 : 1536 / kThreads)
     policy_kernel(const T* x, const int64_t* targets, Policy p, RowOut out, double* terms, T* dx,
                   float scale, View v, int64_t dss, int64_t dst, uint32_t N) {
   __shared__ Part red[32];
@@ -453,9 +466,8 @@ __global__ void __launch_bounds__(block_of<kThreads>())
   if (kThreads == 32 && r >= N) return;
   const int64_t t = targets[r];
   const int me = rank<kThreads>(), V = (int)v.V;
-  const float w = p.weight[r];
   T* drow = dx ? dx + row_offset(r, v.T, dss, dst) : nullptr;
-  if (t < 0 || w == 0.f) {
+  if (t < 0) {
     if (me == 0) {
       out.logp[r] = 0.f;
       if (out.stats) out.stats[r] = make_float2(0.f, 1.f);
@@ -466,15 +478,29 @@ __global__ void __launch_bounds__(block_of<kThreads>())
     return;
   }
   const T* row = x + row_offset(r, v.T, v.ss, v.st);
-  float m = 0.f;
+  float m = 0.f, old_logp = 0.f, ref_logp = 0.f;
   double s = 1.0;
+  if (me == 0) {
+    if (p.old_logp) old_logp = p.old_logp[r];
+    if (p.ref_logp) ref_logp = p.ref_logp[r];
+  }
   row_stats<T, kThreads>(row, V, red, m, s);
   float3 f;  // m, -g / s (0: a zero row) and g
   if (me == 0) {
-    double term[3];
     const double lp = logp_of(row, V, t, m, s);
-    const float g = (float)(policy_terms(p, r, v.T, lp, term) * (double)w);
-    out.logp[r] = (float)lp;
+    cudaGridDependencySynchronize();
+    const float w = p.weight[r];
+    double term[3] = {0.0, 0.0, 0.0};
+    float g = 0.f;
+    if (w != 0.f) {  // else outside every sequence: left out
+      const uint32_t a = p.by_seq ? (p.seq ? (uint32_t)p.seq[r] : r / (uint32_t)v.T) : r;
+      g = (float)(policy_terms(p.adv[a], p.old_logp, old_logp, p.ref_logp, ref_logp, p.lo, p.hi,
+                               p.kl_coef, lp, term) *
+                  (double)w);
+    } else {
+      m = 0.f, s = 1.0;
+    }
+    out.logp[r] = w != 0.f ? (float)lp : 0.f;
     if (out.stats) out.stats[r] = make_float2(m, (float)s);
     if (out.g_row) out.g_row[r] = g;
     terms[r] = term[0];
@@ -545,6 +571,7 @@ __global__ void __launch_bounds__(kSeqThreads)
   __shared__ double red[32];
   const int64_t p = blockIdx.x;
   int64_t a[2], b[2];
+  cudaGridDependencySynchronize();
   double ratio[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -570,6 +597,7 @@ __global__ void __launch_bounds__(kSeqThreads)
     preference_mean_kernel(const double* pair_loss, int64_t P, float* loss) {
   __shared__ double red[32];
   double v = 0.0;
+  cudaGridDependencySynchronize();
   for (int64_t p = threadIdx.x; p < P; p += kSeqThreads) v += pair_loss[p];
   v = block_sum(v, red);
   if (threadIdx.x == 0) *loss = (float)(v / (double)P);
@@ -585,6 +613,7 @@ __global__ void __launch_bounds__(kWeightThreads)
                           uint32_t N, bool per_sequence, uint32_t* counts, float* weight,
                           int32_t* seq) {
   __shared__ double red[32];
+  cudaTriggerProgrammaticLaunchCompletion();  // the rows' kernel may start
   for (uint32_t s = threadIdx.x; s < S; s += kWeightThreads) counts[s] = 0;
   __syncthreads();
   auto sequence = [&](uint32_t r) -> uint32_t {  // S for none
@@ -638,11 +667,12 @@ __global__ void __launch_bounds__(kWeightThreads)
                       float* loss, float* statistics) {
   __shared__ double red[32];
   double v[3] = {0.0, 0.0, 0.0};
+  cudaGridDependencySynchronize();
+#pragma unroll 4
   for (uint32_t r = threadIdx.x; r < N; r += kWeightThreads) {
-    const double w = weight[r];
-    if (w != 0.0)
+    const double w = weight[r];  // the terms of a row without weight are 0
 #pragma unroll
-      for (int k = 0; k < 3; ++k) v[k] += w * terms[k * (size_t)N + r];
+    for (int k = 0; k < 3; ++k) v[k] += w * terms[k * (size_t)N + r];
   }
 #pragma unroll
   for (int k = 0; k < 3; ++k) v[k] = block_sum(v[k], red);
@@ -658,15 +688,33 @@ bool dims_ok(int64_t S, int64_t T, int64_t V) {
   return S > 0 && T > 0 && V > 0 && V <= (1 << 30) && S <= INT32_MAX && T <= INT32_MAX / S;
 }
 
+// Launches a kernel that may start before the one in front of it on the stream has ended: it
+// waits for that one's results itself (cudaGridDependencySynchronize).
+template <typename... P, typename... A>
+void launch_early(void (*kernel)(P...), unsigned grid, unsigned block, cudaStream_t q, A... args) {
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(block);
+  config.stream = q;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
+}
+
 int launched() { return cudaGetLastError() == cudaSuccess ? SQB_OK : SQB_ERR_LAUNCH; }
 
-// Calls f(type, threads, grid) for the rows' type and width.
-template <typename F>
+// Calls f(type, threads, grid) for the rows' type and width: a warp for a short row, else a
+// CTA of kCta threads.
+template <int kCta, typename F>
 void dispatch(int dtype, int64_t N, int64_t V, F&& f) {
   const unsigned rows = (unsigned)N, packed = (unsigned)((N + kWarpRows - 1) / kWarpRows);
-  const bool warp = V * elt_of(dtype) <= kWarpRowBytes;
+  const int64_t bytes = V * elt_of(dtype);
+  const bool warp = bytes <= (N < kFewRows ? kFewRowBytes : kWarpRowBytes);
   using W = std::integral_constant<int, 32>;
-  using B = std::integral_constant<int, kRowThreads>;
+  using B = std::integral_constant<int, kCta>;
   if (dtype == SQB_BF16)
     warp ? f(__nv_bfloat16(), W(), packed) : f(__nv_bfloat16(), B(), rows);
   else
@@ -675,7 +723,7 @@ void dispatch(int dtype, int64_t N, int64_t V, F&& f) {
 
 void launch_logp(const void* x, const int64_t* targets, const RowOut& out, int64_t S, int64_t T,
                  int64_t V, int64_t ss, int64_t st, int dtype, cudaStream_t q) {
-  dispatch(dtype, S * T, V, [&](auto type, auto threads, unsigned grid) {
+  dispatch<kReadThreads>(dtype, S * T, V, [&](auto type, auto threads, unsigned grid) {
     using X = decltype(type);
     constexpr int kThreads = decltype(threads)::value;
     logp_fwd_kernel<X, kThreads><<<grid, block_of<kThreads>(), 0, q>>>(
@@ -708,7 +756,7 @@ extern "C" int sqb_logp_bwd(const void* logits, const int64_t* targets, const fl
   if (!logits || !targets || !stats || !g_row || !dlogits || !dims_ok(S, T, V))
     return SQB_ERR_ARG;
   if (!elt_of(dtype)) return SQB_ERR_DTYPE;
-  dispatch(dtype, S * T, V, [&](auto type, auto threads, unsigned grid) {
+  dispatch<kWriteThreads>(dtype, S * T, V, [&](auto type, auto threads, unsigned grid) {
     using X = decltype(type);
     constexpr int kThreads = decltype(threads)::value;
     logp_bwd_kernel<X, kThreads>
@@ -744,10 +792,14 @@ extern "C" int sqb_preference_fwd(const void* logits, const int64_t* targets,
   // rows of a packed batch that belong to no sequence keep the zero written here
   const RowOut out{nullptr, logp, reinterpret_cast<float2*>(stats), cu_seqlens ? g_row : nullptr};
   if (N > 0) launch_logp(logits, targets, out, S, T, V, ss, st, dtype, q);
-  preference_pair_kernel<<<(unsigned)P, kSeqThreads, 0, q>>>(logp, cu_seqlens, ref_logps, P, T, N,
-                                                             beta, label_smoothing, pair_loss,
-                                                             rewards, g_row);
-  preference_mean_kernel<<<1, kSeqThreads, 0, q>>>(pair_loss, P, loss);
+  if (N > 0)
+    launch_early(preference_pair_kernel, (unsigned)P, kSeqThreads, q, logp, cu_seqlens, ref_logps,
+                 P, T, N, beta, label_smoothing, pair_loss, rewards, g_row);
+  else
+    preference_pair_kernel<<<(unsigned)P, kSeqThreads, 0, q>>>(logp, cu_seqlens, ref_logps, P, T,
+                                                               N, beta, label_smoothing,
+                                                               pair_loss, rewards, g_row);
+  launch_early(preference_mean_kernel, 1, kSeqThreads, q, pair_loss, P, loss);
   return launched();
 }
 
@@ -785,14 +837,18 @@ extern "C" int sqb_policy_fwd(const void* logits, const int64_t* targets,
   const Policy p{old_logp,        ref_logp,       adv,    cu_seqlens ? seq : nullptr, weight,
                  adv_by_seq != 0, 1.0 - clip_low, 1.0 + clip_high, kl_coef};
   const RowOut out{logp, nullptr, reinterpret_cast<float2*>(stats), g_row};
-  dispatch(dtype, N, V, [&](auto type, auto threads, unsigned grid) {
+  auto rows = [&](auto type, auto threads, unsigned grid) {
     using X = decltype(type);
     constexpr int kThreads = decltype(threads)::value;
-    policy_kernel<X, kThreads><<<grid, block_of<kThreads>(), 0, q>>>(
-        static_cast<const X*>(logits), targets, p, out, terms, static_cast<X*>(dlogits),
-        grad_scale, View{T, V, ss, st}, dss, dst, (uint32_t)N);
-  });
-  policy_sum_kernel<<<1, kWeightThreads, 0, q>>>(terms, weight, (uint32_t)N, kl_coef, loss,
-                                                 statistics);
+    launch_early(policy_kernel<X, kThreads>, grid, block_of<kThreads>(), q,
+                 static_cast<const X*>(logits), targets, p, out, terms, static_cast<X*>(dlogits),
+                 grad_scale, View{T, V, ss, st}, dss, dst, (uint32_t)N);
+  };
+  if (dlogits)
+    dispatch<kWriteThreads>(dtype, N, V, rows);
+  else
+    dispatch<kReadThreads>(dtype, N, V, rows);
+  launch_early(policy_sum_kernel, 1, kWeightThreads, q, terms, weight, (uint32_t)N, kl_coef, loss,
+               statistics);
   return launched();
 }

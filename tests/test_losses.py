@@ -402,8 +402,11 @@ def test_policy_loss(S, T, V, per_token, kl, reduction, with_old, layout, dtype)
                                                          **kw)
     assert not grad.requires_grad
     check_grad(grad, torch.where(shown, gx, 0.0) * 2, x, tt, g_row * 2, g_err * 2)
-    # the same terms, added in the same order
-    assert torch.equal(one, loss) and torch.equal(logps1, logps) and torch.equal(stats1, stats)
+    # (the two forms may give a row to different numbers of threads: not the same bits)
+    assert_within(one, w_loss, loss_err + 1e-30, "loss, one pass")
+    assert_within(stats1, w_stats, stat_err + 1e-30, "statistics, one pass")
+    assert_within(logps1, lp, torch.where(keep.view(t.shape), rel(V) + lp.abs() * 2 * U, 0.0),
+                  "logps, one pass")
 
 
 @pytest.mark.gpu
