@@ -5,6 +5,9 @@
 b = round_up(ceil(sqrt(T)), 16) for the running sequence length T.
 ``sqrt_block_impl``: kernel family, "auto" (tcgen05 where supported), "simt"
 or "tcgen05".
+``post_norm``: a second LayerNorm on each attention's and MLP's output, before the
+residual add.  ``layer_scale``: initial value of a learned gate for each channel of that
+output (None: no gate).  Both are off in the reference's models.
 """
 
 from __future__ import annotations
@@ -25,6 +28,8 @@ class ModelConfig:
     attention: str = "sqrt_block"
     sqrt_block_b: Optional[int] = None
     sqrt_block_impl: str = "auto"
+    post_norm: bool = False
+    layer_scale: Optional[float] = None
 
 
 def gpt2_small(**kw) -> ModelConfig:

@@ -2,7 +2,7 @@
 
 from __future__ import annotations
 
-import ctypes
+import array
 import math
 
 import torch
@@ -16,8 +16,6 @@ _DTYPES = {torch.float32: _lib.SQB_F32, torch.bfloat16: _lib.SQB_BF16}
 
 def _dense(t):
     """Whether t's elements fill one run of memory, in whatever order."""
-    if t.is_contiguous():
-        return True
     at = 1
     for stride, size in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
         if stride != at:
@@ -29,14 +27,17 @@ def _dense(t):
 def _checked(fn, tensors, what="gradients"):
     """The device of `tensors`, all of them strided CUDA float32 or bfloat16 on it."""
     device = tensors[0].device
-    for t in tensors:
-        if t.layout != torch.strided:
-            raise ValueError(f"{fn}: {what} must be strided tensors, got layout {t.layout}")
-        if t.dtype not in _DTYPES:
-            raise TypeError(f"{fn} supports float32 and bfloat16, got {t.dtype}")
-        if t.device != device:
-            raise ValueError(f"{fn}: {what} are on {device} and {t.device}: one call takes one "
-                             "device")
+    if ({t.layout for t in tensors} != {torch.strided}
+            or not {t.dtype for t in tensors} <= _DTYPES.keys()
+            or {t.device for t in tensors} != {device}):
+        for t in tensors:
+            if t.layout != torch.strided:
+                raise ValueError(f"{fn}: {what} must be strided tensors, got layout {t.layout}")
+            if t.dtype not in _DTYPES:
+                raise TypeError(f"{fn} supports float32 and bfloat16, got {t.dtype}")
+            if t.device != device:
+                raise ValueError(f"{fn}: {what} are on {device} and {t.device}: one call takes "
+                                 "one device")
     if device.type != "cuda":
         raise RuntimeError(f"{fn}: {what} must be CUDA tensors (the op has no CPU "
                            "implementation)")
@@ -44,13 +45,17 @@ def _checked(fn, tensors, what="gradients"):
 
 
 def _tables(tensors):
-    n = len(tensors)
-    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors]),
-            (ctypes.c_int32 * n)(*[_DTYPES[t.dtype] for t in tensors]))
+    """Host arrays of the tensors' pointers and dtypes."""
+    return (array.array("Q", [t.data_ptr() for t in tensors]),
+            array.array("i", [_DTYPES[t.dtype] for t in tensors]))
 
 
 def _numels(tensors):
-    return (ctypes.c_int64 * len(tensors))(*[t.numel() for t in tensors])
+    return array.array("q", [t.numel() for t in tensors])
+
+
+def _at(table):
+    return table.buffer_info()[0]
 
 
 def _workspace(n, device):
@@ -66,25 +71,25 @@ def grad_norm(tensors):
     if not tensors:
         return torch.tensor(0.0)
     device = _checked("grad_norm", tensors, "tensors")
-    tensors = [t if _dense(t) else t.contiguous() for t in tensors]
+    tensors = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in tensors]
     norm = torch.empty((), dtype=torch.float32, device=device)
-    ptrs, dtypes = _tables(tensors)
+    (ptrs, dtypes), numels = _tables(tensors), _numels(tensors)
     ws, nbytes = _workspace(len(tensors), device)
     with _lib.on_device(device):
         _lib.check("sqb_grad_norm", _lib.lib().sqb_grad_norm(
-            ptrs, _numels(tensors), dtypes, len(tensors), ws.data_ptr(), nbytes,
+            _at(ptrs), _at(numels), _at(dtypes), len(tensors), ws.data_ptr(), nbytes,
             norm.data_ptr(), _lib.stream(device)))
     return norm
 
 
 def _clip(grads, outs, max_norm, device):
     norm = torch.empty((), dtype=torch.float32, device=device)
-    ptrs, dtypes = _tables(grads)
+    (ptrs, dtypes), numels = _tables(grads), _numels(grads)
     out_ptrs, out_dtypes = (ptrs, dtypes) if outs is grads else _tables(outs)
     ws, nbytes = _workspace(len(grads), device)
     with _lib.on_device(device):
         _lib.check("sqb_grad_clip", _lib.lib().sqb_grad_clip(
-            ptrs, out_ptrs, _numels(grads), dtypes, out_dtypes, len(grads), max_norm,
+            _at(ptrs), _at(out_ptrs), _at(numels), _at(dtypes), _at(out_dtypes), len(grads), max_norm,
             ws.data_ptr(), nbytes, norm.data_ptr(),
             _lib.stream(device)))
     return norm
@@ -109,18 +114,20 @@ def clip_grads(grads, max_norm, out=None):
     if not grads:
         return [], torch.tensor(0.0)
     device = _checked(fn, grads)
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    if not all([g.is_contiguous() for g in grads]):
+        grads = [g.contiguous() for g in grads]
     if out is None:
         out = [torch.empty_like(g) for g in grads]
     else:
         out = list(out)
-        if len(out) != len(grads) or any(o.shape != g.shape for o, g in zip(out, grads)):
+        if [o.shape for o in out] != [g.shape for g in grads]:
             raise ValueError(f"{fn}: out must hold one tensor of each gradient's shape")
         if _checked(fn, out, "out") != device:
             raise ValueError(f"{fn}: out must be on the gradients' device, {device}")
-        if not all(o.is_contiguous() for o in out):
+        if not all([o.is_contiguous() for o in out]):
             raise ValueError(f"{fn}: out must be contiguous")
-        if len({o.data_ptr() for o in out if o.numel()}) < sum(o.numel() > 0 for o in out):
+        at = [o.data_ptr() for o in out if o.numel()]
+        if len(set(at)) < len(at):
             raise ValueError(f"{fn}: out holds one tensor twice")
     return out, _clip(grads, out, max_norm, device)
 
@@ -142,14 +149,14 @@ def clip_grad_norm_(parameters, max_norm):
     if not grads:
         return torch.tensor(0.0)
     device = _checked(fn, grads)
-    if all(map(_dense, grads)):
+    if all([g.is_contiguous() or _dense(g) for g in grads]):
         return _clip(grads, grads, max_norm, device)
     # a gradient with gaps (a view of a larger buffer) goes through a copy
     for g in grads:
         if any(s == 0 and n > 1 for n, s in zip(g.shape, g.stride())):
             raise ValueError(f"{fn}: a gradient expanded over its own memory cannot be scaled "
                              "in place")
-    work = [g if _dense(g) else g.contiguous() for g in grads]
+    work = [g if g.is_contiguous() or _dense(g) else g.contiguous() for g in grads]
     norm = _clip(work, work, max_norm, device)
     for g, w in zip(grads, work):
         if w is not g:

@@ -17,7 +17,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ..ops import add_layer_norm, add_layer_norm_supported, layer_norm, layer_norm_supported
+from ..ops import (add_layer_norm, add_layer_norm_supported, layer_norm, layer_norm_supported,
+                   residual_norm)
 from .attention_registry import build_attention
 
 
@@ -45,16 +46,35 @@ class LayerNorm(nn.Module):
                 return layer_norm(x, self.ln.weight, self.ln.bias, self.ln.eps, out)
         return self.ln(x)
 
-    def add_forward(self, x, h):
+    def add_forward(self, x, h, post=None, gate=None):
         """(x + h, this LayerNorm of x + h): the residual add and the LayerNorm
         that reads its sum, as one kernel each way on the CUDA fp32 residual
-        stream (the same fp32 sum and LayerNorm as the two separate ops)."""
+        stream (the same fp32 sum and LayerNorm as the two separate ops).  With
+        ``post`` (a LayerNorm) or ``gate`` (C,) the block's output goes through
+        them first, in the same kernel: x + gate * post(h)."""
+        if post is not None or gate is not None:
+            if residual_step_fused(x, h):
+                ln, out = post.ln if post is not None else None, self._out_dtype()
+                return residual_norm(
+                    x, h, self.ln.weight, self.ln.bias, gate=gate, eps=self.ln.eps,
+                    post_weight=ln.weight if ln is not None else None,
+                    post_bias=ln.bias if ln is not None else None, out_dtype=out)
+            h = post(h) if post is not None else h
+            x = x + (h if gate is None else gate * h)
+            return x, self(x)
         if add_layer_norm_supported(x, h, self.ln.weight):
             out = self._out_dtype()
             if out is not None:
                 return add_layer_norm(x, h, self.ln.weight, self.ln.bias, self.ln.eps, out)
         x = x + h
         return x, self(x)
+
+
+def residual_step_fused(x, h) -> bool:
+    """Whether ``add_forward`` with a post norm or a gate runs as the library's kernel."""
+    kinds = (torch.float32, torch.bfloat16)
+    return (x.is_cuda and x.dtype in kinds and h.dtype in kinds and x.shape[-1] <= 4096
+            and LayerNorm._out_dtype() is not None)
 
 
 class MLP(nn.Module):
@@ -76,10 +96,24 @@ class Attention_Block(nn.Module):  # noqa: N801  (reference class name)
         self.attn = build_attention(config)
         self.lm2 = LayerNorm(config.n_embd, bias=config.bias)
         self.mlp = MLP(config)
+        # what a block's outputs go through before the residual add: a second
+        # LayerNorm and a gate for each channel, if the config has them
+        post = getattr(config, "post_norm", False)
+        self.lp1 = LayerNorm(config.n_embd, bias=config.bias) if post else None
+        self.lp2 = LayerNorm(config.n_embd, bias=config.bias) if post else None
+        scale = getattr(config, "layer_scale", None)
+        for name in ("gate1", "gate2"):
+            self.register_parameter(name, None if scale is None else nn.Parameter(
+                torch.full((config.n_embd,), float(scale))))
+
+    @staticmethod
+    def _out(y, post, gate):
+        y = post(y) if post is not None else y
+        return y if gate is None else gate * y
 
     def forward(self, x):
-        x = x + self.attn(self.lm1(x))
-        x = x + self.mlp(self.lm2(x))
+        x = x + self._out(self.attn(self.lm1(x)), self.lp1, self.gate1)
+        x = x + self._out(self.mlp(self.lm2(x)), self.lp2, self.gate2)
         return x
 
 
@@ -146,9 +180,9 @@ class GPT(nn.Module):
         blocks = self.transformer.attn_blocks
         h = (blocks[0].lm1 if len(blocks) else self.transformer.ln_)(x)
         for i, block in enumerate(blocks):
-            x, y = block.lm2.add_forward(x, block.attn(h))
+            x, y = block.lm2.add_forward(x, block.attn(h), block.lp1, block.gate1)
             nxt = blocks[i + 1].lm1 if i + 1 < len(blocks) else self.transformer.ln_
-            x, h = nxt.add_forward(x, block.mlp(y))
+            x, h = nxt.add_forward(x, block.mlp(y), block.lp2, block.gate2)
         V = self.config.vocab_size
         if not pad_vocab or V % self.VOCAB_ALIGN == 0:
             return self.lm_head(h)

@@ -20,7 +20,7 @@ import torch
 import torch.nn.functional as F
 
 from .model.gpt import GPT
-from .ops import check_status, cross_entropy
+from .ops import check_status, clip_grad_norm_, cross_entropy
 
 
 def calculate_loss(logits, targets):
@@ -98,7 +98,9 @@ class Trainer:
         with span("backward"):
             loss.backward()
         with span("optimizer"):
-            norm = torch.nn.utils.clip_grad_norm_(self.model.parameters(), 1.0)
+            clip = (clip_grad_norm_ if self.device.type == "cuda"
+                    else torch.nn.utils.clip_grad_norm_)
+            norm = clip(self.model.parameters(), 1.0)
             self.optimizer.step()
         return loss.detach(), norm
 
