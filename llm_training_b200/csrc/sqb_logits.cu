@@ -280,8 +280,22 @@ __device__ void row_stats(const T* row, int V, Part* red, float& m, double& s) {
   s *= 1.0 + kExp2Short + y * (1.0 + y * (0.5 + y * (1.0 / 6 + y / 24)));
 }
 
+// A vector's load and store; kLast: nothing of either is wanted in L2 any longer (where rows
+// that will be read a second time lie).
+template <bool kLast>
+__device__ __forceinline__ uint4 get(const uint4* p) {
+  return kLast ? __ldcs(p) : *p;
+}
+template <bool kLast>
+__device__ __forceinline__ void put(uint4* p, uint4 v) {
+  if (kLast)
+    __stcs(p, v);
+  else
+    *p = v;
+}
+
 // drow[c] = g [c == t] + k exp(row[c] - m) for c < V, k = -g / s, by the group.
-template <typename T, int kThreads>
+template <typename T, int kThreads, bool kLast>
 __device__ void write_grad(const T* row, T* drow, int V, int64_t t, float m, float k, float g) {
   constexpr int kN = 16 / sizeof(T);
   const int me = rank<kThreads>();
@@ -309,11 +323,11 @@ __device__ void write_grad(const T* row, T* drow, int V, int64_t t, float m, flo
   for (; i + (kUnroll - 1) * kThreads < nvec; i += kUnroll * kThreads) {
     uint4 u[kUnroll];
 #pragma unroll
-    for (int j = 0; j < kUnroll; ++j) u[j] = body[i + j * kThreads];
+    for (int j = 0; j < kUnroll; ++j) u[j] = get<kLast>(body + i + j * kThreads);
 #pragma unroll
-    for (int j = 0; j < kUnroll; ++j) out[i + j * kThreads] = vector(u[j]);
+    for (int j = 0; j < kUnroll; ++j) put<kLast>(out + i + j * kThreads, vector(u[j]));
   }
-  for (; i < nvec; i += kThreads) out[i] = vector(body[i]);
+  for (; i < nvec; i += kThreads) put<kLast>(out + i, vector(get<kLast>(body + i)));
   const int tail = head + nvec * kN + me;
   if (tail < V) drow[tail] = grad(to_f(row[tail]), tail);
   // the target's element, by the thread that wrote its vector
@@ -322,13 +336,13 @@ __device__ void write_grad(const T* row, T* drow, int V, int64_t t, float m, flo
     drow[t] = grad(to_f(row[t]), (int)t);
 }
 
-template <typename T, int kThreads>
+template <typename T, int kThreads, bool kLast>
 __device__ void write_zeros(T* drow, int V) {
   constexpr int kN = 16 / sizeof(T);
   const int head = head_of(drow, V), nvec = (V - head) / kN, me = rank<kThreads>();
   if (me < head) drow[me] = from_f<T>(0.f);
   uint4* out = reinterpret_cast<uint4*>(drow + head);
-  for (int i = me; i < nvec; i += kThreads) out[i] = make_uint4(0, 0, 0, 0);
+  for (int i = me; i < nvec; i += kThreads) put<kLast>(out + i, make_uint4(0, 0, 0, 0));
   const int tail = head + nvec * kN + me;
   if (tail < V) drow[tail] = from_f<T>(0.f);
 }
@@ -412,9 +426,9 @@ __global__ void __launch_bounds__(block_of<kThreads>())
   // a zero factor (an ignored token, a clipped one) makes a zero row, which needs no
   // logits - unless they hold a NaN or an infinity, which the sum then shows
   if (t < 0 || (g == 0.f && isfinite(ms.x) && isfinite(ms.y)))
-    write_zeros<T, kThreads>(drow, (int)v.V);
+    write_zeros<T, kThreads, false>(drow, (int)v.V);
   else
-    write_grad<T, kThreads>(x + row_offset(r, v.T, v.ss, v.st), drow, (int)v.V, t, ms.x,
+    write_grad<T, kThreads, false>(x + row_offset(r, v.T, v.ss, v.st), drow, (int)v.V, t, ms.x,
                             -g / ms.y, g);
 }
 
@@ -453,9 +467,11 @@ __device__ __noinline__ double policy_terms(double A, bool has_old, double old_l
 // One row of the policy loss: log-probability, terms and d loss / d logp; with dx, also the
 // row's gradient times `scale`, the row read again where it is still in L2.  Launched while
 // the weights are still being counted: it waits for them once it has its sum.
-// Three CTAs of 512 threads an SM: 8192 rows of 50304 bf16, 4975 of them counted, 250 us, 5.3
-// TB/s.  Measured: four, 272 us (59 MB of rows between their two readings in L2); the row
-// kept in shared memory, two an SM, 284 us.
+// Three CTAs of 512 threads an SM, the second reading and the gradient passing through L2 as
+// what is needed last: 8192 rows of 50304 bf16, 4975 of them counted, 237 us, 5.6 TB/s of the
+// 1.32 GB it cannot do without.  Measured: 250 us without those hints, 272 with four CTAs
+// besides (59 MB of rows wait in L2 between their readings; 234 with the hints and some
+// spilled registers); the row kept in shared memory, two an SM, 284 us.
 template <typename T, int kThreads>
 __global__ void __launch_bounds__(block_of<kThreads>(), kThreads == 32 ? 1 : 1536 / kThreads)
     policy_kernel(const T* x, const int64_t* targets, Policy p, RowOut out, double* terms, T* dx,
@@ -474,7 +490,7 @@ __global__ void __launch_bounds__(block_of<kThreads>(), kThreads == 32 ? 1 : 153
       if (out.g_row) out.g_row[r] = 0.f;
       terms[r] = terms[(size_t)N + r] = terms[2 * (size_t)N + r] = 0.0;
     }
-    if (dx) write_zeros<T, kThreads>(drow, V);
+    if (dx) write_zeros<T, kThreads, true>(drow, V);
     return;
   }
   const T* row = x + row_offset(r, v.T, v.ss, v.st);
@@ -520,9 +536,9 @@ __global__ void __launch_bounds__(block_of<kThreads>(), kThreads == 32 ? 1 : 153
     f = known;
   }
   if (f.y == 0.f && f.z == 0.f)
-    write_zeros<T, kThreads>(drow, V);
+    write_zeros<T, kThreads, true>(drow, V);
   else
-    write_grad<T, kThreads>(row, drow, V, t, f.x, f.y, f.z);
+    write_grad<T, kThreads, true>(row, drow, V, t, f.x, f.y, f.z);
 }
 
 // ---- sequences ------------------------------------------------------------------
