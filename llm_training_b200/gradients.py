@@ -89,9 +89,10 @@ def _clip(grads, outs, max_norm, device):
     ws, nbytes = _workspace(len(grads), device)
     with _lib.on_device(device):
         _lib.check("sqb_grad_clip", _lib.lib().sqb_grad_clip(
-            _at(ptrs), _at(out_ptrs), _at(numels), _at(dtypes), _at(out_dtypes), len(grads), max_norm,
-            ws.data_ptr(), nbytes, norm.data_ptr(),
-            _lib.stream(device)))
+            _at(ptrs), _at(out_ptrs), _at(numels), _at(dtypes), _at(out_dtypes), len(grads),
+            max_norm, ws.data_ptr(), nbytes, norm.data_ptr(), _lib.stream(device)))
+    # written behind autograd's back
+    torch.autograd.graph.increment_version([o for o in outs if not o.is_inference()])
     return norm
 
 

@@ -9,7 +9,8 @@ packed, logits (N, V) with targets (N,) and ``cu_seqlens`` (S + 1,), the sequenc
 first rows and their end, non-decreasing; rows outside ``[cu_seqlens[0],
 cu_seqlens[S])`` are left out too.  A target past the vocabulary is never read: its
 log-probability and gradient row are NaN, as is everything summed from them.  Gradients
-reach the logits only, in their dtype and with their strides.
+reach the logits only, once (a second derivative is refused), in the logits' dtype and, as
+far as those leave no large gaps, with their strides.
 """
 
 from __future__ import annotations
@@ -18,6 +19,8 @@ import math
 from typing import Optional
 
 import torch
+
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -31,16 +34,35 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
+def _grad_strides(x):
+    """Strides for the gradient: x's, or where x's rows lie far apart (a few tokens of a longer
+    batch) ones without the gaps, that keep every row's place between 16-byte boundaries."""
+    strides = x.stride()
+    if x.numel() == 0 or 1 + sum((n - 1) * s for n, s in zip(x.shape, strides)) <= 2 * x.numel():
+        return strides
+    step, got = 16 // x.element_size(), [1]
+    span = x.shape[-1]
+    for n, s in zip(reversed(x.shape[:-1]), reversed(strides[:-1])):
+        span += (s - span) % step
+        got.append(span)
+        span *= n
+    return tuple(reversed(got))
+
+
 def _grad_like(x):
-    """An uninitialised tensor of x's shape, strides and 16-byte phase (the gradient is
-    written with the vector stores the logits are read with)."""
-    elt = x.element_size()
-    phase = x.data_ptr() % 16 // elt
+    """An uninitialised gradient of x: its shape and the 16-byte phase of each of its rows (it
+    is written with the vector stores the logits are read with)."""
+    strides = _grad_strides(x)
+    phase = x.data_ptr() % 16 // x.element_size()
     if phase == 0 or x.numel() == 0:
-        return torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=x.device)
-    span = 1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+        return torch.empty_strided(x.shape, strides, dtype=x.dtype, device=x.device)
+    span = 1 + sum((n - 1) * s for n, s in zip(x.shape, strides))
     buf = torch.empty(span + phase, dtype=x.dtype, device=x.device)
-    return buf.as_strided(x.shape, x.stride(), phase)
+    return buf.as_strided(x.shape, strides, phase)
+
+
+def _fake_grad(x):
+    return torch.empty_strided(x.shape, _grad_strides(x), dtype=x.dtype, device=x.device)
 
 
 # ---- the operators --------------------------------------------------------------------
@@ -98,8 +120,8 @@ def _(x, t):
 
 def _logp_bwd_raw(x: torch.Tensor, t: torch.Tensor, stats: torch.Tensor,
                   g_row: Optional[torch.Tensor], scale: Optional[torch.Tensor]) -> torch.Tensor:
-    """g_row[r] * scale * ([c == t] - softmax) in x's dtype and strides; without a g_row the
-    factors follow the row statistics."""
+    """g_row[r] * scale * ([c == t] - softmax) in x's dtype; without a g_row the factors follow
+    the row statistics."""
     S, T, V, ss, st = _dims(x)
     dx = _grad_like(x)
     if S * T:
@@ -107,7 +129,7 @@ def _logp_bwd_raw(x: torch.Tensor, t: torch.Tensor, stats: torch.Tensor,
         with _lib.on_device(x.device):
             _lib.check("sqb_logp_bwd", _lib.lib().sqb_logp_bwd(
                 x.data_ptr(), t.data_ptr(), stats.data_ptr(), g, _ptr(scale), dx.data_ptr(), S,
-                T, V, ss, st, ss, st, _DTYPES[x.dtype], _lib.stream(x.device)))
+                T, V, ss, st, *_dims(dx)[3:], _DTYPES[x.dtype], _lib.stream(x.device)))
     return dx
 
 
@@ -116,7 +138,7 @@ _logp_bwd = torch.library.custom_op("sqrtblock::logp_bwd", _logp_bwd_raw, mutate
 
 @_logp_bwd.register_fake
 def _(x, t, stats, g_row, scale):
-    return torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=x.device)
+    return _fake_grad(x)
 
 
 def _rows_grad(x, *args):
@@ -143,7 +165,7 @@ class _LogP(torch.autograd.Function):
         _logp_setup(ctx, args, out)
         return out
 
-    backward = staticmethod(_logp_grad)
+    backward = staticmethod(once_differentiable(_logp_grad))
 
 
 def _preference_raw(x: torch.Tensor, t: torch.Tensor, ref: Optional[torch.Tensor],
@@ -208,7 +230,7 @@ class _Preference(torch.autograd.Function):
         _preference_setup(ctx, args, out)
         return out
 
-    backward = staticmethod(_preference_grad)
+    backward = staticmethod(once_differentiable(_preference_grad))
 
 
 def _policy_raw(x: torch.Tensor, t: torch.Tensor, adv: torch.Tensor,
@@ -237,7 +259,8 @@ def _policy_raw(x: torch.Tensor, t: torch.Tensor, adv: torch.Tensor,
             adv_by_seq, clip_low, clip_high, kl_coef, per_seq, loss.data_ptr(),
             statistics.data_ptr(), logps.data_ptr(), None if fused else at,
             None if fused else at + 8 * N, at if fused else None, grad_scale if fused else 1.0,
-            S, T, V, ss, st, ss, st, _DTYPES[x.dtype], ws.data_ptr(), nbytes, _lib.stream(x.device)))
+            S, T, V, ss, st, *(_dims(last)[3:] if fused else (ss, st)), _DTYPES[x.dtype],
+            ws.data_ptr(), nbytes, _lib.stream(x.device)))
     return loss, logps, statistics, last
 
 
@@ -248,8 +271,7 @@ _policy_fwd = torch.library.custom_op("sqrtblock::policy_fwd", _policy_raw, muta
 def _(x, t, adv, old, ref, cu, seqs, adv_by_seq, per_seq, clip_low, clip_high, kl_coef,
       grad_scale):
     f32 = torch.float32
-    last = (torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=x.device)
-            if grad_scale is not None else x.new_empty(3 * t.numel(), dtype=f32))
+    last = _fake_grad(x) if grad_scale is not None else x.new_empty(3 * t.numel(), dtype=f32)
     return (x.new_empty((), dtype=f32), x.new_empty(t.shape, dtype=f32),
             x.new_empty(3, dtype=f32), last)
 
@@ -277,7 +299,7 @@ class _Policy(torch.autograd.Function):
         _policy_setup(ctx, args, out)
         return out
 
-    backward = staticmethod(_policy_grad)
+    backward = staticmethod(once_differentiable(_policy_grad))
 
 
 # ---- public entry points --------------------------------------------------------------
@@ -448,7 +470,7 @@ def policy_loss_and_grad(logits, targets, advantages, old_logps=None, ref_logps=
     """``policy_loss`` and its gradient in one pass over the logits -> (loss, gradient,
     log-probabilities, statistics).
 
-    The gradient (the logits' shape, dtype and strides) is that of ``grad_scale * loss``;
+    The gradient (the logits' shape and dtype) is that of ``grad_scale * loss``;
     hand it on with ``logits.backward(gradient)``.  A token's factor needs its own row
     only, so each row is read from HBM once and its gradient written once, where the
     autograd form reads the logits a second time."""

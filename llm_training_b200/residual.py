@@ -7,6 +7,8 @@ from typing import Optional
 
 import torch
 
+from torch.autograd.function import once_differentiable
+
 from . import _lib
 
 __all__ = ["residual_norm"]
@@ -132,7 +134,7 @@ class _Residual(torch.autograd.Function):
         _setup(ctx, args, out)
         return out
 
-    backward = staticmethod(_grad)
+    backward = staticmethod(once_differentiable(_grad))
 
 
 def _run(*args):
@@ -182,7 +184,7 @@ def residual_norm(x, h, weight, bias=None, *, post_weight=None, post_bias=None, 
     LayerNorm, "rms" an RMS norm (no mean).  ``gate`` is (C,), or one row for each sample
     of x's first dimension: (B, C) or (B, 1, ..., C).  All math is fp32, each output
     rounded once (y is the norm of x' before x' is rounded to bfloat16); weights and gates
-    may be bfloat16.  Differentiable in every tensor (``sqrtblock::residual_norm_fwd/bwd``);
+    may be bfloat16.  Differentiable, once, in every tensor (``sqrtblock::residual_norm_fwd/bwd``);
     parameter gradients are summed in a fixed order (bit-reproducible)."""
     if not x.is_cuda:
         raise RuntimeError("residual_norm: x must be a CUDA tensor (the op has no CPU "

@@ -220,6 +220,18 @@ def test_layouts_and_parameters_listed_twice():
 
 
 @pytest.mark.gpu
+def test_autograd_sees_the_write():
+    """A graph that holds a tensor scaled in place says so, as after any in-place operation."""
+    p = torch.nn.Parameter(torch.zeros(8, device="cuda"))
+    w = torch.ones(8, device="cuda", requires_grad=True)
+    p.grad = torch.full((8,), 3.0, device="cuda")
+    loss = (w * p.grad).sum()
+    ops.clip_grad_norm_([p], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@pytest.mark.gpu
 def test_captured_and_on_two_streams():
     grads = tensors([(768, 300), (77,)], (F32,))
     src = [g.clone() for g in grads]

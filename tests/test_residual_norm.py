@@ -306,6 +306,15 @@ def test_bf16_parameters_get_bf16_gradients_and_one_output_unused():
 
 
 @pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    x = torch.randn(3, 64, device="cuda", requires_grad=True)
+    _, y = ops.residual_norm(x, x.detach(), torch.ones(64, device="cuda"))
+    (g,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)
+
+
+@pytest.mark.gpu
 def test_no_rows():
     x = torch.empty(0, 5, 64, device="cuda", requires_grad=True)
     w = torch.ones(64, device="cuda", requires_grad=True)
