@@ -373,11 +373,74 @@ __device__ __forceinline__ void pair_sums(float& u, float& v, float2* red, int G
   }
   if ((lane & 15) == 0) reinterpret_cast<float*>(red + member)[lane >> 4] = t;
   group_barrier();
-  u = v = 0.f;
-  for (int i = 0; i < G; ++i) {
-    const float2 p = red[i];
-    u += p.x, v += p.y;
+  // the places of members that are not there hold zeros
+  const float4* all = reinterpret_cast<const float4*>(red);
+  const float4 p = all[0], q = all[1];
+  u = (p.x + p.z) + (q.x + q.z);
+  v = (p.y + p.w) + (q.y + q.w);
+  if (G > 4) {
+    const float4 r = all[2], t = all[3];
+    u += (r.x + r.z) + (t.x + t.z);
+    v += (r.y + r.w) + (t.y + t.w);
   }
+}
+
+// A warp's 32 E columns of a row on their way through shared memory, a row ahead of its use:
+// the next row's loads then neither wait for this one's barriers nor take registers.
+// Four elements a lane: each lane copies and reads its own.  Single elements: the warp copies
+// the stretch in whole 16-byte pieces, from the boundary before it to the one after (other
+// elements there are not used), so that rows of any phase arrive at full speed; a piece that
+// would reach past the tensor is copied element by element.
+template <typename T, int E>
+__host__ __device__ constexpr int stage_bytes() {
+  return 32 * E * (int)sizeof(T) + 32;
+}
+
+template <typename X, typename H, typename Y, int E>
+__host__ __device__ constexpr int bwd_slot() {  // x, dx', h and dy
+  return 2 * stage_bytes<X, E>() + stage_bytes<H, E>() + stage_bytes<Y, E>();
+}
+
+template <int kBytes>
+__device__ __forceinline__ void cp_async(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(kBytes)
+               : "memory");
+}
+
+// Starts the copy of elements [at, at + n) of p, which has `all`, to `to` (kFull: n = 32 E), of
+// which `to_shared` is the address in shared memory.
+template <typename T, int E, int W, bool kFull>
+__device__ __forceinline__ void stage_in(char* to, uint32_t to_shared, const T* p, size_t at, int n,
+                                         size_t all) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (W == 4) {
+    const T* from = p + at + lane * 4;
+    to_shared += lane * 4 * sizeof(T);
+#pragma unroll
+    for (int k = 0; k < E / 4; ++k)
+      if (kFull || (k * 32 + lane) * 4 < n)
+        cp_async<4 * sizeof(T)>(to_shared + k * 128 * sizeof(T), from + k * 128);
+  } else {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(p + at), first = from & ~(uintptr_t)15;
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(p), hi = reinterpret_cast<uintptr_t>(p + all);
+    const int pieces = (int)((from + n * sizeof(T) - first + 15) / 16);
+    for (int i = lane; i < pieces; i += 32) {
+      const uintptr_t piece = first + (uintptr_t)i * 16;
+      if (piece >= lo && piece + 16 <= hi)
+        cp_async<16>(to_shared + i * 16, reinterpret_cast<const void*>(piece));
+      else
+        for (uintptr_t b = piece; b < piece + 16; b += sizeof(T))
+          if (b >= lo && b < hi)
+            *reinterpret_cast<T*>(to + (b - first)) = *reinterpret_cast<const T*>(b);
+    }
+  }
+}
+// The lane's k-th group of those elements.
+template <typename T, int W>
+__device__ __forceinline__ Raw<T, W> staged(const char* to, const T* p, size_t at, int k) {
+  const int c = (k * 32 + (int)(threadIdx.x & 31)) * W;
+  const int phase = W == 4 ? 0 : (int)(reinterpret_cast<uintptr_t>(p + at) & 15);
+  return *reinterpret_cast<const Raw<T, W>*>(to + phase + c * sizeof(T));
 }
 
 template <int E>
@@ -396,8 +459,8 @@ struct BwdArgs {
 template <typename X, typename H, typename Y, int E, int W, bool kBias, bool kFull>
 __device__ __forceinline__ void bwd_rows(const Args& a, const BwdArgs& p, const Y* dy,
                                          const X* dxo, X* dx, H* dh, ColumnSums<E>& sum,
-                                         float2* red, uint32_t run, uint32_t first, uint32_t last,
-                                         int c0, int member) {
+                                         float2* red, char* stage, uint32_t run, uint32_t first,
+                                         uint32_t last, int c0, int member) {
   constexpr int K = E / W, kStep = 32 * W;
   constexpr bool kKeep = E == 8 && !kBias;  // the gate and post weight in registers
   const int C = a.C;
@@ -418,25 +481,46 @@ __device__ __forceinline__ void bwd_rows(const Args& a, const BwdArgs& p, const 
       load_wp(k, k * W);
       load_gate(gate, k, k * W);
     }
-  int flip = 0;
-  for (uint32_t r = first; r < last; ++r) {
-    const size_t base = (size_t)r * C + c0;
-    const X* xr = static_cast<const X*>(a.x) + base;
-    const H* hr = static_cast<const H*>(a.h) + base;
-    const Y* yr = dy + base;
-    const X* ur = dxo + base;
-    Raw<X, W> xw[K], uw[K];
+  const X* xp = static_cast<const X*>(a.x);
+  const H* hp = static_cast<const H*>(a.h);
+  const size_t all = (size_t)a.N * C;
+  const int w0 = member * 32 * E, here = kFull ? 32 * E : C - w0;  // the warp's columns
+  constexpr int kX = stage_bytes<X, E>(), kH = stage_bytes<H, E>(), kY = stage_bytes<Y, E>();
+  constexpr int kSlot = bwd_slot<X, H, Y, E>();
+  const uint32_t stage_shared = (uint32_t)__cvta_generic_to_shared(stage);
+  auto start = [&](uint32_t r, int slot) {
+    if (r < last) {
+      char* to = stage + slot * kSlot;
+      const uint32_t ts = stage_shared + slot * kSlot;
+      const size_t at = (size_t)r * C + w0;
+      stage_in<H, E, W, kFull>(to, ts, hp, at, here, all);
+      stage_in<X, E, W, kFull>(to + kH, ts + kH, xp, at, here, all);
+      stage_in<Y, E, W, kFull>(to + kH + kX, ts + kH + kX, dy, at, here, all);
+      if (dxo)
+        stage_in<X, E, W, kFull>(to + kH + kX + kY, ts + kH + kX + kY, dxo, at, here, all);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  start(first, 0);
+  float4 st = p.stats[first];
+  int flip = 0, slot = 0;
+  for (uint32_t r = first; r < last; ++r, slot ^= 1) {
+    const size_t base = (size_t)r * C + c0, at = (size_t)r * C + w0;
+    const char* in = stage + slot * kSlot;
+    if (W == 1) __syncwarp();  // the other slot has been read
+    start(r + 1, slot ^ 1);
+    const float4 next = r + 1 < last ? p.stats[r + 1] : st;
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    if (W == 1) __syncwarp();
+    Raw<X, W> xw[K];
     Raw<H, W> hw[K];
     Raw<Y, W> yw[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int i = on(k) ? k * kStep : -c0;  // a column that is not there: the row's first
-      hw[k] = fetch<H, W>(hr + i);
-      xw[k] = fetch<X, W>(xr + i);
-      yw[k] = fetch<Y, W>(yr + i);
-      if (dxo) uw[k] = fetch<X, W>(ur + i);
+      hw[k] = staged<H, W>(in, hp, at, k);
+      xw[k] = staged<X, W>(in + kH, xp, at, k);
+      yw[k] = staged<Y, W>(in + kH + kX, dy, at, k);
     }
-    const float4 st = p.stats[r];
     if (r == turn) {
       ++grp, turn += a.T;
       if (a.gate) {
@@ -452,7 +536,11 @@ __device__ __forceinline__ void bwd_rows(const Args& a, const BwdArgs& p, const 
     for (int k = 0; k < K; ++k) {
       const int i = kKeep ? k * W : 0;
       if (!kKeep) load_wp(k, 0), load_gate(gate, k, 0);
-      param<W>(on(k) ? a.w : nullptr, c0 + k * kStep, 0.f, w);
+      if (on(k))
+        unpack(fetch<float, W>(a.w + c0 + k * kStep), w);
+      else
+#pragma unroll
+        for (int j = 0; j < W; ++j) w[j] = 0.f;
       param<W>(kBias && on(k) ? a.bp : nullptr, c0 + k * kStep, 0.f, bp);
       unpack(hw[k], hh + k * W);
       unpack(xw[k], xh + k * W);
@@ -483,7 +571,7 @@ __device__ __forceinline__ void bwd_rows(const Args& a, const BwdArgs& p, const 
       const int i = kKeep ? k * W : 0;
       float d[W];
       if (dxo)
-        unpack(uw[k], d);
+        unpack(staged<X, W>(in + kH + kX + kY, dxo, at, k), d);
       else
 #pragma unroll
         for (int j = 0; j < W; ++j) d[j] = 0.f;
@@ -531,30 +619,36 @@ __device__ __forceinline__ void bwd_rows(const Args& a, const BwdArgs& p, const 
           sum.g[k * W + j] = 0.f;
         }
     }
+    st = next;
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 template <typename X, typename H, typename Y, int E, int W, bool kBias>
 __global__ void __launch_bounds__(kMaxThreads, E == 8 ? 2 : 1)
     bwd_kernel(const Args a, const BwdArgs p, const Y* dy, const X* dxo, X* dx, H* dh) {
   constexpr int K = E / W, kStep = 32 * W;
-  __shared__ float2 red[2 * 8];
+  extern __shared__ __align__(16) char stages[];
+  __shared__ __align__(16) float2 red[2 * 8];
   __shared__ float sums[kMaxThreads * E];
   const int C = a.C, warp = threadIdx.x >> 5, groups = p.G == 1 ? (int)blockDim.x >> 5 : 1;
   const int group = p.G == 1 ? warp : 0, member = p.G == 1 ? 0 : warp;
   const int c0 = member * 32 * E + (threadIdx.x & 31) * W;
   const uint32_t run = blockIdx.x * groups + group;
   const uint32_t first = min(run * p.rows, a.N), last = min(first + p.rows, a.N);
+  if (threadIdx.x < 16) red[threadIdx.x] = make_float2(0.f, 0.f);
+  __syncthreads();
   ColumnSums<E> sum;
 #pragma unroll
   for (int e = 0; e < E; ++e) sum.w[e] = sum.b[e] = sum.wp[e] = sum.bp[e] = sum.g[e] = 0.f;
+  char* stage = stages + warp * (2 * bwd_slot<X, H, Y, E>());
   if (first < last) {
     if ((member + 1) * 32 * E <= C)
-      bwd_rows<X, H, Y, E, W, kBias, true>(a, p, dy, dxo, dx, dh, sum, red, run, first, last, c0,
-                                           member);
+      bwd_rows<X, H, Y, E, W, kBias, true>(a, p, dy, dxo, dx, dh, sum, red, stage, run, first,
+                                           last, c0, member);
     else
-      bwd_rows<X, H, Y, E, W, kBias, false>(a, p, dy, dxo, dx, dh, sum, red, run, first, last, c0,
-                                            member);
+      bwd_rows<X, H, Y, E, W, kBias, false>(a, p, dy, dxo, dx, dh, sum, red, stage, run, first,
+                                            last, c0, member);
   }
   // the groups' sums, added in order
   auto total = [&](const float* v, float f, int part) {
@@ -803,12 +897,18 @@ extern "C" int sqb_residual_norm_bwd(const void* dy, int y_dtype, const void* dx
   float* gate_parts = gate && gates > 1 ? parts + (size_t)kParts * p.ctas * p.pitch : nullptr;
   const BwdArgs more_args{reinterpret_cast<const float4*>(stats), parts, gate_parts, p.pitch, p.G,
                           p.rows};
+  bool ok = true;
   by_type(x_dtype, h_dtype, y_dtype, [&](auto tx, auto th, auto ty) {
     using X = decltype(tx);
     using H = decltype(th);
     using Y = decltype(ty);
     auto run = [&](auto kernel) {
-      kernel<<<p.ctas, 32 * p.G * p.groups, 0, q>>>(
+      const int warps = p.G * p.groups;
+      const int smem = warps * 2 * (p.E == 8 ? bwd_slot<X, H, Y, 8>() : bwd_slot<X, H, Y, 16>());
+      ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ==
+           cudaSuccess;
+      if (!ok) return;
+      kernel<<<p.ctas, 32 * warps, smem, q>>>(
           a, more_args, static_cast<const Y*>(dy), static_cast<const X*>(dx_out),
           static_cast<X*>(dx), static_cast<H*>(dh));
     };
@@ -821,6 +921,7 @@ extern "C" int sqb_residual_norm_bwd(const void* dy, int y_dtype, const void* dx
     };
     biased ? sized(std::true_type()) : sized(std::false_type());
   });
+  if (!ok) return SQB_ERR_CUDA;
   Sums s;
   s.parts = parts;
   s.out[0] = dweight, s.out[1] = bias ? dbias : nullptr;
