@@ -350,12 +350,14 @@ __global__ void __launch_bounds__(kMaxThreads)
 //
 // The columns' sums (d weight and so on) stay in registers over a run of rows; each CTA
 // writes one partial row of each (parts: (kParts, grid, pitch)), which a second kernel adds
-// in a fixed order (bit-reproducible).  A gate for each sample has its sums written where the gate
-// changes: one row for each (run, gate) that meet, at slot run + gate (each step along the
-// rows raises one of the two, so no slot is shared).
+// in a fixed order (bit-reproducible).  A gate for each sample has its sums written where the
+// gate changes: one row for each (run, gate) that meet, at slot run + gate (each step along
+// the rows raises one of the two, so no slot is shared).
 // What binds it first is the issue of instructions, with 16 warps an SM to cover their
-// latencies: 25 for each element are the mathematics.  No more is kept in registers than 16
-// warps of 128 have room for.
+// latencies: some 25 for each element are the mathematics.  No more is kept in registers than
+// 16 warps of 128 have room for.  16384 rows of 768 (fp32 stream, bf16 h and dy): 49 us, 4.6
+// TB/s of the 226 MB; 9006 of 1999, bf16: 85 us.  Measured on the way: loads straight into
+// registers 55 us, 24 columns a lane 62 us, rows shared by whole CTAs 85 to 108 us.
 
 // Sums of a pair over the G warps of a row, the same in all of them.  red: the group's,
 // member: this warp's place in it.
