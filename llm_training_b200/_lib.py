@@ -9,12 +9,14 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 
 import torch
 
-from .build import LIBPATH
+from .build import BINDING, BINDINGPATH, LIBPATH
 
 SQB_F32 = 0
 SQB_BF16 = 1
@@ -114,6 +116,29 @@ TRAIN_SIGNATURES = {
                               [_c_i64, ctypes.c_float, ctypes.c_float, ctypes.c_int] +
                               [_vp] * 9 + [ctypes.c_size_t, _c_i64, _c_i64, _vp]),
 }
+
+
+_binding = None
+
+
+def binding():
+    """The C++ PyTorch binding of the post-training operators, on the library of ``lib()``;
+    raises if it is absent."""
+    global _binding
+    if _binding is None:
+        lib()
+        with _lock:
+            if _binding is None:
+                if not os.path.exists(BINDINGPATH):
+                    raise RuntimeError(f"PyTorch binding not found at {BINDINGPATH}; build it "
+                                       "with `python -m llm_training_b200.build`")
+                loader = importlib.machinery.ExtensionFileLoader(BINDING, BINDINGPATH)
+                module = importlib.util.module_from_spec(
+                    importlib.util.spec_from_loader(BINDING, loader))
+                loader.exec_module(module)
+                module.attach(library_path())
+                _binding = module
+    return _binding
 
 
 def on_device(device):

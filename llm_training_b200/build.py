@@ -4,17 +4,21 @@
 
 Produces ``llm_training_b200/lib/libsqrtblock.so`` from ``csrc/*.cu``.  The
 library exports the C ABI of ``include/sqrtblock.h`` and links the CUDA
-runtime statically, so it depends only on the driver at run time.
+runtime statically, so it depends only on the driver at run time.  And
+``lib/sqb_torch.so`` from ``csrc/torch_binding.cpp`` (g++, PyTorch's headers): the
+eager PyTorch binding of the post-training operators.
 """
 
 from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG)
@@ -24,6 +28,8 @@ BUILD = os.path.join(PKG, "_build")
 LIBDIR = os.path.join(PKG, "lib")
 LIBNAME = "libsqrtblock.so"
 LIBPATH = os.path.join(LIBDIR, LIBNAME)
+BINDING = "sqb_torch"
+BINDINGPATH = os.path.join(LIBDIR, BINDING + ".so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -53,6 +59,24 @@ def _headers():
     return hs
 
 
+def _binding_command(out: str):
+    """g++ command of the PyTorch binding."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise RuntimeError("PyTorch not found: its binding cannot be built")
+    torch_dir = spec.submodule_search_locations[0]
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc_path()))), "include")
+    headers = [os.path.join(torch_dir, "include"),
+               os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"), cuda,
+               sysconfig.get_paths()["include"]]
+    return ([os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared",
+             "-fvisibility=hidden", f"-DTORCH_EXTENSION_NAME={BINDING}", "-I", INCLUDE]
+            + [f for h in headers for f in ("-isystem", h)]
+            + [os.path.join(CSRC, "torch_binding.cpp"), "-o", out,
+               "-L", os.path.join(torch_dir, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+               "-ltorch", "-ltorch_python"])
+
+
 def _stale(target: str, deps) -> bool:
     if not os.path.exists(target):
         return True
@@ -61,7 +85,8 @@ def _stale(target: str, deps) -> bool:
 
 
 def build(force: bool = False, debug: bool = False, verbose: bool = False) -> str:
-    """Compile every .cu for sm_100a and link the shared library; returns its path."""
+    """Compile every .cu for sm_100a, link the shared library and build the PyTorch binding;
+    returns the library's path."""
     nvcc = nvcc_path()
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
@@ -76,19 +101,27 @@ def build(force: bool = False, debug: bool = False, verbose: bool = False) -> st
         if force or _stale(obj, [s] + hdrs + [__file__]):
             jobs.append([nvcc, *flags, "-c", s, "-o", obj])
 
+    binding_src = os.path.join(CSRC, "torch_binding.cpp")
+    binding_tmp = BINDINGPATH + ".tmp"
+    new_binding = force or _stale(BINDINGPATH, [binding_src] + hdrs + [__file__])
+    if new_binding:
+        jobs.insert(0, _binding_command(binding_tmp))
+
     def run(cmd):
         if verbose:
             print(" ".join(cmd), flush=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise RuntimeError(f"nvcc failed ({' '.join(cmd)}):\n{r.stdout}\n{r.stderr}")
+            raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({' '.join(cmd)}):\n{r.stdout}\n{r.stderr}")
         return r.stdout + r.stderr
 
     with cf.ThreadPoolExecutor(max_workers=max(1, min(len(jobs), os.cpu_count() or 1))) as ex:
         for out in ex.map(run, jobs):
             if verbose and out.strip():
                 print(out, flush=True)
-    if force or jobs or _stale(LIBPATH, objs):
+    if new_binding:
+        os.replace(binding_tmp, BINDINGPATH)
+    if force or _stale(LIBPATH, objs):
         tmp = LIBPATH + ".tmp"
         run([nvcc, *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-o", tmp, *objs])
         os.replace(tmp, LIBPATH)

@@ -20,22 +20,16 @@ from typing import Optional
 
 import torch
 
-from torch.autograd.function import once_differentiable
-
 from . import _lib
 
 __all__ = ["token_log_probs", "preference_loss", "policy_loss", "policy_loss_and_grad"]
 
-_DTYPES = {torch.float32: _lib.SQB_F32, torch.bfloat16: _lib.SQB_BF16}
+_DTYPES = (torch.float32, torch.bfloat16)
 _INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 
-def _ptr(t):
-    return t.data_ptr() if t is not None else None
-
-
 def _grad_strides(x):
-    """Strides for the gradient: x's, or where x's rows lie far apart (a few tokens of a longer
+    """Strides of the gradient, as the binding makes it: x's, or where x's rows lie far apart (a few tokens of a longer
     batch) ones without the gaps, that keep every row's place between 16-byte boundaries."""
     strides = x.stride()
     if x.numel() == 0 or 1 + sum((n - 1) * s for n, s in zip(x.shape, strides)) <= 2 * x.numel():
@@ -49,26 +43,14 @@ def _grad_strides(x):
     return tuple(reversed(got))
 
 
-def _grad_like(x):
-    """An uninitialised gradient of x: its shape and the 16-byte phase of each of its rows (it
-    is written with the vector stores the logits are read with)."""
-    strides = _grad_strides(x)
-    phase = x.data_ptr() % 16 // x.element_size()
-    if phase == 0 or x.numel() == 0:
-        return torch.empty_strided(x.shape, strides, dtype=x.dtype, device=x.device)
-    span = 1 + sum((n - 1) * s for n, s in zip(x.shape, strides))
-    buf = torch.empty(span + phase, dtype=x.dtype, device=x.device)
-    return buf.as_strided(x.shape, strides, phase)
-
-
 def _fake_grad(x):
     return torch.empty_strided(x.shape, _grad_strides(x), dtype=x.dtype, device=x.device)
 
 
 # ---- the operators --------------------------------------------------------------------
-# x is (S, T, V), or (N, V) as one sequence; t int64, contiguous, one target a row.  Each
-# has a function that launches it, registered as a custom op for traced calls and wrapped in
-# an autograd function, with the same backward, for eager ones.
+# x is (S, T, V), or (N, V) as one sequence; t int64, contiguous, one target a row.  An eager
+# call goes to the C++ binding, which has the autograd nodes; these are the same launches
+# registered as custom ops, for traced calls.
 
 
 def _dims(x):
@@ -78,38 +60,10 @@ def _dims(x):
     return (*x.shape, x.stride(0), x.stride(1))
 
 
-def _scratch(N):
-    """Where the scratch begins in a buffer that starts with 3 N floats, in bytes."""
-    return -(-12 * N // 256) * 256
-
-
-def _rows_and(nbytes, N):
-    """Floats of a buffer of 3 N floats and then `nbytes` of scratch."""
-    return (_scratch(N) + nbytes + 3) // 4
-
-
-def _run(raw, op, function, x, *args):
-    if not _lib.plain(x):
-        return op(x, *args)
-    if x.requires_grad and torch.is_grad_enabled():
-        return function.apply(x, *args)
-    return raw(x, *args)
-
-
-def _logp_fwd_raw(x: torch.Tensor, t: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+@torch.library.custom_op("sqrtblock::logp_fwd", mutates_args=())
+def _logp_fwd(x: torch.Tensor, t: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(logp in t's shape, row statistics (2 S T,))."""
-    S, T, V, ss, st = _dims(x)
-    logp = torch.empty(t.shape, dtype=torch.float32, device=x.device)
-    stats = torch.empty(2 * S * T, dtype=torch.float32, device=x.device)
-    if S * T:
-        with _lib.on_device(x.device):
-            _lib.check("sqb_logp_fwd", _lib.lib().sqb_logp_fwd(
-                x.data_ptr(), t.data_ptr(), logp.data_ptr(), stats.data_ptr(), S, T, V, ss, st,
-                _DTYPES[x.dtype], _lib.stream(x.device)))
-    return logp, stats
-
-
-_logp_fwd = torch.library.custom_op("sqrtblock::logp_fwd", _logp_fwd_raw, mutates_args=())
+    return _lib.binding().logp_fwd(x, t)
 
 
 @_logp_fwd.register_fake
@@ -118,31 +72,17 @@ def _(x, t):
             x.new_empty(2 * t.numel(), dtype=torch.float32))
 
 
-def _logp_bwd_raw(x: torch.Tensor, t: torch.Tensor, stats: torch.Tensor,
-                  g_row: Optional[torch.Tensor], scale: Optional[torch.Tensor]) -> torch.Tensor:
+@torch.library.custom_op("sqrtblock::logp_bwd", mutates_args=())
+def _logp_bwd(x: torch.Tensor, t: torch.Tensor, stats: torch.Tensor,
+              g_row: Optional[torch.Tensor], scale: Optional[torch.Tensor]) -> torch.Tensor:
     """g_row[r] * scale * ([c == t] - softmax) in x's dtype; without a g_row the factors follow
     the row statistics."""
-    S, T, V, ss, st = _dims(x)
-    dx = _grad_like(x)
-    if S * T:
-        g = g_row.data_ptr() if g_row is not None else stats.data_ptr() + 8 * S * T
-        with _lib.on_device(x.device):
-            _lib.check("sqb_logp_bwd", _lib.lib().sqb_logp_bwd(
-                x.data_ptr(), t.data_ptr(), stats.data_ptr(), g, _ptr(scale), dx.data_ptr(), S,
-                T, V, ss, st, *_dims(dx)[3:], _DTYPES[x.dtype], _lib.stream(x.device)))
-    return dx
-
-
-_logp_bwd = torch.library.custom_op("sqrtblock::logp_bwd", _logp_bwd_raw, mutates_args=())
+    return _lib.binding().logp_bwd(x, t, stats, g_row, scale)
 
 
 @_logp_bwd.register_fake
 def _(x, t, stats, g_row, scale):
     return _fake_grad(x)
-
-
-def _rows_grad(x, *args):
-    return (_logp_bwd_raw if _lib.plain(x) else _logp_bwd)(x, *args)
 
 
 def _logp_setup(ctx, inputs, output):
@@ -151,120 +91,56 @@ def _logp_setup(ctx, inputs, output):
 
 
 def _logp_grad(ctx, dlogp, _dstats):
-    x, t, stats = ctx.saved_tensors
-    return _rows_grad(x, t, stats, dlogp.to(torch.float32).contiguous(), None), None
+    return _logp_bwd(*ctx.saved_tensors, dlogp.to(torch.float32).contiguous(), None), None
 
 
 _logp_fwd.register_autograd(_logp_grad, setup_context=_logp_setup)
 
 
-class _LogP(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, *args):
-        out = _logp_fwd_raw(*args)
-        _logp_setup(ctx, args, out)
-        return out
-
-    backward = staticmethod(once_differentiable(_logp_grad))
-
-
-def _preference_raw(x: torch.Tensor, t: torch.Tensor, ref: Optional[torch.Tensor],
+@torch.library.custom_op("sqrtblock::preference_fwd", mutates_args=())
+def _preference_fwd(x: torch.Tensor, t: torch.Tensor, ref: Optional[torch.Tensor],
                     cu: Optional[torch.Tensor], pairs: int, beta: float, label_smoothing: float
                     ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(loss, rewards (2, P), row statistics and d loss / d logp of each row (3 S T floats, and
     scratch))."""
-    S, T, V, ss, st = _dims(x)
-    dev, N, f32 = x.device, S * T, torch.float32
-    loss = torch.empty((), dtype=f32, device=dev)
-    rewards = torch.empty((2, pairs), dtype=f32, device=dev)
-    lib = _lib.lib()
-    nbytes = lib.sqb_preference_workspace_bytes(N, pairs)
-    rows = torch.empty(_rows_and(nbytes, N), dtype=f32, device=dev)
-    at = rows.data_ptr()
-    with _lib.on_device(dev):
-        _lib.check("sqb_preference_fwd", lib.sqb_preference_fwd(
-            x.data_ptr(), t.data_ptr(), _ptr(cu), _ptr(ref), pairs, beta, label_smoothing,
-            loss.data_ptr(), rewards.data_ptr(), at, at + 8 * N, S, T, V, ss, st,
-            _DTYPES[x.dtype], at + _scratch(N), nbytes, _lib.stream(x.device)))
-    return loss, rewards, rows
-
-
-_preference_fwd = torch.library.custom_op("sqrtblock::preference_fwd", _preference_raw,
-                                          mutates_args=())
+    return _lib.binding().preference_fwd(x, t, ref, cu, pairs, beta, label_smoothing)
 
 
 @_preference_fwd.register_fake
 def _(x, t, ref, cu, pairs, beta, label_smoothing):
-    f32 = torch.float32
-    N = t.numel()
-    nbytes = -(-8 * N // 256) * 256 + 8 * pairs  # sqb_preference_workspace_bytes
+    f32, N = torch.float32, t.numel()
+    up = lambda n: -(-n // 256) * 256  # noqa: E731
+    scratch = up(8 * N) + 8 * pairs  # sqb_preference_workspace_bytes
     return (x.new_empty((), dtype=f32), x.new_empty((2, pairs), dtype=f32),
-            x.new_empty(_rows_and(nbytes, N), dtype=f32))
+            x.new_empty((up(12 * N) + scratch + 3) // 4, dtype=f32))
 
 
-def _loss_grad(ctx, dloss):
+def _loss_setup(ctx, inputs, output):
+    _, *others, last = output
+    ctx.save_for_backward(*inputs[:2], last)
+    ctx.mark_non_differentiable(*others, last)
+    ctx.arguments = len(inputs)
+
+
+def _loss_grad(ctx, dloss, *_):
     x, t, rows = ctx.saved_tensors
-    return _rows_grad(x, t, rows, None, dloss.to(torch.float32))
+    return (_logp_bwd(x, t, rows, None, dloss.to(torch.float32)),) + (None,) * (
+        ctx.arguments - 1)
 
 
-def _preference_setup(ctx, inputs, output):
-    _, rewards, rows = output
-    ctx.save_for_backward(*inputs[:2], rows)
-    ctx.mark_non_differentiable(rewards, rows)
-    ctx.set_materialize_grads(False)
+_preference_fwd.register_autograd(_loss_grad, setup_context=_loss_setup)
 
 
-def _preference_grad(ctx, dloss, *_):
-    if dloss is None:
-        return (None,) * 7
-    return (_loss_grad(ctx, dloss),) + (None,) * 6
-
-
-_preference_fwd.register_autograd(_preference_grad, setup_context=_preference_setup)
-
-
-class _Preference(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, *args):
-        out = _preference_raw(*args)
-        _preference_setup(ctx, args, out)
-        return out
-
-    backward = staticmethod(once_differentiable(_preference_grad))
-
-
-def _policy_raw(x: torch.Tensor, t: torch.Tensor, adv: torch.Tensor,
+@torch.library.custom_op("sqrtblock::policy_fwd", mutates_args=())
+def _policy_fwd(x: torch.Tensor, t: torch.Tensor, adv: torch.Tensor,
                 old: Optional[torch.Tensor], ref: Optional[torch.Tensor],
                 cu: Optional[torch.Tensor], seqs: int, adv_by_seq: bool, per_seq: bool,
                 clip_low: float, clip_high: float, kl_coef: float, grad_scale: Optional[float]
                 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(loss, logps, (policy term, KL, clipped share), last): `last` is the logits' gradient
     times grad_scale, or for None the row statistics and d loss / d logp (3 S T,)."""
-    S, T, V, ss, st = _dims(x)
-    dev, N, f32 = x.device, S * T, torch.float32
-    logps = torch.empty(t.shape, dtype=f32, device=dev)
-    loss = torch.empty((), dtype=f32, device=dev)
-    statistics = torch.empty(3, dtype=f32, device=dev)
-    fused = grad_scale is not None
-    last = _grad_like(x) if fused else torch.empty(3 * N, dtype=f32, device=dev)
-    if N == 0:
-        return loss.zero_(), logps, statistics.zero_(), last
-    lib = _lib.lib()
-    nbytes = lib.sqb_policy_workspace_bytes(N, seqs)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    at = last.data_ptr()
-    with _lib.on_device(dev):
-        _lib.check("sqb_policy_fwd", lib.sqb_policy_fwd(
-            x.data_ptr(), t.data_ptr(), _ptr(cu), seqs, _ptr(old), _ptr(ref), adv.data_ptr(),
-            adv_by_seq, clip_low, clip_high, kl_coef, per_seq, loss.data_ptr(),
-            statistics.data_ptr(), logps.data_ptr(), None if fused else at,
-            None if fused else at + 8 * N, at if fused else None, grad_scale if fused else 1.0,
-            S, T, V, ss, st, *(_dims(last)[3:] if fused else (ss, st)), _DTYPES[x.dtype],
-            ws.data_ptr(), nbytes, _lib.stream(x.device)))
-    return loss, logps, statistics, last
-
-
-_policy_fwd = torch.library.custom_op("sqrtblock::policy_fwd", _policy_raw, mutates_args=())
+    return _lib.binding().policy_fwd(x, t, adv, old, ref, cu, seqs, adv_by_seq, per_seq,
+                                     clip_low, clip_high, kl_coef, grad_scale)
 
 
 @_policy_fwd.register_fake
@@ -276,30 +152,7 @@ def _(x, t, adv, old, ref, cu, seqs, adv_by_seq, per_seq, clip_low, clip_high, k
             x.new_empty(3, dtype=f32), last)
 
 
-def _policy_setup(ctx, inputs, output):
-    _, logps, statistics, last = output
-    ctx.save_for_backward(*inputs[:2], last)
-    ctx.mark_non_differentiable(logps, statistics, last)
-    ctx.set_materialize_grads(False)
-
-
-def _policy_grad(ctx, dloss, *_):
-    if dloss is None:
-        return (None,) * 13
-    return (_loss_grad(ctx, dloss),) + (None,) * 12
-
-
-_policy_fwd.register_autograd(_policy_grad, setup_context=_policy_setup)
-
-
-class _Policy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, *args):
-        out = _policy_raw(*args)
-        _policy_setup(ctx, args, out)
-        return out
-
-    backward = staticmethod(once_differentiable(_policy_grad))
+_policy_fwd.register_autograd(_loss_grad, setup_context=_loss_setup)
 
 
 # ---- public entry points --------------------------------------------------------------
@@ -384,7 +237,7 @@ def token_log_probs(logits, targets):
     (``sqrtblock::logp_fwd/bwd``): one read of the logits forward, and one read and one
     write backward, with no softmax kept in between."""
     x, t = _rows("token_log_probs", logits, targets)
-    return _run(_logp_fwd_raw, _logp_fwd, _LogP, x, t)[0]
+    return _lib.binding().logp(x, t) if _lib.plain(x) else _logp_fwd(x, t)[0]
 
 
 def preference_loss(logits, targets, ref_logps=None, *, beta=0.1, label_smoothing=0.0,
@@ -408,8 +261,10 @@ def preference_loss(logits, targets, ref_logps=None, *, beta=0.1, label_smoothin
     ref = _given(fn, "ref_logps", ref_logps, [(seqs,)], x.device)
     beta = _number(fn, "beta", beta, most=1e30)
     label_smoothing = _number(fn, "label_smoothing", label_smoothing, most=1.0)
-    loss, rewards, _ = _run(_preference_raw, _preference_fwd, _Preference, x, t, ref, cu,
-                            seqs // 2, beta, label_smoothing)
+    args = (x, t, ref, cu, seqs // 2, beta, label_smoothing)
+    if _lib.plain(x):
+        return _lib.binding().preference(*args)
+    loss, rewards, _ = _preference_fwd(*args)
     return (loss, *rewards.unbind(0))
 
 
@@ -460,8 +315,9 @@ def policy_loss(logits, targets, advantages, old_logps=None, ref_logps=None, *, 
     loss - are for logging and for the next step's ``old_logps``, not differentiable."""
     args = _policy_args("policy_loss", logits, targets, advantages, old_logps, ref_logps, clip,
                         clip_high, kl_coef, reduction, cu_seqlens)
-    loss, logps, stats, _ = _run(_policy_raw, _policy_fwd, _Policy, *args, None)
-    return loss, logps, stats
+    if _lib.plain(args[0]):
+        return _lib.binding().policy(*args)
+    return _policy_fwd(*args, None)[:3]
 
 
 def policy_loss_and_grad(logits, targets, advantages, old_logps=None, ref_logps=None, *,
@@ -480,5 +336,6 @@ def policy_loss_and_grad(logits, targets, advantages, old_logps=None, ref_logps=
     grad_scale = float(grad_scale)
     if not math.isfinite(grad_scale):
         raise ValueError(f"{fn}: grad_scale must be finite, got {grad_scale}")
-    loss, logps, stats, dx = _run(_policy_raw, _policy_fwd, _Policy, *args, grad_scale)
-    return loss, dx, logps, stats
+    run = _lib.binding().policy_fwd if _lib.plain(args[0]) else _policy_fwd
+    loss, logps, stats, grad = run(*args, grad_scale)
+    return loss, grad, logps, stats
