@@ -108,11 +108,15 @@ __device__ __forceinline__ void param(const float* p, int c, float none, float* 
 
 // ---- rows ---------------------------------------------------------------------------
 //
-// G warps (1 to 8) hold a row, E columns a lane, each warp 32 E consecutive ones, and walk a
+// G warps (1 to 16) hold a row, E columns a lane, each warp 32 E consecutive ones, and walk a
 // run of consecutive rows.  A CTA is one such group, or eight groups of one warp.  A warp
-// whose columns all exist takes a path without a comparison for each.
+// whose columns all exist takes a path without a comparison for each.  More warps before more
+// columns a lane: 2728 rows of 4001 (bf16, y fp32) take 52 + 62 us, forward + backward, and
+// took 69 + 96 with eight warps of 16 columns; and fewer columns where one warp has room: 51155
+// rows of 102 take 37 + 50 us with 4 a lane, 59 + 93 with 8.
 
-constexpr int kMaxThreads = 256;
+constexpr int kMaxWarps = 16;               // of a row
+constexpr int kBwdWarps = 16, kFwdWarps = 24;  // on an SM, as registers allow
 
 // The CTA's barrier: its warps arrive from two places in the code.
 __device__ __forceinline__ void group_barrier() { asm volatile("bar.sync 0;" ::: "memory"); }
@@ -170,7 +174,7 @@ __device__ __forceinline__ void fwd_rows(const Args& a, X* xo, Y* y, float4* sta
                                          uint32_t first, uint32_t last, int c0, int member,
                                          int G) {
   constexpr int K = E / W, kStep = 32 * W;
-  constexpr bool kKeep = E == 8 && !kBias;  // parameters in registers
+  constexpr bool kKeep = !kBias;  // parameters in registers
   const int C = a.C;
   auto on = [&](int k) { return kFull || c0 + k * kStep < C; };
   float w[kKeep ? E : W], wp[kKeep ? E : W], gw[kKeep ? E : W], b[W], bp[W];
@@ -233,8 +237,8 @@ __device__ __forceinline__ void fwd_rows(const Args& a, X* xo, Y* y, float4* sta
       }
       if (on(k)) store<W>(xo + base + k * kStep, x + k * W);
     }
-    moments<E, W>(x, a, on, G, member, red + 8, mx, rx);
-    if (G > 1 && !a.wp) group_barrier();  // red + 8 is written again before another barrier
+    moments<E, W>(x, a, on, G, member, red + kMaxWarps, mx, rx);
+    if (G > 1 && !a.wp) group_barrier();  // these are written again before another barrier
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int i = kKeep ? k * W : 0;
@@ -250,9 +254,9 @@ __device__ __forceinline__ void fwd_rows(const Args& a, X* xo, Y* y, float4* sta
 }
 
 template <typename X, typename H, typename Y, int E, int W, bool kBias>
-__global__ void __launch_bounds__(kMaxThreads, E == 8 ? 3 : 2)
+__global__ void __launch_bounds__(kFwdWarps * 32)  // for its registers: CTAs are smaller
     fwd_kernel(const Args a, X* xo, Y* y, float4* stats, int G, uint32_t rows) {
-  __shared__ float2 red[2 * 8];
+  __shared__ float2 red[2 * kMaxWarps];
   const int warp = threadIdx.x >> 5, groups = G == 1 ? (int)blockDim.x >> 5 : 1;
   const int group = G == 1 ? warp : 0, member = G == 1 ? 0 : warp;
   const int c0 = member * 32 * E + (threadIdx.x & 31) * W;
@@ -270,11 +274,12 @@ __global__ void __launch_bounds__(kMaxThreads, E == 8 ? 3 : 2)
 // warps a row; wider rows would leave too few registers, single elements too many
 // instructions: 9006 x 1999 53 us with eight warps a row, 89 us with four and more columns
 // a lane).
+constexpr int kWarpRows = 8;  // rows of a CTA
 template <typename X, typename H, typename Y, int K>
-__global__ void __launch_bounds__(kMaxThreads)
+__global__ void __launch_bounds__(kWarpRows * 32)
     fwd_warp_kernel(const Args a, X* xo, Y* y, float4* stats) {
   const int lane = threadIdx.x & 31, C = a.C;
-  const uint32_t r = blockIdx.x * (kMaxThreads / 32) + (threadIdx.x >> 5);
+  const uint32_t r = blockIdx.x * kWarpRows + (threadIdx.x >> 5);
   if (r >= a.N) return;
   const size_t base = (size_t)r * C;
   const X* xr = static_cast<const X*>(a.x) + base;
@@ -385,6 +390,13 @@ __device__ __forceinline__ void pair_sums(float& u, float& v, float2* red, int G
     u += (r.x + r.z) + (t.x + t.z);
     v += (r.y + r.w) + (t.y + t.w);
   }
+  if (G > 8)
+#pragma unroll
+    for (int i = 4; i < kMaxWarps / 2; i += 2) {
+      const float4 r = all[i], t = all[i + 1];
+      u += (r.x + r.z) + (t.x + t.z);
+      v += (r.y + r.w) + (t.y + t.w);
+    }
 }
 
 // A warp's 32 E columns of a row on their way through shared memory, a row ahead of its use:
@@ -464,7 +476,7 @@ __device__ __forceinline__ void bwd_rows(const Args& a, const BwdArgs& p, const 
                                          float2* red, char* stage, uint32_t run, uint32_t first,
                                          uint32_t last, int c0, int member) {
   constexpr int K = E / W, kStep = 32 * W;
-  constexpr bool kKeep = E == 8 && !kBias;  // the gate and post weight in registers
+  constexpr bool kKeep = !kBias;  // the gate and post weight in registers
   const int C = a.C;
   auto on = [&](int k) { return kFull || c0 + k * kStep < C; };
   const float inv = 1.f / C, mean_inv = a.rms ? 0.f : inv;
@@ -562,7 +574,7 @@ __device__ __forceinline__ void bwd_rows(const Args& a, const BwdArgs& p, const 
       }
     }
     s0 += t0, s1 += t1;
-    pair_sums(s0, s1, red + flip * 8, p.G, member);
+    pair_sums(s0, s1, red + flip * kMaxWarps, p.G, member);
     flip ^= 1;
     const float k0 = -st.w * (s0 * mean_inv), k1 = -s1 * inv;
     float q0 = 0.f, q1 = 0.f;
@@ -598,7 +610,7 @@ __device__ __forceinline__ void bwd_rows(const Args& a, const BwdArgs& p, const 
     float l0 = 0.f, l1 = 0.f;
     if (a.wp) {
       q0 += t0, q1 += t1;
-      pair_sums(q0, q1, red + flip * 8, p.G, member);
+      pair_sums(q0, q1, red + flip * kMaxWarps, p.G, member);
       flip ^= 1;
       l0 = -st.y * (q0 * mean_inv), l1 = -q1 * inv;
     }
@@ -627,18 +639,18 @@ __device__ __forceinline__ void bwd_rows(const Args& a, const BwdArgs& p, const 
 }
 
 template <typename X, typename H, typename Y, int E, int W, bool kBias>
-__global__ void __launch_bounds__(kMaxThreads, E == 8 ? 2 : 1)
+__global__ void __launch_bounds__(kBwdWarps * 32)
     bwd_kernel(const Args a, const BwdArgs p, const Y* dy, const X* dxo, X* dx, H* dh) {
   constexpr int K = E / W, kStep = 32 * W;
   extern __shared__ __align__(16) char stages[];
-  __shared__ __align__(16) float2 red[2 * 8];
-  __shared__ float sums[kMaxThreads * E];
+  static_assert(2 * bwd_slot<X, H, Y, E>() >= 32 * E * (int)sizeof(float), "a warp's sums");
+  __shared__ __align__(16) float2 red[2 * kMaxWarps];
   const int C = a.C, warp = threadIdx.x >> 5, groups = p.G == 1 ? (int)blockDim.x >> 5 : 1;
   const int group = p.G == 1 ? warp : 0, member = p.G == 1 ? 0 : warp;
   const int c0 = member * 32 * E + (threadIdx.x & 31) * W;
   const uint32_t run = blockIdx.x * groups + group;
   const uint32_t first = min(run * p.rows, a.N), last = min(first + p.rows, a.N);
-  if (threadIdx.x < 16) red[threadIdx.x] = make_float2(0.f, 0.f);
+  if (threadIdx.x < 2 * kMaxWarps) red[threadIdx.x] = make_float2(0.f, 0.f);
   __syncthreads();
   ColumnSums<E> sum;
 #pragma unroll
@@ -652,7 +664,8 @@ __global__ void __launch_bounds__(kMaxThreads, E == 8 ? 2 : 1)
       bwd_rows<X, H, Y, E, W, kBias, false>(a, p, dy, dxo, dx, dh, sum, red, stage, run, first,
                                             last, c0, member);
   }
-  // the groups' sums, added in order
+  // the groups' sums, added in order: a row of each, where the staged rows were
+  float* sums = reinterpret_cast<float*>(stages);
   auto total = [&](const float* v, float f, int part) {
     __syncthreads();
 #pragma unroll
@@ -733,23 +746,22 @@ bool aligned(const void* p, int bytes) {
 
 bool known(int dtype) { return dtype == SQB_BF16 || dtype == SQB_F32; }
 
-// How N rows of C columns are dealt out: groups of G warps whose lanes hold E columns (16
-// beyond 2048 columns, so that 8 warps do), as many CTAs of one group (or of eight groups of
-// one warp) on each of 148 SMs as `warps` (for E = 8) allow, runs of as many rows each.
+// How N rows of C columns are dealt out: groups of G warps whose lanes hold E columns (8, or 4
+// where one warp then has the row), as many CTAs of one group (or of eight groups of one warp)
+// on each of 148 SMs as `warps` allow, runs of as many rows each.
 struct Plan {
   int G, E, groups, ctas, runs, pitch;
   uint32_t rows;
 };
 
-constexpr int kBwdWarps = 16, kFwdWarps = 24;
 constexpr int kMaxCtas = 148 * 8;
 
 Plan plan_of(int64_t N, int64_t C, int warps) {
   Plan p;
-  p.E = C <= 2048 ? 8 : 16;
+  p.E = C <= 128 ? 4 : 8;
   p.G = (int)((C + 32 * p.E - 1) / (32 * p.E));
   p.groups = p.G == 1 ? 8 : 1;
-  const int per_sm = (p.E == 8 ? warps : warps * 2 / 3 / 8 * 8) / (p.G * p.groups);
+  const int per_sm = warps / (p.G * p.groups);
   const int64_t all = (int64_t)148 * per_sm * p.groups;
   p.rows = (uint32_t)((N + all - 1) / all);
   p.runs = (int)((N + p.rows - 1) / p.rows);
@@ -846,13 +858,17 @@ extern "C" int sqb_residual_norm_fwd(const void* x, int x_dtype, const void* h, 
       if (p.E == 8)
         w4 ? run(fwd_kernel<X, H, Y, 8, 4, kb>) : run(fwd_kernel<X, H, Y, 8, 1, kb>);
       else
-        w4 ? run(fwd_kernel<X, H, Y, 16, 4, kb>) : run(fwd_kernel<X, H, Y, 16, 1, kb>);
+        w4 ? run(fwd_kernel<X, H, Y, 4, 4, kb>) : run(fwd_kernel<X, H, Y, 4, 1, kb>);
     };
     auto one_warp = [&](auto kernel) {
-      kernel<<<(unsigned)((N + 7) / 8), kMaxThreads, 0, q>>>(a, static_cast<X*>(x_out),
+      kernel<<<(unsigned)((N + kWarpRows - 1) / kWarpRows), kWarpRows * 32, 0, q>>>(a, static_cast<X*>(x_out),
                                                              static_cast<Y*>(y), st);
     };
-    if (w4 && C <= 512)
+    if (w4 && C <= 128)
+      one_warp(fwd_warp_kernel<X, H, Y, 1>);
+    else if (w4 && C <= 256)
+      one_warp(fwd_warp_kernel<X, H, Y, 2>);
+    else if (w4 && C <= 512)
       one_warp(fwd_warp_kernel<X, H, Y, 4>);
     else if (w4 && C <= 768)
       one_warp(fwd_warp_kernel<X, H, Y, 6>);
@@ -906,7 +922,7 @@ extern "C" int sqb_residual_norm_bwd(const void* dy, int y_dtype, const void* dx
     using Y = decltype(ty);
     auto run = [&](auto kernel) {
       const int warps = p.G * p.groups;
-      const int smem = warps * 2 * (p.E == 8 ? bwd_slot<X, H, Y, 8>() : bwd_slot<X, H, Y, 16>());
+      const int smem = warps * 2 * (p.E == 8 ? bwd_slot<X, H, Y, 8>() : bwd_slot<X, H, Y, 4>());
       ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ==
            cudaSuccess;
       if (!ok) return;
@@ -919,7 +935,7 @@ extern "C" int sqb_residual_norm_bwd(const void* dy, int y_dtype, const void* dx
       if (p.E == 8)
         w4 ? run(bwd_kernel<X, H, Y, 8, 4, kb>) : run(bwd_kernel<X, H, Y, 8, 1, kb>);
       else
-        w4 ? run(bwd_kernel<X, H, Y, 16, 4, kb>) : run(bwd_kernel<X, H, Y, 16, 1, kb>);
+        w4 ? run(bwd_kernel<X, H, Y, 4, 4, kb>) : run(bwd_kernel<X, H, Y, 4, 1, kb>);
     };
     biased ? sized(std::true_type()) : sized(std::false_type());
   });

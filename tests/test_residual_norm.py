@@ -229,6 +229,38 @@ def test_many_rows_and_gates(shape, gate):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(900, 31), (3, 400, 127), (2, 1500, 128), (700, 129), (700, 132),
+                                   (500, 256), (500, 257), (400, 2048), (5, 80, 2049),
+                                   (400, 2304), (400, 2305), (3, 120, 3333), (350, 4093),
+                                   (2, 170, 4096)])
+@pytest.mark.parametrize("bias,gate", [(True, "channel"), (False, "sample")])
+def test_widths_around_the_layouts_borders(shape, bias, gate):
+    """Widths at which another number of warps or columns a lane takes a row."""
+    check(shape, BF16, F32, BF16, "flat" if len(shape) == 2 and gate == "sample" else gate, bias,
+          True, "layer")
+
+
+@pytest.mark.gpu
+def test_more_elements_than_32_bits_count():
+    """The last rows of a stream of more than 2**31 elements are what they are on their own."""
+    N, C, n = 2**31 // 2050 + 400, 2050, 300
+    gen = torch.Generator("cuda").manual_seed(3)
+    x, h, dy, dxo = (torch.empty(N, C, device="cuda", dtype=BF16).normal_(generator=gen)
+                     for _ in range(4))
+    w, wp = (torch.rand(C, device="cuda", generator=gen) + 0.5 for _ in range(2))
+
+    def grads(x, h, dy, dxo):
+        x, h = x.requires_grad_(), h.requires_grad_()
+        out = ops.residual_norm(x, h, w, post_weight=wp, out_dtype=BF16)
+        return [t.detach() for t in (*out, *torch.autograd.grad(out, (x, h), (dxo, dy)))]
+
+    assert N * C > 2**31
+    few = grads(*(t[-n:].clone() for t in (x, h, dy, dxo)))
+    for got, want in zip(grads(x, h, dy, dxo), few):
+        assert torch.equal(got[-n:], want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["layer", "rms"])
 def test_constant_rows_and_zero_rows(kind):
     """Rows without variance: 1/std is 1/sqrt(eps), nothing is NaN."""
