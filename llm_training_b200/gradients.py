@@ -127,9 +127,11 @@ def clip_grads(grads, max_norm, out=None):
             raise ValueError(f"{fn}: out must be on the gradients' device, {device}")
         if not all([o.is_contiguous() for o in out]):
             raise ValueError(f"{fn}: out must be contiguous")
-        at = [o.data_ptr() for o in out if o.numel()]
-        if len(set(at)) < len(at):
+        at = {o.data_ptr(): i for i, o in enumerate(out) if o.numel()}
+        if len(at) < sum(o.numel() > 0 for o in out):
             raise ValueError(f"{fn}: out holds one tensor twice")
+        if any([at.get(g.data_ptr(), i) != i for i, g in enumerate(grads)]):
+            raise ValueError(f"{fn}: out holds another gradient's memory")
     return out, _clip(grads, out, max_norm, device)
 
 
@@ -139,7 +141,8 @@ def clip_grad_norm_(parameters, max_norm):
     that their global 2-norm is at most ``max_norm``, and returns the norm before, a
     float32 scalar: ``torch.nn.utils.clip_grad_norm_`` for CUDA float32 and bfloat16
     gradients on one device, with the norm of ``grad_norm``.  A parameter listed twice
-    counts once.  Gradients below the bound are not written.  A NaN norm makes every
+    counts once; parameters that share one gradient tensor are refused, and gradients must
+    not overlap.  Gradients below the bound are not written.  A NaN norm makes every
     gradient NaN, as there.  No gradients: 0."""
     fn = "clip_grad_norm_"
     if isinstance(parameters, torch.Tensor):
@@ -150,6 +153,9 @@ def clip_grad_norm_(parameters, max_norm):
     if not grads:
         return torch.tensor(0.0)
     device = _checked(fn, grads)
+    at = [g.data_ptr() for g in grads if g.numel()]
+    if len(set(at)) < len(at):
+        raise ValueError(f"{fn}: two parameters share one gradient")
     if all([g.is_contiguous() or _dense(g) for g in grads]):
         return _clip(grads, grads, max_norm, device)
     # a gradient with gaps (a view of a larger buffer) goes through a copy

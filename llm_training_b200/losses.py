@@ -333,9 +333,7 @@ def policy_loss_and_grad(logits, targets, advantages, old_logps=None, ref_logps=
     fn = "policy_loss_and_grad"
     args = _policy_args(fn, logits.detach(), targets, advantages, old_logps, ref_logps, clip,
                         clip_high, kl_coef, reduction, cu_seqlens)
-    grad_scale = float(grad_scale)
-    if not math.isfinite(grad_scale):
-        raise ValueError(f"{fn}: grad_scale must be finite, got {grad_scale}")
+    grad_scale = _number(fn, "grad_scale", grad_scale, least=-1e30, most=1e30)
     run = _lib.binding().policy_fwd if _lib.plain(args[0]) else _policy_fwd
     loss, logps, stats, grad = run(*args, grad_scale)
     return loss, grad, logps, stats

@@ -220,6 +220,45 @@ def test_layouts_and_parameters_listed_twice():
 
 
 @pytest.mark.gpu
+def test_more_elements_than_32_bits_count():
+    n = 2**31 + 70_003
+    g = torch.zeros(n, device="cuda", dtype=torch.bfloat16)
+    g[-70_000:] = 2.0
+    g[0] = 2.0
+    other = torch.ones(5, device="cuda")
+    want = (4 * 70_001 + 5) ** 0.5
+    (a, b), norm = ops.clip_grads([g, other], 1.0, out=[torch.empty_like(g), other])
+    # the norm and the factor are rounded to 24 bits, the product once more to 8
+    assert abs(float(norm) - want) <= want * 2**-24
+    factor = 1.0 / (want + 1e-6)
+    for got, times, eps in ((a, 2.0, 2**-8), (b, 1.0, 2**-24)):
+        size = got[got != 0].double()
+        assert (size - times * factor).abs().max() <= times * factor * (eps + 3 * 2**-24)
+    assert int((a != 0).sum()) == 70_001 and a[0] != 0 and (a[-70_000:] != 0).all()
+
+
+@pytest.mark.gpu
+def test_shared_gradients_are_refused():
+    """Memory that would be scaled twice, or read while it is written."""
+    p, q = (torch.nn.Parameter(torch.ones(3, device="cuda")) for _ in range(2))
+    p.grad = q.grad = torch.ones(3, device="cuda")
+    with pytest.raises(ValueError, match="share"):
+        ops.clip_grad_norm_([p, q], 0.5)
+    a, b = torch.ones(4, device="cuda"), torch.ones(4, device="cuda")
+    with pytest.raises(ValueError, match="another gradient"):
+        ops.clip_grads([a, b], 0.5, out=[b, torch.empty_like(a)])
+    with pytest.raises(ValueError, match="another gradient"):
+        ops.clip_grads([a, b], 0.5, out=[b, a])
+    with pytest.raises(ValueError, match="twice"):
+        ops.clip_grads([a, a], 0.5, out=[a, a])
+    assert p.grad.eq(1).all() and a.eq(1).all() and b.eq(1).all()
+    # out of place a gradient may be listed twice: it counts twice
+    (c, d), norm = ops.clip_grads([a, a], 10.0)
+    assert float(norm) == 8**0.5 or abs(float(norm) - 8**0.5) <= 2**-23
+    assert torch.equal(c, a) and torch.equal(d, a)
+
+
+@pytest.mark.gpu
 def test_autograd_sees_the_write():
     """A graph that holds a tensor scaled in place says so, as after any in-place operation."""
     p = torch.nn.Parameter(torch.zeros(8, device="cuda"))

@@ -619,6 +619,44 @@ def test_captured_and_replayed_on_new_inputs():
 
 
 @pytest.mark.gpu
+def test_more_logits_than_32_bits_count():
+    """Rows behind 2**31 logits, and rows that lie that far apart."""
+    V, n = 32_768, 6
+    N = 2**31 // V + 100
+    x = torch.empty(N, V, device="cuda", dtype=torch.bfloat16).normal_(
+        generator=torch.Generator("cuda").manual_seed(4))
+    t = torch.full((N,), -1, device="cuda")
+    t[-n:] = torch.arange(n, device="cuda") * 5000
+    adv = torch.linspace(-1, 2, N, device="cuda")
+    old = torch.linspace(-10, -11, N, device="cuda")
+
+    def everything(x, t, adv, old):
+        x = x.detach().requires_grad_()
+        cu = torch.tensor([0, t.numel() - n // 2, t.numel()], device="cuda")
+        got = []
+        for loss, *others in (ops.preference_loss(x, t, cu_seqlens=cu),
+                              ops.policy_loss(x, t, adv, old, cu_seqlens=cu),
+                              (ops.token_log_probs(x, t),)):
+            got += [loss.detach(), *others]
+            got.append(torch.autograd.grad(loss, x, torch.ones_like(loss))[0][-n:])
+        loss, grad, logps, stats = ops.policy_loss_and_grad(x, t, adv, old, cu_seqlens=cu)
+        assert not grad[: -n].any()
+        return got + [loss, grad[-n:], logps[-n:], stats]
+
+    def same(a, b):
+        for p, q in zip(a, b):
+            if p.dim() == 1 and p.numel() == N:
+                p = p[-n:]
+            assert torch.equal(p, q)
+
+    few = everything(x[-n:].clone(), t[-n:], adv[-n:], old[-n:])
+    same(everything(x, t, adv, old), few)
+    apart = x.flatten().as_strided((n, V), ((N - 1) // (n - 1) * V, 1))
+    apart.copy_(x[-n:].clone())
+    same(everything(apart, t[-n:], adv[-n:], old[-n:]), few)
+
+
+@pytest.mark.gpu
 def test_retained_graph_and_compile():
     x, t, _, _ = batch(2, 6, 65, torch.float32, "plain", masked=0.1)
     x.requires_grad_(True)
