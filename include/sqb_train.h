@@ -7,8 +7,10 @@
  * gradient once in the logits' dtype.  It computes what the reference's
  * calculate_loss (training_utils.py:8-17: F.cross_entropy over the flattened
  * logits under bf16 autocast, fp32 softmax math) computes, per token; the mean
- * over the non-ignored tokens is taken by the caller.  And a LayerNorm (last
- * entry points) with one warp per row and a fixed-order weight gradient.
+ * over the non-ignored tokens is taken by the caller.  A LayerNorm with one
+ * warp per row and a fixed-order weight gradient.  For training on answers:
+ * token log-probabilities, a preference loss, a clipped policy loss, gradient
+ * clipping, and a residual step between two norms.
  *
  * Conventions as in sqrtblock.h: caller-owned device pointers, asynchronous on
  * `stream` (a cudaStream_t; NULL = legacy default stream), return SQB_OK or an
