@@ -331,8 +331,8 @@ __device__ void write_grad(const T* row, T* drow, int V, int64_t t, float m, flo
   const int tail = head + nvec * kN + me;
   if (tail < V) drow[tail] = grad(to_f(row[tail]), tail);
   // the target's element, by the thread that wrote its vector
-  const int at = (int)(t - head);
-  if (t >= head && at < nvec * kN && (at / kN) % kThreads == me)
+  const int64_t at = t - head;  // one past the vocabulary may be past 32 bits
+  if (at >= 0 && at < nvec * kN && ((int)at / kN) % kThreads == me)
     drow[t] = grad(to_f(row[t]), (int)t);
 }
 

@@ -426,6 +426,28 @@ def test_target_past_the_vocabulary_is_nan_in_its_own_row():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [40, 1000, 20_000])
+def test_target_far_past_the_vocabulary(V):
+    """Targets whose low 32 bits lie inside: their rows are NaN, nothing else is written."""
+    far = [2**31, 2**31 + 8, 2**32, 2**32 + 5, 2**32 + V - 1, 2**40 + 33, 2**63 - 1]
+    t = torch.tensor([3] + [k for f in far for k in (f, 3)], device="cuda")
+    inside = t < V
+    gen = torch.Generator("cuda").manual_seed(5)
+    x = torch.randn(t.numel(), V, device="cuda", generator=gen).bfloat16().requires_grad_()
+
+    def both(t):
+        lp = ops.token_log_probs(x, t)
+        return lp.detach(), torch.autograd.grad(lp, x, torch.ones_like(lp))[0]
+
+    for got, want in zip(both(t), both(torch.where(inside, t, -1))):
+        assert torch.equal(got[inside], want[inside])
+        assert got[~inside].isnan().all()
+    cu = torch.tensor([0, t.numel()], device="cuda")
+    grad = ops.policy_loss_and_grad(x, t, torch.ones(t.numel(), device="cuda"), cu_seqlens=cu)[1]
+    assert grad[inside].isfinite().all() and grad[~inside].isnan().all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("V", [33, 5003, 40001])
 def test_rows_without_a_softmax_are_nan(V, dtype):
