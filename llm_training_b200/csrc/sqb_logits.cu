@@ -491,6 +491,8 @@ __global__ void __launch_bounds__(block_of<kThreads>(), kThreads == 32 ? 1 : 153
       terms[r] = terms[(size_t)N + r] = terms[2 * (size_t)N + r] = 0.0;
     }
     if (dx) write_zeros<T, kThreads, true>(drow, V);
+    // no kernel behind this one may start before the weights are there, whatever rows there are
+    if (r == 0 && me == 0) cudaGridDependencySynchronize();
     return;
   }
   const T* row = x + row_offset(r, v.T, v.ss, v.st);

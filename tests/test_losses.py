@@ -84,6 +84,8 @@ def test_bad_arguments_are_refused():
             (ValueError, "reduction", lambda: ops.policy_loss(x, t, adv, reduction="sum")),
             (ValueError, "grad_scale", lambda: ops.policy_loss_and_grad(
                 x, t, adv, grad_scale=math.inf)),
+            (ValueError, "grad_scale", lambda: ops.policy_loss_and_grad(
+                x, t, adv, grad_scale=-1e39)),
         ]
         for kind, text, call in cases:
             with pytest.raises(kind, match=text):
@@ -524,6 +526,24 @@ def test_target_without_probability():
     (g,) = torch.autograd.grad(loss, x)
     assert float(loss) == math.inf and float(chosen[0]) == -math.inf
     assert g.isfinite().all() and float(g[0, 1, t[0, 1]]) == pytest.approx(-0.1, rel=1e-6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [3, 3000])
+def test_no_row_waits_for_weights(V):
+    """A batch of nothing but left-out rows: its kernel has nothing to wait for, and what the
+    memory of the weights held before does not show in the sums."""
+    N = 30_000
+    x = torch.zeros(N, V, device="cuda")
+    t, adv = torch.full((N,), -1, device="cuda"), torch.ones(N, device="cuda")
+    cu = torch.tensor([0, N // 3, N], device="cuda")
+    for _ in range(10):
+        old = [torch.full((n,), math.nan, device="cuda") for n in (N, 8 * N + 66, 9 * N)]
+        del old
+        loss, logps, stats = ops.policy_loss(x, t, adv, cu_seqlens=cu)
+        assert not loss and not stats.any() and not logps.any()
+        loss, grad, logps, stats = ops.policy_loss_and_grad(x, t, adv, cu_seqlens=cu)
+        assert not loss and not stats.any() and not grad.any()
 
 
 @pytest.mark.gpu
