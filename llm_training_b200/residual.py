@@ -2,7 +2,6 @@
 
 from __future__ import annotations
 
-import math
 from typing import Optional
 
 import torch
@@ -143,7 +142,7 @@ def residual_norm(x, h, weight, bias=None, *, post_weight=None, post_bias=None, 
     if post_bias is not None and post_weight is None:
         raise ValueError("residual_norm: a post_bias needs a post_weight")
     scale, eps = float(scale), float(eps)
-    if not math.isfinite(scale) or not (math.isfinite(eps) and eps >= 0):
+    if not abs(scale) <= 1e30 or not 0 <= eps <= 1e30:  # float32 arguments of the kernels
         raise ValueError(f"residual_norm: scale must be finite and eps finite and not negative, "
                          f"got {scale}, {eps}")
     if x.numel() // C > 2**31 - 1:

@@ -46,6 +46,7 @@ def test_refusals():
             (ValueError, "gate", (x, x, w), dict(gate=torch.empty(3, 4, 8, device="cuda"))),
             (ValueError, "gate", (x, x, w), dict(gate=w.double())),
             (ValueError, "scale", (x, x, w), dict(scale=math.nan)),
+            (ValueError, "scale", (x, x, w), dict(scale=1e39)),
             (ValueError, "eps", (x, x, w), dict(eps=-1.0)),
         ]:
             with pytest.raises(kind, match=text):
