@@ -31,22 +31,24 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kPerSm = 4;
 constexpr int kGrid = 148 * kPerSm;  // CTAs on 148 SMs
-constexpr int kMaxTensors = 768;
+// Tensors of a launch, and of one whose smaller table (2 of 23 KB) the host has copied sooner.
+constexpr int kMaxTensors = 768, kFewTensors = 64;
 constexpr int kPiece = 32768;  // elements
 
+template <int kMax>
 struct Table {
-  const void* in[kMaxTensors];
-  void* out[kMaxTensors];
-  int64_t numel[kMaxTensors];
-  int32_t end[kMaxTensors];  // pieces of tensors 0..i
-  uint8_t in_bf16[kMaxTensors], out_bf16[kMaxTensors];
+  const void* in[kMax];
+  void* out[kMax];
+  int64_t numel[kMax];
+  int32_t end[kMax];  // pieces of tensors 0..i
+  uint8_t in_bf16[kMax], out_bf16[kMax];
   int32_t n;
 };
-static_assert(sizeof(Table) <= 32000, "a kernel's arguments are at most 32764 bytes");
+static_assert(sizeof(Table<kMaxTensors>) <= 32000, "a kernel's arguments are at most 32764 bytes");
 
 // Calls f(tensor, first element, elements) for this CTA's pieces.
-template <typename F>
-__device__ __forceinline__ void for_pieces(const Table& t, F&& f) {
+template <int kMax, typename F>
+__device__ __forceinline__ void for_pieces(const Table<kMax>& t, F&& f) {
   const int all = t.end[t.n - 1];
   for (int c = blockIdx.x; c < all; c += gridDim.x) {
     int lo = 0, hi = t.n - 1;  // the first tensor that ends beyond c
@@ -117,8 +119,9 @@ __device__ double square_sum(const T* p, int n) {
   return v[0] + v[1];
 }
 
+template <int kMax>
 __global__ void __launch_bounds__(kThreads, kPerSm)
-    norm_kernel(const __grid_constant__ Table t, double* partial) {
+    norm_kernel(const __grid_constant__ Table<kMax> t, double* partial) {
   __shared__ double red[32];
   double v = 0.0;
   for_pieces(t, [&](int i, int64_t at, int n) {
@@ -182,8 +185,9 @@ __device__ void scale_piece(const I* p, O* o, int n, float f) {
   if (tail < n) put(o + tail, to_f(p[tail]) * f);
 }
 
+template <int kMax>
 __global__ void __launch_bounds__(kThreads, kPerSm)
-    clip_kernel(const __grid_constant__ Table t, const double* partial, int slots,
+    clip_kernel(const __grid_constant__ Table<kMax> t, const double* partial, int slots,
                 float max_norm, bool in_place, float* norm) {
   __shared__ double red[32];
   const float n = norm_of(partial, slots, red);
@@ -212,12 +216,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
 
 // Fills `t` from the next tensors at `at`; returns how many were passed.  Empty
 // tensors take no slot.
-int64_t fill(Table& t, const void* const* in, void* const* out, const int64_t* numel,
+template <int kMax>
+int64_t fill(Table<kMax>& t, const void* const* in, void* const* out, const int64_t* numel,
              const int32_t* in_dtype, const int32_t* out_dtype, int64_t n, int64_t at) {
   t.n = 0;
   int32_t pieces = 0;
   int64_t i = at;
-  for (; i < n && t.n < kMaxTensors; ++i) {
+  for (; i < n && t.n < kMax; ++i) {
     if (numel[i] == 0) continue;
     pieces += (int32_t)((numel[i] + kPiece - 1) / kPiece);
     t.in[t.n] = in[i];
@@ -250,10 +255,14 @@ int check(const void* const* in, void* const* out, const int64_t* numel,
   return SQB_OK;
 }
 
-int grid_of(const Table& t) { return t.end[t.n - 1] < kGrid ? t.end[t.n - 1] : kGrid; }
+template <int kMax>
+int grid_of(const Table<kMax>& t) {
+  return t.end[t.n - 1] < kGrid ? t.end[t.n - 1] : kGrid;
+}
 
 // One launch for each table of tensors; returns the slots of `partial` they write.
-int launch_norms(Table& t, const void* const* in, const int64_t* numel, const int32_t* in_dtype,
+template <int kMax>
+int launch_norms(Table<kMax>& t, const void* const* in, const int64_t* numel, const int32_t* in_dtype,
                  int64_t n, double* partial, cudaStream_t q) {
   int slots = 0;
   for (int64_t at = 0; at < n;) {
@@ -263,6 +272,18 @@ int launch_norms(Table& t, const void* const* in, const int64_t* numel, const in
     slots += grid_of(t);
   }
   return slots;
+}
+
+// Calls f with a table for n tensors.
+template <typename F>
+void with_table(int64_t n, F&& f) {
+  if (n <= kFewTensors) {
+    Table<kFewTensors> t;
+    f(t);
+  } else {
+    Table<kMaxTensors> t;
+    f(t);
+  }
 }
 
 int launched() { return cudaGetLastError() == cudaSuccess ? SQB_OK : SQB_ERR_LAUNCH; }
@@ -286,9 +307,10 @@ extern "C" int sqb_grad_norm(const void* const* grads, const int64_t* numel,
   if (!workspace || ws_bytes < sqb_grad_norm_workspace_bytes(n)) return SQB_ERR_WORKSPACE;
   cudaStream_t q = static_cast<cudaStream_t>(stream);
   double* partial = static_cast<double*>(workspace);
-  Table t;
-  const int slots = launch_norms(t, grads, numel, dtypes, n, partial, q);
-  finish_kernel<<<1, kThreads, 0, q>>>(partial, slots, norm);
+  with_table(n, [&](auto& t) {
+    const int slots = launch_norms(t, grads, numel, dtypes, n, partial, q);
+    finish_kernel<<<1, kThreads, 0, q>>>(partial, slots, norm);
+  });
   return launched();
 }
 
@@ -306,13 +328,14 @@ extern "C" int sqb_grad_clip(const void* const* grads, void* const* outs, const 
   bool in_place = true;
   for (int64_t i = 0; i < n; ++i)
     in_place = in_place && (numel[i] == 0 || (grads[i] == outs[i] && dtypes[i] == out_dtypes[i]));
-  Table t;
-  const int slots = launch_norms(t, grads, numel, dtypes, n, partial, q);
-  if (slots == 0) finish_kernel<<<1, kThreads, 0, q>>>(partial, 0, norm);
-  for (int64_t at = 0; at < n;) {
-    at += fill(t, grads, outs, numel, dtypes, out_dtypes, n, at);
-    if (t.n == 0) continue;
-    clip_kernel<<<grid_of(t), kThreads, 0, q>>>(t, partial, slots, max_norm, in_place, norm);
-  }
+  with_table(n, [&](auto& t) {
+    const int slots = launch_norms(t, grads, numel, dtypes, n, partial, q);
+    if (slots == 0) finish_kernel<<<1, kThreads, 0, q>>>(partial, 0, norm);
+    for (int64_t at = 0; at < n;) {
+      at += fill(t, grads, outs, numel, dtypes, out_dtypes, n, at);
+      if (t.n == 0) continue;
+      clip_kernel<<<grid_of(t), kThreads, 0, q>>>(t, partial, slots, max_norm, in_place, norm);
+    }
+  });
   return launched();
 }

@@ -15,6 +15,7 @@
 #include <dlfcn.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -41,6 +42,9 @@ struct Library {
   SQB_ENTRY(sqb_residual_norm_fwd)
   SQB_ENTRY(sqb_residual_norm_workspace_bytes)
   SQB_ENTRY(sqb_residual_norm_bwd)
+  SQB_ENTRY(sqb_grad_norm_workspace_bytes)
+  SQB_ENTRY(sqb_grad_norm)
+  SQB_ENTRY(sqb_grad_clip)
 #undef SQB_ENTRY
 };
 Library lib;
@@ -64,6 +68,9 @@ void attach(const std::string& path) {
   SQB_ENTRY(sqb_residual_norm_fwd)
   SQB_ENTRY(sqb_residual_norm_workspace_bytes)
   SQB_ENTRY(sqb_residual_norm_bwd)
+  SQB_ENTRY(sqb_grad_norm_workspace_bytes)
+  SQB_ENTRY(sqb_grad_norm)
+  SQB_ENTRY(sqb_grad_clip)
 #undef SQB_ENTRY
 }
 
@@ -369,6 +376,105 @@ struct Residual : torch::autograd::Function<Residual> {
   }
 };
 
+// ---- gradient norm and clipping -------------------------------------------------------------
+
+// The C entries' arrays for tensors that they can take as they are.
+struct Tensors {
+  std::vector<void*> at;
+  std::vector<int64_t> numel;
+  std::vector<int32_t> dtype;
+
+  // Whether they are: plain float32 or bfloat16 tensors on `device`, without gaps (contiguous:
+  // in order, too), no two of them the same memory (`distinct`).
+  bool take(const std::vector<Tensor>& tensors, c10::Device device, bool contiguous,
+            bool distinct) {
+    const size_t n = tensors.size();
+    at.reserve(n), numel.reserve(n), dtype.reserve(n);
+    for (const Tensor& t : tensors) {
+      if (!t.defined() || t.key_set().has(c10::DispatchKey::Python) ||
+          t.layout() != at::kStrided || t.device() != device ||
+          (t.scalar_type() != at::kFloat && t.scalar_type() != at::kBFloat16) ||
+          !(t.is_contiguous() || (!contiguous && t.is_non_overlapping_and_dense())))
+        return false;
+      at.push_back(t.data_ptr());
+      numel.push_back(t.numel());
+      dtype.push_back(dtype_of(t));
+    }
+    return !distinct || none_shared();
+  }
+  std::vector<void*> held() const {  // in order
+    std::vector<void*> h;
+    h.reserve(at.size());
+    for (size_t i = 0; i < at.size(); ++i)
+      if (numel[i]) h.push_back(at[i]);
+    std::sort(h.begin(), h.end());
+    return h;
+  }
+  bool none_shared() const {
+    const auto h = held();
+    return std::adjacent_find(h.begin(), h.end()) == h.end();
+  }
+};
+
+std::tuple<Tensor, Tensor, size_t> norm_buffers(const std::vector<Tensor>& tensors) {
+  const size_t nbytes = lib.sqb_grad_norm_workspace_bytes((int64_t)tensors.size());
+  const auto options = at::TensorOptions(tensors[0].device());
+  return {at::empty({}, options.dtype(at::kFloat)),
+          at::empty({(int64_t)nbytes}, options.dtype(at::kByte)), nbytes};
+}
+
+// The norm, or None for tensors that Python has to look at.
+Maybe grad_norm(const std::vector<Tensor>& tensors) {
+  if (tensors.empty() || !tensors[0].is_cuda()) return std::nullopt;
+  const auto device = tensors[0].device();
+  Tensors in;
+  if (!in.take(tensors, device, false, false)) return std::nullopt;
+  const c10::cuda::CUDAGuard guard(device);
+  auto [norm, ws, nbytes] = norm_buffers(tensors);
+  check("sqb_grad_norm",
+        lib.sqb_grad_norm(in.at.data(), in.numel.data(), in.dtype.data(), (int64_t)in.at.size(),
+                          ws.data_ptr(), nbytes, ptr(norm), stream_of(norm)));
+  return norm;
+}
+
+// (out, norm): the gradients clipped in place, into `out`, or for None into new tensors; None
+// for tensors that Python has to look at.
+std::optional<std::tuple<std::vector<Tensor>, Tensor>> clip(
+    const std::vector<Tensor>& grads, const std::optional<std::vector<Tensor>>& given,
+    double max_norm, bool in_place) {
+  if (grads.empty() || !grads[0].is_cuda()) return std::nullopt;
+  const auto device = grads[0].device();
+  Tensors in, to;
+  if (!in.take(grads, device, !in_place, in_place)) return std::nullopt;
+  std::vector<Tensor> out;
+  const c10::cuda::CUDAGuard guard(device);
+  if (!in_place) {
+    if (given) {
+      out = *given;
+      if (out.size() != grads.size() || !to.take(out, device, true, true)) return std::nullopt;
+      const auto held = in.held();
+      for (size_t i = 0; i < out.size(); ++i)  // each on its own gradient's memory, or on none's
+        if (out[i].sizes() != grads[i].sizes() ||
+            ((to.at[i] != in.at[i] || to.dtype[i] != in.dtype[i]) && to.numel[i] &&
+             std::binary_search(held.begin(), held.end(), to.at[i])))
+          return std::nullopt;
+    } else {
+      out.reserve(grads.size());
+      for (const Tensor& g : grads) out.push_back(at::empty_like(g));
+      to.take(out, device, true, false);
+    }
+  }
+  const Tensors& into = in_place ? in : to;
+  auto [norm, ws, nbytes] = norm_buffers(grads);
+  check("sqb_grad_clip",
+        lib.sqb_grad_clip(in.at.data(), into.at.data(), in.numel.data(), in.dtype.data(),
+                          into.dtype.data(), (int64_t)in.at.size(), (float)max_norm, ws.data_ptr(),
+                          nbytes, ptr(norm), stream_of(norm)));
+  for (const Tensor& t : in_place ? grads : out)  // written behind autograd's back
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  return std::make_tuple(std::move(out), norm);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -384,7 +490,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                         bf16_out ? at::kBFloat16 : at::kFloat);
   });
   m.def("residual_bwd", &residual_bwd);
-  // the same with an autograd node
+  // with an autograd node
   m.def("logp", [](const Tensor& x, const Tensor& t) { return LogP::apply(x, t); });
   m.def("preference", [](const Tensor& x, const Tensor& t, const Maybe& ref, const Maybe& cu,
                          int64_t pairs, double beta, double smooth) {
@@ -405,4 +511,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                                      bf16_out ? at::kBFloat16 : at::kFloat);
     return std::make_tuple(out[0], out[1]);
   });
+  m.def("grad_norm", &grad_norm);
+  m.def("clip", &clip);
 }

@@ -2,7 +2,6 @@
 
 from __future__ import annotations
 
-import array
 import math
 
 import torch
@@ -11,7 +10,7 @@ from . import _lib
 
 __all__ = ["grad_norm", "clip_grads", "clip_grad_norm_"]
 
-_DTYPES = {torch.float32: _lib.SQB_F32, torch.bfloat16: _lib.SQB_BF16}
+_DTYPES = {torch.float32, torch.bfloat16}
 
 
 def _dense(t):
@@ -28,7 +27,7 @@ def _checked(fn, tensors, what="gradients"):
     """The device of `tensors`, all of them strided CUDA float32 or bfloat16 on it."""
     device = tensors[0].device
     if ({t.layout for t in tensors} != {torch.strided}
-            or not {t.dtype for t in tensors} <= _DTYPES.keys()
+            or not {t.dtype for t in tensors} <= _DTYPES
             or {t.device for t in tensors} != {device}):
         for t in tensors:
             if t.layout != torch.strided:
@@ -44,55 +43,24 @@ def _checked(fn, tensors, what="gradients"):
     return device
 
 
-def _tables(tensors):
-    """Host arrays of the tensors' pointers and dtypes."""
-    return (array.array("Q", [t.data_ptr() for t in tensors]),
-            array.array("i", [_DTYPES[t.dtype] for t in tensors]))
-
-
-def _numels(tensors):
-    return array.array("q", [t.numel() for t in tensors])
-
-
-def _at(table):
-    return table.buffer_info()[0]
-
-
-def _workspace(n, device):
-    nbytes = _lib.lib().sqb_grad_norm_workspace_bytes(n)
-    return torch.empty(nbytes // 8, dtype=torch.float64, device=device), nbytes
+def _done(fn, result):
+    if result is None:
+        raise RuntimeError(f"{fn}: needs ordinary CUDA tensors that do not share memory")
+    return result
 
 
 def grad_norm(tensors):
     """2-norm of all elements of ``tensors`` (CUDA float32 or bfloat16, any mixture, one
     device) as a float32 scalar on their device.  The squares are summed in 64 bits in a
     fixed order: no overflow, and the same bits on every run.  No tensors: 0."""
-    tensors = list(tensors)
+    fn, tensors = "grad_norm", list(tensors)
     if not tensors:
         return torch.tensor(0.0)
-    device = _checked("grad_norm", tensors, "tensors")
-    tensors = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in tensors]
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    (ptrs, dtypes), numels = _tables(tensors), _numels(tensors)
-    ws, nbytes = _workspace(len(tensors), device)
-    with _lib.on_device(device):
-        _lib.check("sqb_grad_norm", _lib.lib().sqb_grad_norm(
-            _at(ptrs), _at(numels), _at(dtypes), len(tensors), ws.data_ptr(), nbytes,
-            norm.data_ptr(), _lib.stream(device)))
-    return norm
-
-
-def _clip(grads, outs, max_norm, device):
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    (ptrs, dtypes), numels = _tables(grads), _numels(grads)
-    out_ptrs, out_dtypes = (ptrs, dtypes) if outs is grads else _tables(outs)
-    ws, nbytes = _workspace(len(grads), device)
-    with _lib.on_device(device):
-        _lib.check("sqb_grad_clip", _lib.lib().sqb_grad_clip(
-            _at(ptrs), _at(out_ptrs), _at(numels), _at(dtypes), _at(out_dtypes), len(grads),
-            max_norm, ws.data_ptr(), nbytes, norm.data_ptr(), _lib.stream(device)))
-    # written behind autograd's back
-    torch.autograd.graph.increment_version([o for o in outs if not o.is_inference()])
+    norm = _lib.binding().grad_norm(tensors) if tensors[0].is_cuda else None
+    if norm is None:
+        _checked(fn, tensors, "tensors")
+        norm = _done(fn, _lib.binding().grad_norm(
+            [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in tensors]))
     return norm
 
 
@@ -114,28 +82,34 @@ def clip_grads(grads, max_norm, out=None):
     grads, max_norm = list(grads), _bound(fn, max_norm)
     if not grads:
         return [], torch.tensor(0.0)
-    device = _checked(fn, grads)
-    if not all([g.is_contiguous() for g in grads]):
+    out = list(out) if out is not None else None
+    done = _lib.binding().clip(grads, out, max_norm, False) if grads[0].is_cuda else None
+    if done is None:
+        device = _checked(fn, grads)
+        if out is not None:
+            _check_out(fn, grads, out, device)
         grads = [g.contiguous() for g in grads]
-    if out is None:
-        out = [torch.empty_like(g) for g in grads]
-    else:
-        out = list(out)
-        if [o.shape for o in out] != [g.shape for g in grads]:
-            raise ValueError(f"{fn}: out must hold one tensor of each gradient's shape")
-        if _checked(fn, out, "out") != device:
-            raise ValueError(f"{fn}: out must be on the gradients' device, {device}")
-        if not all([o.is_contiguous() for o in out]):
-            raise ValueError(f"{fn}: out must be contiguous")
-        at = {o.data_ptr(): i for i, o in enumerate(out) if o.numel()}
-        if len(at) < sum(o.numel() > 0 for o in out):
-            raise ValueError(f"{fn}: out holds one tensor twice")
-        if any([at.get(g.data_ptr(), i) != i for i, g in enumerate(grads)]):
-            raise ValueError(f"{fn}: out holds another gradient's memory")
-    return out, _clip(grads, out, max_norm, device)
+        done = _done(fn, _lib.binding().clip(grads, out, max_norm, False))
+    return out if out is not None else done[0], done[1]
 
 
-@torch.no_grad()
+def _check_out(fn, grads, out, device):
+    if [o.shape for o in out] != [g.shape for g in grads]:
+        raise ValueError(f"{fn}: out must hold one tensor of each gradient's shape")
+    if _checked(fn, out, "out") != device:
+        raise ValueError(f"{fn}: out must be on the gradients' device, {device}")
+    if not all([o.is_contiguous() for o in out]):
+        raise ValueError(f"{fn}: out must be contiguous")
+    at = {o.data_ptr(): i for i, o in enumerate(out) if o.numel()}
+    if len(at) < sum(o.numel() > 0 for o in out):
+        raise ValueError(f"{fn}: out holds one tensor twice")
+    if any([at.get(g.data_ptr(), i) != i for i, g in enumerate(grads)]):
+        raise ValueError(f"{fn}: out holds another gradient's memory")
+    if any([o.data_ptr() == g.data_ptr() and (o.dtype != g.dtype or not g.is_contiguous())
+            for g, o in zip(grads, out) if o.numel()]):
+        raise ValueError(f"{fn}: out holds a gradient's memory in another layout or dtype")
+
+
 def clip_grad_norm_(parameters, max_norm):
     """Scales the gradients of ``parameters`` (an iterable of tensors, or one) in place so
     that their global 2-norm is at most ``max_norm``, and returns the norm before, a
@@ -152,20 +126,22 @@ def clip_grad_norm_(parameters, max_norm):
     max_norm = _bound(fn, max_norm)
     if not grads:
         return torch.tensor(0.0)
-    device = _checked(fn, grads)
+    done = _lib.binding().clip(grads, None, max_norm, True) if grads[0].is_cuda else None
+    if done is not None:
+        return done[1]
+    _checked(fn, grads)
     at = [g.data_ptr() for g in grads if g.numel()]
     if len(set(at)) < len(at):
         raise ValueError(f"{fn}: two parameters share one gradient")
-    if all([g.is_contiguous() or _dense(g) for g in grads]):
-        return _clip(grads, grads, max_norm, device)
     # a gradient with gaps (a view of a larger buffer) goes through a copy
     for g in grads:
         if any(s == 0 and n > 1 for n, s in zip(g.shape, g.stride())):
             raise ValueError(f"{fn}: a gradient expanded over its own memory cannot be scaled "
                              "in place")
     work = [g if g.is_contiguous() or _dense(g) else g.contiguous() for g in grads]
-    norm = _clip(work, work, max_norm, device)
-    for g, w in zip(grads, work):
-        if w is not g:
-            g.copy_(w)
+    _, norm = _done(fn, _lib.binding().clip(work, None, max_norm, True))
+    with torch.no_grad():
+        for g, w in zip(grads, work):
+            if w is not g:
+                g.copy_(w)
     return norm
