@@ -6,8 +6,11 @@
 // run for 10 us, and its Python node is called by autograd's device thread, which has to get
 // the interpreter's lock from the thread that waits for it.  A short preference step, forward
 // and backward, took 260 us as a registered custom op, 140 us as a Python function.
+// Clipping walks over the gradients here for the same reason: 24 small ones took 46 us from
+// Python, 15 us so.
 //
-// Arguments are checked by the Python entry points.  A failed call of the library throws
+// Arguments are checked by the Python entry points (clipping: here, and what does not pass,
+// there).  A failed call of the library throws
 // (a RuntimeError in Python).
 
 #include <c10/cuda/CUDAGuard.h>
