@@ -7,7 +7,6 @@ raises, and every op that needs it fails with that error.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import importlib.machinery
 import importlib.util
@@ -139,20 +138,6 @@ def binding():
                 module.attach(library_path())
                 _binding = module
     return _binding
-
-
-def on_device(device):
-    """Context in which `device` is the current one: a launch goes to the current device,
-    whatever its stream's."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
-def stream(device) -> int:
-    """The current stream of a CUDA device, as the library takes it."""
-    return torch._C._cuda_getCurrentRawStream(
-        torch.cuda.current_device() if device.index is None else device.index)
 
 
 def plain(x) -> bool:

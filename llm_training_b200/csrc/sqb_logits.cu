@@ -358,7 +358,6 @@ __device__ __forceinline__ double logp_of(const T* row, int V, int64_t t, float 
   return logp_of(t < V ? (double)to_f(row[t]) : (double)NAN, m, s);
 }
 
-
 // ---- rows -------------------------------------------------------------------------
 
 // Threads of a row's CTA: of the kernels that only read it (4685 of 8192 rows of 50304 bf16:
@@ -429,7 +428,7 @@ __global__ void __launch_bounds__(block_of<kThreads>())
     write_zeros<T, kThreads, false>(drow, (int)v.V);
   else
     write_grad<T, kThreads, false>(x + row_offset(r, v.T, v.ss, v.st), drow, (int)v.V, t, ms.x,
-                            -g / ms.y, g);
+                                   -g / ms.y, g);
 }
 
 // Per-row terms of the policy loss.  In all of it NaN arguments give NaN results.
@@ -462,7 +461,6 @@ __device__ __noinline__ double policy_terms(double A, bool has_old, double old_l
   }
   return d;
 }
-
 
 // One row of the policy loss: log-probability, terms and d loss / d logp; with dx, also the
 // row's gradient times `scale`, the row read again where it is still in L2.  Launched while

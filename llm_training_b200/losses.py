@@ -29,8 +29,9 @@ _INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 
 def _grad_strides(x):
-    """Strides of the gradient, as the binding makes it: x's, or where x's rows lie far apart (a few tokens of a longer
-    batch) ones without the gaps, that keep every row's place between 16-byte boundaries."""
+    """Strides of the gradient, as the binding makes it: x's, or where x's rows lie far apart
+    (a few tokens of a longer batch) ones without the gaps, that keep every row's place
+    between 16-byte boundaries."""
     strides = x.stride()
     if x.numel() == 0 or 1 + sum((n - 1) * s for n, s in zip(x.shape, strides)) <= 2 * x.numel():
         return strides
