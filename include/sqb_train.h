@@ -96,13 +96,15 @@ int sqb_add_layernorm_bwd(const void* dy, int dy_dtype, const float* x_out, cons
 
 /* Per row: logp = log softmax(logits)[target], and stats = (m, sum of exp(x - m)) with m
  * a number near the row's maximum, fp32 (S * T, 2), 8-byte aligned (a row left out:
- * (0, 1)). */
+ * (0, 0), which no other row has; a target of V or more: the sum is NaN). */
 int sqb_logp_fwd(const void* logits, const int64_t* targets, float* logp, float* stats, int64_t S,
                  int64_t T, int64_t V, int64_t ss, int64_t st, int dtype, void* stream);
 
 /* dlogits[r, c] = g_row[r] * scale[0] * ([c == target] - softmax(logits)[r, c]) in the
- * logits' dtype, strides dss and dst; scale (one fp32 on the device) may be NULL.  Rows
- * whose 16-byte phase is the logits' are written with vector stores. */
+ * logits' dtype, strides dss and dst; scale (one fp32 on the device) may be NULL.  Zero for
+ * rows whose target is negative or whose statistics say that they are left out, whatever
+ * their target, factor and logits.  Rows whose 16-byte phase is the logits' are written with
+ * vector stores. */
 int sqb_logp_bwd(const void* logits, const int64_t* targets, const float* stats,
                  const float* g_row, const float* scale, void* dlogits, int64_t S, int64_t T,
                  int64_t V, int64_t ss, int64_t st, int64_t dss, int64_t dst, int dtype,

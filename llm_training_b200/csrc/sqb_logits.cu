@@ -357,6 +357,10 @@ template <typename T>
 __device__ __forceinline__ double logp_of(const T* row, int V, int64_t t, float m, double s) {
   return logp_of(t < V ? (double)to_f(row[t]) : (double)NAN, m, s);
 }
+// What is kept of a row for its gradient: NaN for a target past the vocabulary.
+__device__ __forceinline__ float2 stats_of(int64_t V, int64_t t, float m, double s) {
+  return make_float2(m, t < V ? (float)s : NAN);
+}
 
 // ---- rows -------------------------------------------------------------------------
 
@@ -380,6 +384,23 @@ __device__ __forceinline__ uint32_t row_of() {
   return kThreads == 32 ? blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
 }
 
+// Rows of a packed batch that lie in a sequence: [cu[0], cu[seqs]), all for a null cu.
+struct Inside {
+  const int64_t* cu;
+  int64_t seqs;
+};
+
+// The row's target; negative for a row that is left out: without one, or in no sequence.
+__device__ __forceinline__ int64_t target_of(const int64_t* targets, const Inside& in,
+                                             uint32_t r) {
+  const int64_t t = targets[r];
+  return in.cu && (r < in.cu[0] || r >= in.cu[in.seqs]) ? -1 : t;
+}
+
+// The statistics of a row that is left out, which tell the backward so: a softmax's sum is at
+// least a half, or 0 next to a maximum of -inf.
+__device__ __forceinline__ float2 left_out() { return make_float2(0.f, 0.f); }
+
 // Per-row outputs: logp (either or both), stats = (m, s), and a zero for g_row.
 struct RowOut {
   float* logp;
@@ -390,20 +411,26 @@ struct RowOut {
 
 template <typename T, int kThreads>
 __global__ void __launch_bounds__(block_of<kThreads>())
-    logp_fwd_kernel(const T* x, const int64_t* targets, RowOut out, View v, uint32_t N) {
+    logp_fwd_kernel(const T* x, const int64_t* targets, Inside in, RowOut out, View v,
+                    uint32_t N) {
   __shared__ Part red[32];
   const uint32_t r = row_of<kThreads>();
   if (kThreads == 32 && r >= N) return;
-  const int64_t t = targets[r];
-  float m = 0.f;
-  double s = 1.0, lp = 0.0;
+  const int64_t t = target_of(targets, in, r);
+  float2 ms = left_out();
+  double lp = 0.0;
   if (t >= 0) {
     const T* row = x + row_offset(r, v.T, v.ss, v.st);
+    float m;
+    double s;
     row_stats<T, kThreads>(row, (int)v.V, red, m, s);
-    if (rank<kThreads>() == 0) lp = logp_of(row, (int)v.V, t, m, s);
+    if (rank<kThreads>() == 0) {
+      lp = logp_of(row, (int)v.V, t, m, s);
+      ms = stats_of(v.V, t, m, s);
+    }
   }
   if (rank<kThreads>() == 0) {
-    out.stats[r] = make_float2(m, (float)s);
+    out.stats[r] = ms;
     if (out.logp) out.logp[r] = (float)lp;
     if (out.logp64) out.logp64[r] = lp;
     if (out.g_row) out.g_row[r] = 0.f;
@@ -419,12 +446,12 @@ __global__ void __launch_bounds__(block_of<kThreads>())
   const int64_t t = targets[r];
   T* drow = dx + row_offset(r, v.T, dss, dst);
   const float2 ms = stats[r];
-  float g = t < 0 ? 0.f : g_row[r];
-  if (t >= 0 && scale) g *= *scale;
-  if (t >= v.V) g = NAN;
-  // a zero factor (an ignored token, a clipped one) makes a zero row, which needs no
-  // logits - unless they hold a NaN or an infinity, which the sum then shows
-  if (t < 0 || (g == 0.f && isfinite(ms.x) && isfinite(ms.y)))
+  const bool left = t < 0 || (ms.x == 0.f && ms.y == 0.f);
+  float g = left ? 0.f : g_row[r];
+  if (!left && scale) g *= *scale;
+  // a zero factor (a clipped token) makes a zero row, which needs no logits - unless they
+  // hold a NaN or an infinity or have no such target, which the sum then shows
+  if (left || (g == 0.f && isfinite(ms.x) && isfinite(ms.y)))
     write_zeros<T, kThreads, false>(drow, (int)v.V);
   else
     write_grad<T, kThreads, false>(x + row_offset(r, v.T, v.ss, v.st), drow, (int)v.V, t, ms.x,
@@ -472,19 +499,20 @@ __device__ __noinline__ double policy_terms(double A, bool has_old, double old_l
 // spilled registers); the row kept in shared memory, two an SM, 284 us.
 template <typename T, int kThreads>
 __global__ void __launch_bounds__(block_of<kThreads>(), kThreads == 32 ? 1 : 1536 / kThreads)
-    policy_kernel(const T* x, const int64_t* targets, Policy p, RowOut out, double* terms, T* dx,
-                  float scale, View v, int64_t dss, int64_t dst, uint32_t N) {
+    policy_kernel(const T* x, const int64_t* targets, Inside in, Policy p, RowOut out,
+                  double* terms, T* dx, float scale, View v, int64_t dss, int64_t dst,
+                  uint32_t N) {
   __shared__ Part red[32];
   __shared__ float3 known;
   const uint32_t r = row_of<kThreads>();
   if (kThreads == 32 && r >= N) return;
-  const int64_t t = targets[r];
+  const int64_t t = target_of(targets, in, r);
   const int me = rank<kThreads>(), V = (int)v.V;
   T* drow = dx ? dx + row_offset(r, v.T, dss, dst) : nullptr;
   if (t < 0) {
     if (me == 0) {
       out.logp[r] = 0.f;
-      if (out.stats) out.stats[r] = make_float2(0.f, 1.f);
+      if (out.stats) out.stats[r] = left_out();
       if (out.g_row) out.g_row[r] = 0.f;
       terms[r] = terms[(size_t)N + r] = terms[2 * (size_t)N + r] = 0.0;
     }
@@ -508,22 +536,22 @@ __global__ void __launch_bounds__(block_of<kThreads>(), kThreads == 32 ? 1 : 153
     const float w = p.weight[r];
     double term[3] = {0.0, 0.0, 0.0};
     float g = 0.f;
-    if (w != 0.f) {  // else outside every sequence: left out
+    float2 ms = left_out();
+    if (w != 0.f) {  // else between sequences that do not follow one another: left out
+      ms = stats_of(V, t, m, s);
       const uint32_t a = p.by_seq ? (p.seq ? (uint32_t)p.seq[r] : r / (uint32_t)v.T) : r;
       g = (float)(policy_terms(p.adv[a], p.old_logp, old_logp, p.ref_logp, ref_logp, p.lo, p.hi,
                                p.kl_coef, lp, term) *
                   (double)w);
-    } else {
-      m = 0.f, s = 1.0;
     }
     out.logp[r] = w != 0.f ? (float)lp : 0.f;
-    if (out.stats) out.stats[r] = make_float2(m, (float)s);
+    if (out.stats) out.stats[r] = ms;
     if (out.g_row) out.g_row[r] = g;
     terms[r] = term[0];
     terms[(size_t)N + r] = term[1];
     terms[2 * (size_t)N + r] = term[2];
-    const float gs = g * scale;
-    f = make_float3(m, gs == 0.f && isfinite(m) && isfinite(s) ? 0.f : -gs / (float)s, gs);
+    const float gs = w != 0.f ? g * scale : 0.f;
+    f = make_float3(ms.x, gs == 0.f && isfinite(ms.x) && isfinite(ms.y) ? 0.f : -gs / ms.y, gs);
     if (kThreads > 32) known = f;
   }
   if (!dx) return;
@@ -737,13 +765,14 @@ void dispatch(int dtype, int64_t N, int64_t V, F&& f) {
     warp ? f(float(), W(), packed) : f(float(), B(), rows);
 }
 
-void launch_logp(const void* x, const int64_t* targets, const RowOut& out, int64_t S, int64_t T,
-                 int64_t V, int64_t ss, int64_t st, int dtype, cudaStream_t q) {
+void launch_logp(const void* x, const int64_t* targets, const Inside& in, const RowOut& out,
+                 int64_t S, int64_t T, int64_t V, int64_t ss, int64_t st, int dtype,
+                 cudaStream_t q) {
   dispatch<kReadThreads>(dtype, S * T, V, [&](auto type, auto threads, unsigned grid) {
     using X = decltype(type);
     constexpr int kThreads = decltype(threads)::value;
     logp_fwd_kernel<X, kThreads><<<grid, block_of<kThreads>(), 0, q>>>(
-        static_cast<const X*>(x), targets, out, View{T, V, ss, st}, (uint32_t)(S * T));
+        static_cast<const X*>(x), targets, in, out, View{T, V, ss, st}, (uint32_t)(S * T));
   });
 }
 
@@ -761,7 +790,8 @@ extern "C" int sqb_logp_fwd(const void* logits, const int64_t* targets, float* l
   if (!logits || !targets || !logp || !stats || !dims_ok(S, T, V)) return SQB_ERR_ARG;
   if (!elt_of(dtype)) return SQB_ERR_DTYPE;
   const RowOut out{logp, nullptr, reinterpret_cast<float2*>(stats), nullptr};
-  launch_logp(logits, targets, out, S, T, V, ss, st, dtype, static_cast<cudaStream_t>(stream));
+  launch_logp(logits, targets, Inside{nullptr, 0}, out, S, T, V, ss, st, dtype,
+              static_cast<cudaStream_t>(stream));
   return launched();
 }
 
@@ -807,7 +837,8 @@ extern "C" int sqb_preference_fwd(const void* logits, const int64_t* targets,
   double* pair_loss = logp + align256((size_t)N * sizeof(double)) / sizeof(double);
   // rows of a packed batch that belong to no sequence keep the zero written here
   const RowOut out{nullptr, logp, reinterpret_cast<float2*>(stats), cu_seqlens ? g_row : nullptr};
-  if (N > 0) launch_logp(logits, targets, out, S, T, V, ss, st, dtype, q);
+  if (N > 0)
+    launch_logp(logits, targets, Inside{cu_seqlens, 2 * P}, out, S, T, V, ss, st, dtype, q);
   if (N > 0)
     launch_early(preference_pair_kernel, (unsigned)P, kSeqThreads, q, logp, cu_seqlens, ref_logps,
                  P, T, N, beta, label_smoothing, pair_loss, rewards, g_row);
@@ -857,8 +888,8 @@ extern "C" int sqb_policy_fwd(const void* logits, const int64_t* targets,
     using X = decltype(type);
     constexpr int kThreads = decltype(threads)::value;
     launch_early(policy_kernel<X, kThreads>, grid, block_of<kThreads>(), q,
-                 static_cast<const X*>(logits), targets, p, out, terms, static_cast<X*>(dlogits),
-                 grad_scale, View{T, V, ss, st}, dss, dst, (uint32_t)N);
+                 static_cast<const X*>(logits), targets, Inside{cu_seqlens, seqs}, p, out, terms,
+                 static_cast<X*>(dlogits), grad_scale, View{T, V, ss, st}, dss, dst, (uint32_t)N);
   };
   if (dlogits)
     dispatch<kWriteThreads>(dtype, N, V, rows);
