@@ -484,7 +484,7 @@ __device__ __noinline__ double policy_terms(double A, bool has_old, double old_l
   if (has_ref) {
     const double gap = ref_logp - lp, e = expm1(gap);
     term[1] = e - gap;
-    d -= kl_coef * e;
+    if (kl_coef != 0.0) d -= kl_coef * e;  // e may be infinite where the KL is only logged
   }
   return d;
 }

@@ -305,7 +305,8 @@ def policy_loss(logits, targets, advantages, old_logps=None, ref_logps=None, *, 
 
     averaged over the counted tokens (``reduction="token"``), or over each sequence's
     counted tokens and then over the sequences that have any (``"sequence"``); 0 where no
-    token is counted.  ``clip_high`` None is ``clip``.  ``old_logps`` and ``ref_logps``
+    token is counted.  ``clip_high`` None is ``clip``; with a ``kl_coef`` of 0 ``ref_logps``
+    serve the statistics alone, whatever they hold.  ``old_logps`` and ``ref_logps``
     have the targets' shape, ``advantages`` that or one value per sequence (a 1-D tensor
     of as many values as a packed batch has rows is one per token).  The gradient of a
     token on the clip's border is the unclipped one.  What the inputs hold at tokens that
