@@ -628,7 +628,9 @@ __global__ void __launch_bounds__(kSeqThreads)
   const double dz = smooth * sigmoid(z) - (1.0 - smooth) * sigmoid(-z);
   const float g = (float)(dz * beta / (double)P);
   if (threadIdx.x == 0) {
-    pair_loss[p] = (1.0 - smooth) * softplus(-z) + smooth * softplus(z);
+    // a term without weight is not there: its softplus may be infinite
+    pair_loss[p] = (smooth != 1.0 ? (1.0 - smooth) * softplus(-z) : 0.0) +
+                   (smooth != 0.0 ? smooth * softplus(z) : 0.0);
     rewards[p] = (float)(beta * ratio[0]);
     rewards[P + p] = (float)(beta * ratio[1]);
   }

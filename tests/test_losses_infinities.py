@@ -43,3 +43,23 @@ def test_kl_for_logging_only(far, V, dtype):
         assert loss.isfinite() and g.isfinite().all() and grad.isfinite().all()
         got.append([loss.detach(), logps, stats[0], stats[2], g, one, grad])
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@DTYPES
+@VOCABULARIES
+@pytest.mark.parametrize("smooth", [0.0, 1.0])
+def test_preference_term_of_coefficient_zero(smooth, V, dtype):
+    """A pair's z is +inf or -inf where one of its answers has no probability.  The term that
+    counts is then 0 or +inf, the other one is not there."""
+    for rejected in (False, True):
+        x, t = batch(V, dtype, 2)
+        if rejected:
+            x, t = x.flip(0), t.flip(0)
+        x = x.clone().requires_grad_(True)
+        loss, chosen, lost = ops.preference_loss(x, t, label_smoothing=smooth)
+        (g,) = torch.autograd.grad(loss, x)
+        assert float((lost if rejected else chosen)[0]) == -math.inf
+        assert float(loss) == (0.0 if rejected == (smooth == 0.0) else math.inf)
+        assert g.isfinite().all()
+        # the loss's slope: 0 where it is flat, -beta or beta where it is straight
+        assert bool(g.any()) == (float(loss) == math.inf)
