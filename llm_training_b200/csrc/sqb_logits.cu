@@ -473,7 +473,8 @@ struct Policy {
 __device__ __noinline__ double policy_terms(double A, bool has_old, double old_logp,
                                             bool has_ref, double ref_logp, double lo, double hi,
                                             double kl_coef, double lp, double* term) {
-  const double ratio = has_old ? exp(lp - old_logp) : exp(lp - lp);
+  // without an old one 1, also for a -inf log-probability
+  const double ratio = has_old ? exp(lp - old_logp) : isnan(lp) ? lp : 1.0;
   const double kept = ratio < lo ? lo : ratio > hi ? hi : ratio;
   const double open = ratio * A, held = kept * A;
   const bool clipped = held < open;

@@ -63,3 +63,39 @@ def test_preference_term_of_coefficient_zero(smooth, V, dtype):
         assert g.isfinite().all()
         # the loss's slope: 0 where it is flat, -beta or beta where it is straight
         assert bool(g.any()) == (float(loss) == math.inf)
+
+
+@DTYPES
+@VOCABULARIES
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+def test_ratio_without_old_logps_is_one(reduction, V, dtype):
+    """Also for a token without probability: its term is -A, its gradient that of the
+    log-probability."""
+    x, t = batch(V, dtype)
+    adv = torch.linspace(-1, 2, 4, device="cuda")
+    leaf = x.clone().requires_grad_(True)
+    loss, logps, stats = ops.policy_loss(leaf, t, adv, reduction=reduction)
+    (g,) = torch.autograd.grad(loss, leaf)
+    one, grad, _, _ = ops.policy_loss_and_grad(x, t, adv, reduction=reduction)
+    want = -adv.double().mean()  # as many tokens in every sequence
+    for v in (loss, one, stats[0]):
+        # weights, advantages and the result rounded to fp32, of terms up to 2
+        assert abs(float(v) - float(want)) <= 2 * 4 * 2.0**-24
+    assert float(logps[0, 1]) == -math.inf
+    for v in (g, grad):
+        p = torch.softmax(x[0, 1].double(), -1)
+        p[t[0, 1]] -= 1.0
+        exact = float(adv[0]) / 12 * p
+        # V / 32 + 100 roundings in a row's sum at most, as for the other losses
+        room = exact.abs() * (torch.finfo(dtype).eps / 2 * 1.01 + (V / 32 + 100) * 2.0**-24)
+        assert ((v[0, 1].double() - exact).abs() <= room + 2.0**-126).all()
+        assert v.isfinite().all()
+
+
+def test_nan_log_probabilities_stay_nan_without_old_logps():
+    x, t = batch(9, torch.float32)
+    x[1, 0] = math.nan
+    t[2, 1] = 9  # past the vocabulary
+    loss, grad, logps, _ = ops.policy_loss_and_grad(x, t, torch.ones(4, device="cuda"))
+    assert loss.isnan() and grad[1, 0].isnan().all() and grad[2, 1].isnan().all()
+    assert logps[1, 0].isnan() and logps[2, 1].isnan() and int(logps.isnan().sum()) == 2
