@@ -107,16 +107,22 @@ Tensor floats(const Tensor& like, int64_t n) {
 Tensor or_none(const Maybe& t) { return t ? *t : Tensor(); }
 
 // A node that refuses to be differentiated: what a backward that has no derivative of its own
-// hands on while a graph of the gradients is being made.
+// hands on while a graph of the gradients is being made.  It depends on all that the gradient
+// depends on: a derivative with respect to any of it has to come through here, and is not
+// taken for zero where the gradient is a part of a larger expression.
 struct NoSecond : torch::autograd::Function<NoSecond> {
-  static Tensor forward(AutogradContext*, const Tensor& t) { return t.view_as(t); }
+  static Tensor forward(AutogradContext*, const Tensor& grad, const Tensor&) {
+    return grad.view_as(grad);
+  }
   static variable_list backward(AutogradContext*, const variable_list&) {
     TORCH_CHECK(false, "this operator has no second derivative");
   }
 };
-Tensor once(const Tensor& grad) {
+Tensor once(Tensor grad, const variable_list& from) {
   if (!at::GradMode::is_enabled() || !grad.defined()) return grad;
-  return NoSecond::apply(grad.detach().requires_grad_(true));
+  for (const Tensor& t : from)
+    if (t.defined() && t.requires_grad()) grad = NoSecond::apply(grad, t);
+  return grad;
 }
 
 // ---- losses on logits: x (S, T, V) or (N, V), t one int64 target a row --------------------
@@ -186,7 +192,8 @@ Tensor logp_bwd(const Tensor& x, const Tensor& t, const Tensor& stats, const May
 
 Tensor loss_grad(AutogradContext* ctx, const Tensor& up) {
   const auto saved = ctx->get_saved_variables();
-  return once(logp_bwd(saved[0], saved[1], saved[2], std::nullopt, up.to(at::kFloat)));
+  return once(logp_bwd(saved[0], saved[1], saved[2], std::nullopt, up.to(at::kFloat)),
+              {saved[0], up});
 }
 
 struct LogP : torch::autograd::Function<LogP> {
@@ -198,7 +205,8 @@ struct LogP : torch::autograd::Function<LogP> {
   static variable_list backward(AutogradContext* ctx, variable_list up) {
     const auto saved = ctx->get_saved_variables();
     return {once(logp_bwd(saved[0], saved[1], saved[2], up[0].to(at::kFloat).contiguous(),
-                          std::nullopt)),
+                          std::nullopt),
+                 {saved[0], up[0]}),
             Tensor()};
   }
 };
@@ -366,13 +374,18 @@ struct Residual : torch::autograd::Function<Residual> {
                                      maybe(s[5]), maybe(s[6]), ctx->saved_data["scale"].toDouble(),
                                      ctx->saved_data["eps"].toDouble(),
                                      ctx->saved_data["rms"].toBool(), s[7]);
-    grads[0] = once(dx);
-    grads[1] = once(dh);
+    variable_list from;
+    if (at::GradMode::is_enabled()) {
+      from.assign(s.begin(), s.begin() + 7);
+      from.insert(from.end(), up.begin(), up.end());
+    }
+    grads[0] = once(dx, from);
+    grads[1] = once(dh, from);
     int64_t at = 0;
     for (int i = 2; i < 7; ++i)
       if (s[i].defined()) {
         const Tensor part = dp.narrow(0, at, s[i].numel());
-        grads[i] = once(s[i].dim() == 1 ? part : part.view(s[i].sizes()));
+        grads[i] = once(s[i].dim() == 1 ? part : part.view(s[i].sizes()), from);
         at += s[i].numel();
       }
     return grads;
