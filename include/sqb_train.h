@@ -14,7 +14,8 @@
  *
  * Conventions as in sqrtblock.h: caller-owned device pointers, asynchronous on
  * `stream` (a cudaStream_t; NULL = legacy default stream), return SQB_OK or an
- * SQB_ERR_* code.  logits / dlogits are (N, ld) row-major with ld >= V,
+ * SQB_ERR_* code.  From the token log-probabilities on, every pointer off its type's
+ * boundary is refused with SQB_ERR_ALIGN.  logits / dlogits are (N, ld) row-major with ld >= V,
  * dtype SQB_BF16 or SQB_F32; columns [V, ld) of logits are not read.  A column
  * holding -inf takes no probability and gets a zero gradient.
  */
@@ -152,7 +153,7 @@ int sqb_policy_fwd(const void* logits, const int64_t* targets, const int64_t* cu
  * n tensors as host arrays of device pointers (element-aligned), element counts (0
  * allowed) and dtypes; the arrays are read before the call returns.
  * norm: one fp32 on the device, sqrt of the sum of squares, summed in 64 bits in a
- * fixed order. */
+ * fixed order.  The workspace is 8-byte aligned. */
 size_t sqb_grad_norm_workspace_bytes(int64_t n_tensors);
 int sqb_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtypes,
                   int64_t n, void* workspace, size_t ws_bytes, float* norm, void* stream);
@@ -182,7 +183,8 @@ size_t sqb_residual_norm_workspace_bytes(int64_t N, int64_t C, int64_t gates);
 
 /* Backward from x, h and the forward's stats: dy (y_dtype), dx_out (x's dtype; NULL: 0)
  * -> dx, dh in x's and h's dtypes and the gradient of every parameter given (fp32,
- * overwritten; dgate (gates, C)), summed in a fixed order.  At most 65530 gates. */
+ * overwritten; dgate (gates, C)), summed in a fixed order.  At most 65530 gates.  The
+ * workspace is 16-byte aligned. */
 int sqb_residual_norm_bwd(const void* dy, int y_dtype, const void* dx_out, const void* x,
                           int x_dtype, const void* h, int h_dtype, const float* weight,
                           const float* bias, const float* post_weight, const float* post_bias,

@@ -286,6 +286,12 @@ void with_table(int64_t n, F&& f) {
   }
 }
 
+// The scratch's doubles and the norm on their boundaries.
+bool aligned(const void* workspace, const float* norm) {
+  return reinterpret_cast<uintptr_t>(workspace) % sizeof(double) == 0 &&
+         reinterpret_cast<uintptr_t>(norm) % sizeof(float) == 0;
+}
+
 int launched() { return cudaGetLastError() == cudaSuccess ? SQB_OK : SQB_ERR_LAUNCH; }
 
 }  // namespace
@@ -305,6 +311,7 @@ extern "C" int sqb_grad_norm(const void* const* grads, const int64_t* numel,
   if (!grads || !numel || !dtypes || n <= 0 || !norm) return SQB_ERR_ARG;
   if (const int rc = check(grads, nullptr, numel, dtypes, nullptr, n)) return rc;
   if (!workspace || ws_bytes < sqb_grad_norm_workspace_bytes(n)) return SQB_ERR_WORKSPACE;
+  if (!aligned(workspace, norm)) return SQB_ERR_ALIGN;
   cudaStream_t q = static_cast<cudaStream_t>(stream);
   double* partial = static_cast<double*>(workspace);
   with_table(n, [&](auto& t) {
@@ -323,6 +330,7 @@ extern "C" int sqb_grad_clip(const void* const* grads, void* const* outs, const 
     return SQB_ERR_ARG;
   if (const int rc = check(grads, outs, numel, dtypes, out_dtypes, n)) return rc;
   if (!workspace || ws_bytes < sqb_grad_norm_workspace_bytes(n)) return SQB_ERR_WORKSPACE;
+  if (!aligned(workspace, norm)) return SQB_ERR_ALIGN;
   cudaStream_t q = static_cast<cudaStream_t>(stream);
   double* partial = static_cast<double*>(workspace);
   bool in_place = true;

@@ -781,6 +781,12 @@ void launch_logp(const void* x, const int64_t* targets, const Inside& in, const 
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
+// Whether every pointer (a null one, too) is a multiple of `bytes`.
+template <typename... P>
+bool aligned(uintptr_t bytes, P... p) {
+  return (... && (reinterpret_cast<uintptr_t>(p) % bytes == 0));
+}
+
 }  // namespace
 }  // namespace logits
 }  // namespace sqb
@@ -791,7 +797,10 @@ extern "C" int sqb_logp_fwd(const void* logits, const int64_t* targets, float* l
                             int64_t S, int64_t T, int64_t V, int64_t ss, int64_t st, int dtype,
                             void* stream) {
   if (!logits || !targets || !logp || !stats || !dims_ok(S, T, V)) return SQB_ERR_ARG;
-  if (!elt_of(dtype)) return SQB_ERR_DTYPE;
+  const int elt = elt_of(dtype);
+  if (!elt) return SQB_ERR_DTYPE;
+  if (!aligned(elt, logits) || !aligned(8, targets, stats) || !aligned(4, logp))
+    return SQB_ERR_ALIGN;
   const RowOut out{logp, nullptr, reinterpret_cast<float2*>(stats), nullptr};
   launch_logp(logits, targets, Inside{nullptr, 0}, out, S, T, V, ss, st, dtype,
               static_cast<cudaStream_t>(stream));
@@ -804,7 +813,10 @@ extern "C" int sqb_logp_bwd(const void* logits, const int64_t* targets, const fl
                             int64_t dst, int dtype, void* stream) {
   if (!logits || !targets || !stats || !g_row || !dlogits || !dims_ok(S, T, V))
     return SQB_ERR_ARG;
-  if (!elt_of(dtype)) return SQB_ERR_DTYPE;
+  const int elt = elt_of(dtype);
+  if (!elt) return SQB_ERR_DTYPE;
+  if (!aligned(elt, logits, dlogits) || !aligned(8, targets, stats) || !aligned(4, g_row, scale))
+    return SQB_ERR_ALIGN;
   dispatch<kWriteThreads>(dtype, S * T, V, [&](auto type, auto threads, unsigned grid) {
     using X = decltype(type);
     constexpr int kThreads = decltype(threads)::value;
@@ -831,10 +843,14 @@ extern "C" int sqb_preference_fwd(const void* logits, const int64_t* targets,
   if (T > 0 && (!logits || !targets || !stats || !g_row || !dims_ok(S, T, V)))
     return SQB_ERR_ARG;
   if (cu_seqlens ? S != 1 : S != 2 * P) return SQB_ERR_ARG;
-  if (!elt_of(dtype)) return SQB_ERR_DTYPE;
+  const int elt = elt_of(dtype);
+  if (!elt) return SQB_ERR_DTYPE;
   const int64_t N = S * T;
   if (!workspace || ws_bytes < sqb_preference_workspace_bytes(N, P)) return SQB_ERR_WORKSPACE;
-  if (reinterpret_cast<uintptr_t>(workspace) % sizeof(double)) return SQB_ERR_ALIGN;
+  if (!aligned(elt, logits) || !aligned(8, targets, cu_seqlens, stats) ||
+      !aligned(4, ref_logps, loss, rewards, g_row) ||
+      !aligned(8, workspace))
+    return SQB_ERR_ALIGN;
   cudaStream_t q = static_cast<cudaStream_t>(stream);
   double* logp = static_cast<double*>(workspace);
   double* pair_loss = logp + align256((size_t)N * sizeof(double)) / sizeof(double);
@@ -871,10 +887,14 @@ extern "C" int sqb_policy_fwd(const void* logits, const int64_t* targets,
   if (!logits || !targets || !adv || !loss || !statistics || !logp || !dims_ok(S, T, V) ||
       seqs <= 0 || seqs > INT32_MAX || (cu_seqlens ? S != 1 : S != seqs))
     return SQB_ERR_ARG;
-  if (!elt_of(dtype)) return SQB_ERR_DTYPE;
+  const int elt = elt_of(dtype);
+  if (!elt) return SQB_ERR_DTYPE;
   const int64_t N = S * T;
   if (!workspace || ws_bytes < sqb_policy_workspace_bytes(N, seqs)) return SQB_ERR_WORKSPACE;
-  if (reinterpret_cast<uintptr_t>(workspace) % sizeof(double)) return SQB_ERR_ALIGN;
+  if (!aligned(elt, logits, dlogits) || !aligned(8, targets, cu_seqlens, stats) ||
+      !aligned(4, old_logp, ref_logp, adv, loss, statistics, logp, g_row) ||
+      !aligned(8, workspace))
+    return SQB_ERR_ALIGN;
   cudaStream_t q = static_cast<cudaStream_t>(stream);
   double* terms = static_cast<double*>(workspace);
   float* weight = reinterpret_cast<float*>(static_cast<char*>(workspace) +

@@ -745,6 +745,7 @@ bool aligned(const void* p, int bytes) {
 }
 
 bool known(int dtype) { return dtype == SQB_BF16 || dtype == SQB_F32; }
+int elt_of(int dtype) { return dtype == SQB_BF16 ? 2 : 4; }
 
 // How N rows of C columns are dealt out: groups of G warps whose lanes hold E columns (8, or 4
 // where one warp then has the row), as many CTAs of one group (or of eight groups of one warp)
@@ -776,7 +777,10 @@ int check(const Args& a, int64_t N, int64_t C, int x_dtype, int h_dtype, int y_d
   if (a.gate && (gates <= 0 || N % gates != 0)) return SQB_ERR_ARG;
   if (!known(x_dtype) || !known(h_dtype) || !known(y_dtype)) return SQB_ERR_DTYPE;
   if (C <= 0 || C > kMaxC) return SQB_ERR_UNSUPPORTED;
-  return SQB_OK;
+  const float* const parameters[] = {a.w, a.b, a.wp, a.bp, a.gate};
+  for (const float* p : parameters)
+    if (!aligned(p, 4)) return SQB_ERR_ALIGN;
+  return aligned(a.x, elt_of(x_dtype)) && aligned(a.h, elt_of(h_dtype)) ? SQB_OK : SQB_ERR_ALIGN;
 }
 
 // Whether every row can be read four elements at a time.
@@ -839,7 +843,8 @@ extern "C" int sqb_residual_norm_fwd(const void* x, int x_dtype, const void* h, 
                            rms, N, C);
   if (const int rc = check(a, N, C, x_dtype, h_dtype, y_dtype, gates)) return rc;
   if (!x_out || !y || !stats) return SQB_ERR_ARG;
-  if (!aligned(stats, 16)) return SQB_ERR_ALIGN;
+  if (!aligned(stats, 16) || !aligned(x_out, elt_of(x_dtype)) || !aligned(y, elt_of(y_dtype)))
+    return SQB_ERR_ALIGN;
   cudaStream_t q = static_cast<cudaStream_t>(stream);
   const void* more[] = {x_out, y};
   const bool w4 = wide(a, more, 2), biased = bias || post_bias;
@@ -906,7 +911,13 @@ extern "C" int sqb_residual_norm_bwd(const void* dy, int y_dtype, const void* dx
   if (gate && gates > 65535 - kParts) return SQB_ERR_UNSUPPORTED;
   if (!workspace || ws_bytes < sqb_residual_norm_workspace_bytes(N, C, gate ? gates : 0))
     return SQB_ERR_WORKSPACE;
-  if (!aligned(stats, 16) || !aligned(workspace, 16)) return SQB_ERR_ALIGN;
+  if (!aligned(stats, 16) || !aligned(workspace, 16) || !aligned(dy, elt_of(y_dtype)) ||
+      !aligned(dx_out, elt_of(x_dtype)) || !aligned(dx, elt_of(x_dtype)) ||
+      !aligned(dh, elt_of(h_dtype)))
+    return SQB_ERR_ALIGN;
+  const float* const gradients[] = {dweight, dbias, dpost_weight, dpost_bias, dgate};
+  for (const float* p : gradients)
+    if (!aligned(p, 4)) return SQB_ERR_ALIGN;
   cudaStream_t q = static_cast<cudaStream_t>(stream);
   const void* more[] = {dy, dx_out, dx, dh};
   const bool w4 = wide(a, more, 4), biased = bias || post_bias;
