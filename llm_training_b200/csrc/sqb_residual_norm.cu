@@ -933,9 +933,12 @@ extern "C" int sqb_residual_norm_bwd(const void* dy, int y_dtype, const void* dx
     using Y = decltype(ty);
     auto run = [&](auto kernel) {
       const int warps = p.G * p.groups;
-      const int smem = warps * 2 * (p.E == 8 ? bwd_slot<X, H, Y, 8>() : bwd_slot<X, H, Y, 4>());
-      ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ==
-           cudaSuccess;
+      const int warp = 2 * (p.E == 8 ? bwd_slot<X, H, Y, 8>() : bwd_slot<X, H, Y, 4>());
+      const int smem = warps * warp;
+      // the limit belongs to the kernel, whatever thread launches it: always the most that any
+      // width takes
+      ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kMaxWarps * warp) == cudaSuccess;
       if (!ok) return;
       kernel<<<p.ctas, 32 * warps, smem, q>>>(
           a, more_args, static_cast<const Y*>(dy), static_cast<const X*>(dx_out),
