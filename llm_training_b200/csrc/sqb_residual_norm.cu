@@ -755,8 +755,6 @@ struct Plan {
   uint32_t rows;
 };
 
-constexpr int kMaxCtas = 148 * 8;
-
 Plan plan_of(int64_t N, int64_t C, int warps) {
   Plan p;
   p.E = C <= 128 ? 4 : 8;
@@ -886,10 +884,10 @@ extern "C" int sqb_residual_norm_fwd(const void* x, int x_dtype, const void* h, 
 }
 
 extern "C" size_t sqb_residual_norm_workspace_bytes(int64_t N, int64_t C, int64_t gates) {
-  if (N <= 0 || C <= 0 || gates < 0) return 0;
-  // partial rows of the CTAs, and of at most 16 runs on each SM
-  const int64_t ctas = N < kMaxCtas ? N : kMaxCtas, runs = N < 148 * 16 ? N : 148 * 16;
-  return (size_t)(kParts * ctas + (gates > 1 ? runs + gates : 0)) * (size_t)((C + 3) / 4 * 4) *
+  if (N <= 0 || N > INT32_MAX || C <= 0 || C > kMaxC || gates < 0) return 0;
+  // partial rows of the CTAs, and one for each run and gate that meet
+  const Plan p = plan_of(N, C, kBwdWarps);
+  return ((size_t)kParts * p.ctas + (gates > 1 ? (size_t)p.runs + gates : 0)) * p.pitch *
          sizeof(float);
 }
 

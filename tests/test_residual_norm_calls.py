@@ -66,3 +66,23 @@ def test_two_threads_with_rows_of_different_widths():
     assert set(codes[0]) == set(codes[1]) == {0}
     for job in jobs:
         assert all(torch.equal(a, b) for a, b in zip(job.out, job.expected()))
+
+
+@pytest.mark.parametrize("gates", [0, 1, 8])
+@pytest.mark.parametrize("C", [1, 32, 100, 128, 129, 768, 1999, 4095, 4096])
+@pytest.mark.parametrize("N", [1, 7, 1184, 16384, 2**31 - 8])
+def test_scratch_is_what_the_rows_need(N, C, gates):
+    """A partial row of each of five parameters for every CTA - at most 16 warps of them on each
+    of 148 SMs, a warp holding 256 columns of a row - and one row for each run and gate that meet."""
+    warps = -(-C // 256)
+    ctas = min(N, 148 * (16 // warps))
+    runs = min(N, 148 * 16)
+    pitch = -(-C // 4) * 4
+    most = (5 * ctas + (runs + gates if gates > 1 else 0)) * pitch * 4
+    nbytes = _lib.lib().sqb_residual_norm_workspace_bytes(N, C, gates)
+    assert 0 < nbytes <= most and nbytes % 16 == 0
+
+
+def test_no_scratch_for_what_is_refused():
+    nbytes = _lib.lib().sqb_residual_norm_workspace_bytes
+    assert nbytes(0, 8, 0) == nbytes(8, 0, 0) == nbytes(8, 8, -1) == nbytes(8, 4097, 0) == 0
