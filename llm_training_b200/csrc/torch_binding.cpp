@@ -22,6 +22,7 @@
 #include <optional>
 #include <string>
 #include <tuple>
+#include <utility>
 #include <vector>
 
 #include "sqb_train.h"
@@ -401,7 +402,7 @@ struct Tensors {
   std::vector<int32_t> dtype;
 
   // Whether they are: plain float32 or bfloat16 tensors on `device`, without gaps (contiguous:
-  // in order, too), no two of them the same memory (`distinct`).
+  // in order, too), no two of them in the same memory (`distinct`).
   bool take(const std::vector<Tensor>& tensors, c10::Device device, bool contiguous,
             bool distinct) {
     const size_t n = tensors.size();
@@ -416,19 +417,26 @@ struct Tensors {
       numel.push_back(t.numel());
       dtype.push_back(dtype_of(t));
     }
-    return !distinct || none_shared();
+    return !distinct || apart();
   }
-  std::vector<void*> held() const {  // in order
-    std::vector<void*> h;
-    h.reserve(at.size());
+  uintptr_t begin(size_t i) const { return reinterpret_cast<uintptr_t>(at[i]); }
+  uintptr_t end(size_t i) const { return begin(i) + numel[i] * (dtype[i] == SQB_F32 ? 4 : 2); }
+  // The first and the last + 1 bytes of those that have any, each in order.
+  std::pair<std::vector<uintptr_t>, std::vector<uintptr_t>> ends() const {
+    std::vector<uintptr_t> lo, hi;
+    lo.reserve(at.size()), hi.reserve(at.size());
     for (size_t i = 0; i < at.size(); ++i)
-      if (numel[i]) h.push_back(at[i]);
-    std::sort(h.begin(), h.end());
-    return h;
+      if (numel[i]) lo.push_back(begin(i)), hi.push_back(end(i));
+    std::sort(lo.begin(), lo.end());
+    std::sort(hi.begin(), hi.end());
+    return {std::move(lo), std::move(hi)};
   }
-  bool none_shared() const {
-    const auto h = held();
-    return std::adjacent_find(h.begin(), h.end()) == h.end();
+  // Spans are apart if and only if no k-th end is past the (k + 1)-th beginning.
+  bool apart() const {
+    const auto [lo, hi] = ends();
+    for (size_t k = 1; k < lo.size(); ++k)
+      if (lo[k] < hi[k - 1]) return false;
+    return true;
   }
 };
 
@@ -468,12 +476,15 @@ std::optional<std::tuple<std::vector<Tensor>, Tensor>> clip(
     if (given) {
       out = *given;
       if (out.size() != grads.size() || !to.take(out, device, true, true)) return std::nullopt;
-      const auto held = in.held();
-      for (size_t i = 0; i < out.size(); ++i)  // each on its own gradient's memory, or on none's
-        if (out[i].sizes() != grads[i].sizes() ||
-            ((to.at[i] != in.at[i] || to.dtype[i] != in.dtype[i]) && to.numel[i] &&
-             std::binary_search(held.begin(), held.end(), to.at[i])))
-          return std::nullopt;
+      const auto [lo, hi] = in.ends();
+      for (size_t i = 0; i < out.size(); ++i) {  // each its own gradient alone, or in none's memory
+        if (out[i].sizes() != grads[i].sizes()) return std::nullopt;
+        if (to.numel[i] == 0) continue;
+        const auto met = (std::lower_bound(lo.begin(), lo.end(), to.end(i)) - lo.begin()) -
+                         (std::upper_bound(hi.begin(), hi.end(), to.begin(i)) - hi.begin());
+        const bool own = to.at[i] == in.at[i] && to.dtype[i] == in.dtype[i];
+        if (met != (own ? 1 : 0)) return std::nullopt;
+      }
     } else {
       out.reserve(grads.size());
       for (const Tensor& g : grads) out.push_back(at::empty_like(g));

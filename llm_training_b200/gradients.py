@@ -23,6 +23,19 @@ def _dense(t):
     return True
 
 
+def _overlap(tensors, more=()):
+    """Whether two of `tensors`, or one of them and one of `more`, have memory in common (all
+    without gaps)."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), mine)
+                   for group, mine in ((tensors, True), (more, False)) for t in group if t.numel())
+    reach = {True: 0, False: 0}  # how far the spans so far go, of either kind
+    for start, end, mine in spans:
+        if start < reach[True] or (mine and start < reach[False]):
+            return True
+        reach[mine] = max(reach[mine], end)
+    return False
+
+
 def _checked(fn, tensors, what="gradients"):
     """The device of `tensors`, all of them strided CUDA float32 or bfloat16 on it."""
     device = tensors[0].device
@@ -77,7 +90,7 @@ def clip_grads(grads, max_norm, out=None):
     computes it, written to ``out``: one tensor for each gradient, of its shape, float32
     or bfloat16 (an optimizer's fp32 buffers for bf16 gradients: the factor is applied
     before the only rounding), sharing no memory with any gradient unless it is the same
-    tensor.  None: new tensors like the gradients."""
+    tensor (any overlap is refused).  None: new tensors like the gradients."""
     fn = "clip_grads"
     grads, max_norm = list(grads), _bound(fn, max_norm)
     if not grads:
@@ -108,6 +121,14 @@ def _check_out(fn, grads, out, device):
     if any([o.data_ptr() == g.data_ptr() and (o.dtype != g.dtype or not g.is_contiguous())
             for g, o in zip(grads, out) if o.numel()]):
         raise ValueError(f"{fn}: out holds a gradient's memory in another layout or dtype")
+    if _overlap(out):
+        raise ValueError(f"{fn}: out holds tensors that overlap")
+    runs = [g for g in grads if g.is_contiguous()]  # others are copied first
+    ours = {o.data_ptr() for o in out}
+    placed = [g for g in runs if g.data_ptr() in ours]
+    if _overlap([o for o in out if o.data_ptr() not in {g.data_ptr() for g in placed}], runs) or (
+            _overlap(placed, [g for g in runs if g.data_ptr() not in ours])):
+        raise ValueError(f"{fn}: out overlaps a gradient that it is not")
 
 
 def clip_grad_norm_(parameters, max_norm):
@@ -115,8 +136,8 @@ def clip_grad_norm_(parameters, max_norm):
     that their global 2-norm is at most ``max_norm``, and returns the norm before, a
     float32 scalar: ``torch.nn.utils.clip_grad_norm_`` for CUDA float32 and bfloat16
     gradients on one device, with the norm of ``grad_norm``.  A parameter listed twice
-    counts once; parameters that share one gradient tensor are refused, and gradients must
-    not overlap.  Gradients below the bound are not written.  A NaN norm makes every
+    counts once; parameters that share one gradient tensor, and gradients that overlap, are
+    refused.  Gradients below the bound are not written.  A NaN norm makes every
     gradient NaN, as there.  No gradients: 0."""
     fn = "clip_grad_norm_"
     if isinstance(parameters, torch.Tensor):
@@ -138,6 +159,8 @@ def clip_grad_norm_(parameters, max_norm):
         if any(s == 0 and n > 1 for n, s in zip(g.shape, g.stride())):
             raise ValueError(f"{fn}: a gradient expanded over its own memory cannot be scaled "
                              "in place")
+    if _overlap([g for g in grads if g.is_contiguous() or _dense(g)]):
+        raise ValueError(f"{fn}: two gradients overlap")
     work = [g if g.is_contiguous() or _dense(g) else g.contiguous() for g in grads]
     _, norm = _done(fn, _lib.binding().clip(work, None, max_norm, True))
     with torch.no_grad():
