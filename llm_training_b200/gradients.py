@@ -8,7 +8,7 @@ import torch
 
 from . import _lib
 
-__all__ = ["grad_norm", "clip_grads", "clip_grad_norm_"]
+__all__ = ["grad_norm", "clip_grads", "clip_grad_norm_", "clip_grad_norm_supported"]
 
 _DTYPES = {torch.float32, torch.bfloat16}
 
@@ -129,6 +129,17 @@ def _check_out(fn, grads, out, device):
     if _overlap([o for o in out if o.data_ptr() not in {g.data_ptr() for g in placed}], runs) or (
             _overlap(placed, [g for g in runs if g.data_ptr() not in ours])):
         raise ValueError(f"{fn}: out overlaps a gradient that it is not")
+
+
+def clip_grad_norm_supported(parameters) -> bool:
+    """Whether ``clip_grad_norm_`` takes the gradients of ``parameters`` (an iterable of tensors,
+    or one): ordinary strided CUDA float32 and bfloat16 tensors on one device, one at least."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    return (bool(grads) and grads[0].is_cuda and {type(g) for g in grads} == {torch.Tensor}
+            and {g.dtype for g in grads} <= _DTYPES and {g.layout for g in grads} == {torch.strided}
+            and len({g.device for g in grads}) == 1)
 
 
 def clip_grad_norm_(parameters, max_norm):

@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .gradients import clip_grad_norm_, clip_grads, grad_norm
+from .gradients import clip_grad_norm_, clip_grad_norm_supported, clip_grads, grad_norm
 from .losses import policy_loss, policy_loss_and_grad, preference_loss, token_log_probs
 from .residual import residual_norm
 
@@ -26,7 +26,8 @@ __all__ = ["sqrt_block_attention", "sqrt_block_forward", "sqrt_block_backward", 
            "block_geometry", "reference_attention", "reference_forward", "reference_backward",
            "cross_entropy", "layer_norm", "layer_norm_supported",
            "token_log_probs", "preference_loss", "policy_loss", "policy_loss_and_grad",
-           "grad_norm", "clip_grads", "clip_grad_norm_", "residual_norm"]
+           "grad_norm", "clip_grads", "clip_grad_norm_", "clip_grad_norm_supported",
+           "residual_norm"]
 
 _DTYPES = {torch.float32: _lib.SQB_F32, torch.bfloat16: _lib.SQB_BF16}
 

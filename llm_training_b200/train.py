@@ -20,7 +20,7 @@ import torch
 import torch.nn.functional as F
 
 from .model.gpt import GPT
-from .ops import check_status, clip_grad_norm_, cross_entropy
+from .ops import check_status, clip_grad_norm_, clip_grad_norm_supported, cross_entropy
 
 
 def calculate_loss(logits, targets):
@@ -98,9 +98,11 @@ class Trainer:
         with span("backward"):
             loss.backward()
         with span("optimizer"):
-            clip = (clip_grad_norm_ if self.device.type == "cuda"
+            # (a plugin's parameters may be of other types than the library's clipping takes)
+            params = list(self.model.parameters())
+            clip = (clip_grad_norm_ if clip_grad_norm_supported(params)
                     else torch.nn.utils.clip_grad_norm_)
-            norm = clip(self.model.parameters(), 1.0)
+            norm = clip(params, 1.0)
             self.optimizer.step()
         return loss.detach(), norm
 
