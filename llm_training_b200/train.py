@@ -113,6 +113,9 @@ class Trainer:
         n = sum(p.numel() for p in raw.parameters())
         emb = raw.transformer.wpe.weight.numel()
         dev = self.device
+        # what the reference's models do not have, where this one has it
+        off = {"post_norm": False, "layer_scale": None}
+        extras = {k: getattr(config, k) for k, v in off.items() if getattr(config, k, v) is not v}
         return {
             "device": dev.type,
             "gpu_name": torch.cuda.get_device_name(dev) if dev.type == "cuda" else None,
@@ -121,9 +124,9 @@ class Trainer:
             "torch_compile": compiled, "attention_profiling": True,
             "attention": config.attention, "seed": seed, "num_parameters": n,
             "num_parameters_non_embedding": n - emb,
-            "model_config": {k: getattr(config, k) for k in (
+            "model_config": {**{k: getattr(config, k) for k in (
                 "block_size", "vocab_size", "n_layer", "n_head", "n_embd", "dropout", "bias",
-                "attention")},
+                "attention")}, **extras},
             "batch_size": batch, "seq_len": seq, "grad_accumulation_steps": 1,
             "max_steps": max_steps, "max_lr": lr, "min_lr": lr, "warmup_steps": 0,
             "eval_interval": 0, "eval_iters": 0, "data_dir": "synthetic (uniform token ids)",
