@@ -6,19 +6,22 @@ Produces ``llm_training_b200/lib/libsqrtblock.so`` from ``csrc/*.cu``.  The
 library exports the C ABI of ``include/sqrtblock.h`` and links the CUDA
 runtime statically, so it depends only on the driver at run time.  And
 ``lib/sqb_torch.so`` from ``csrc/torch_binding.cpp`` (g++, PyTorch's headers): the
-eager PyTorch binding of the post-training operators.
+eager PyTorch binding of the post-training operators, left out (with a warning) where
+PyTorch or the compiler is not there.
 """
 
 from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.metadata
 import importlib.util
 import os
 import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG)
@@ -59,12 +62,20 @@ def _headers():
     return hs
 
 
-def _binding_command(out: str):
-    """g++ command of the PyTorch binding."""
+def _torch():
+    """(folder, version) of the installed PyTorch, which is not imported; None without one."""
     spec = importlib.util.find_spec("torch")
     if spec is None:
-        raise RuntimeError("PyTorch not found: its binding cannot be built")
-    torch_dir = spec.submodule_search_locations[0]
+        return None
+    folder = spec.submodule_search_locations[0]
+    try:
+        return folder, importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        return folder, "of unknown version"
+
+
+def _binding_command(torch_dir: str, out: str):
+    """g++ command of the PyTorch binding."""
     cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc_path()))), "include")
     headers = [os.path.join(torch_dir, "include"),
                os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"), cuda,
@@ -85,8 +96,8 @@ def _stale(target: str, deps) -> bool:
 
 
 def build(force: bool = False, debug: bool = False, verbose: bool = False) -> str:
-    """Compile every .cu for sm_100a, link the shared library and build the PyTorch binding;
-    returns the library's path."""
+    """Compile every .cu for sm_100a, link the shared library and, where PyTorch is, build its
+    binding; returns the library's path."""
     nvcc = nvcc_path()
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
@@ -101,11 +112,14 @@ def build(force: bool = False, debug: bool = False, verbose: bool = False) -> st
         if force or _stale(obj, [s] + hdrs + [__file__]):
             jobs.append([nvcc, *flags, "-c", s, "-o", obj])
 
+    # the binding belongs to a PyTorch and a Python
+    torch = _torch()
+    made_for = f"{torch} {sysconfig.get_config_var('SOABI')}"
+    stamp = os.path.join(BUILD, BINDING + ".stamp")
     binding_src = os.path.join(CSRC, "torch_binding.cpp")
     binding_tmp = BINDINGPATH + ".tmp"
-    new_binding = force or _stale(BINDINGPATH, [binding_src] + hdrs + [__file__])
-    if new_binding:
-        jobs.insert(0, _binding_command(binding_tmp))
+    new_binding = (force or torch is None or _stale(BINDINGPATH, [binding_src] + hdrs + [__file__])
+                   or not os.path.exists(stamp) or open(stamp).read() != made_for)
 
     def run(cmd):
         if verbose:
@@ -115,16 +129,38 @@ def build(force: bool = False, debug: bool = False, verbose: bool = False) -> st
             raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({' '.join(cmd)}):\n{r.stdout}\n{r.stderr}")
         return r.stdout + r.stderr
 
-    with cf.ThreadPoolExecutor(max_workers=max(1, min(len(jobs), os.cpu_count() or 1))) as ex:
+    with cf.ThreadPoolExecutor(max_workers=max(1, min(len(jobs) + 1, os.cpu_count() or 1))) as ex:
+        binding = None
+        if new_binding:
+            # whatever comes of it, an older one does not stay beside a newer library
+            for old in (BINDINGPATH, stamp):
+                if os.path.exists(old):
+                    os.remove(old)
+            if torch is not None:
+                binding = ex.submit(run, _binding_command(torch[0], binding_tmp))
         for out in ex.map(run, jobs):
             if verbose and out.strip():
                 print(out, flush=True)
-    if new_binding:
-        os.replace(binding_tmp, BINDINGPATH)
     if force or _stale(LIBPATH, objs):
         tmp = LIBPATH + ".tmp"
         run([nvcc, *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-o", tmp, *objs])
         os.replace(tmp, LIBPATH)
+    # the library is there; now the binding's outcome
+    why = "PyTorch not found" if torch is None else None
+    if binding is not None:
+        try:
+            out = binding.result()
+        except FileNotFoundError as e:
+            why = f"no C++ compiler ({e})"
+        else:
+            if verbose and out.strip():
+                print(out, flush=True)
+            os.replace(binding_tmp, BINDINGPATH)
+            with open(stamp, "w") as f:
+                f.write(made_for)
+    if why:
+        warnings.warn(f"{why}: {BINDINGPATH} is not built, which eager calls of the post-training "
+                      "operators need", RuntimeWarning, stacklevel=2)
     return LIBPATH
 
 
