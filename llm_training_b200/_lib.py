@@ -140,13 +140,30 @@ def binding():
     return _binding
 
 
-def plain(x) -> bool:
-    """Whether `x` is an ordinary tensor in an ordinary eager call.  The post-training ops
-    then run without the dispatcher, whose custom-op layers cost 100 us a call; a traced,
-    fake or otherwise intercepted call goes through the registered custom op."""
-    return (type(x) in (torch.Tensor, torch.nn.Parameter) and not torch.compiler.is_compiling()
-            and torch._C._len_torch_dispatch_stack() == 0
-            and not torch._C._are_functorch_transforms_active())
+_ORDINARY = (torch.Tensor, torch.nn.Parameter, type(None))
+
+
+def eager() -> bool:
+    """Whether an op is run where it is called: by no tracer (torch.compile's or torch.jit's),
+    dispatch mode or torch.func transform, none of which would see a launch of the binding."""
+    if torch.compiler.is_compiling():
+        return False
+    if torch._C._are_functorch_transforms_active():
+        # the dispatcher takes an op without a forward-mode derivative for a constant
+        jvp = torch._C._functorch.TransformType.Jvp
+        if any(level.key() == jvp for level in torch._C._functorch.get_interpreter_stack()):
+            raise NotImplementedError("the post-training operators have no forward-mode "
+                                      "derivative")
+        return False
+    return torch._C._len_torch_dispatch_stack() == 0 and torch._C._get_tracing_state() is None
+
+
+def plain(*tensors) -> bool:
+    """Whether `tensors` (None where one is not given) are ordinary tensors in an eager call.
+    The post-training ops then run without the dispatcher, whose custom-op layers cost 100 us
+    a call; a traced, fake or otherwise intercepted call goes through the registered custom
+    op."""
+    return all([type(x) in _ORDINARY for x in tensors]) and eager()
 
 
 def library_path() -> str:

@@ -238,7 +238,7 @@ def token_log_probs(logits, targets):
     (``sqrtblock::logp_fwd/bwd``): one read of the logits forward, and one read and one
     write backward, with no softmax kept in between."""
     x, t = _rows("token_log_probs", logits, targets)
-    return _lib.binding().logp(x, t) if _lib.plain(x) else _logp_fwd(x, t)[0]
+    return _lib.binding().logp(x, t) if _lib.plain(x, t) else _logp_fwd(x, t)[0]
 
 
 def preference_loss(logits, targets, ref_logps=None, *, beta=0.1, label_smoothing=0.0,
@@ -263,7 +263,7 @@ def preference_loss(logits, targets, ref_logps=None, *, beta=0.1, label_smoothin
     beta = _number(fn, "beta", beta, most=1e30)
     label_smoothing = _number(fn, "label_smoothing", label_smoothing, most=1.0)
     args = (x, t, ref, cu, seqs // 2, beta, label_smoothing)
-    if _lib.plain(x):
+    if _lib.plain(*args[:4]):
         return _lib.binding().preference(*args)
     loss, rewards, _ = _preference_fwd(*args)
     return (loss, *rewards.unbind(0))
@@ -317,7 +317,7 @@ def policy_loss(logits, targets, advantages, old_logps=None, ref_logps=None, *, 
     loss - are for logging and for the next step's ``old_logps``, not differentiable."""
     args = _policy_args("policy_loss", logits, targets, advantages, old_logps, ref_logps, clip,
                         clip_high, kl_coef, reduction, cu_seqlens)
-    if _lib.plain(args[0]):
+    if _lib.plain(*args[:6]):
         return _lib.binding().policy(*args)
     return _policy_fwd(*args, None)[:3]
 
@@ -336,6 +336,6 @@ def policy_loss_and_grad(logits, targets, advantages, old_logps=None, ref_logps=
     args = _policy_args(fn, logits.detach(), targets, advantages, old_logps, ref_logps, clip,
                         clip_high, kl_coef, reduction, cu_seqlens)
     grad_scale = _number(fn, "grad_scale", grad_scale, least=-1e30, most=1e30)
-    run = _lib.binding().policy_fwd if _lib.plain(args[0]) else _policy_fwd
+    run = _lib.binding().policy_fwd if _lib.plain(*args[:6]) else _policy_fwd
     loss, logps, stats, grad = run(*args, grad_scale)
     return loss, grad, logps, stats

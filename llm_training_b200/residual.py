@@ -153,6 +153,6 @@ def residual_norm(x, h, weight, bias=None, *, post_weight=None, post_bias=None, 
     bp = _param("post_bias", post_bias, C, device)
     args = (x.contiguous(), h.contiguous(), w, b, wp, bp, _gates(gate, x, C, device), scale, eps,
             kind == "rms")
-    if _lib.plain(args[0]):
+    if _lib.plain(*args[:7]):
         return _lib.binding().residual(*args, out_dtype == torch.bfloat16)
     return _fwd(*args, out_dtype)[:2]

@@ -1,0 +1,121 @@
+"""The post-training operators in calls that something else records or transforms: torch.jit's
+tracer, torch.compile, fake tensors, torch.func.  Such a call must reach the registered ops - a
+launch of the C++ binding leaves no trace."""
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from llm_training_b200 import _lib, ops
+
+
+class Wrapped(torch.Tensor):
+    """A tensor that something intercepts."""
+
+
+def test_what_runs_where_it_is_called():
+    x, t = torch.zeros(2, 3), torch.zeros(2, dtype=torch.int64)
+    assert _lib.plain(x, t) and _lib.plain(torch.nn.Parameter(x), None, t)
+    assert not _lib.plain(x.as_subclass(Wrapped)) and not _lib.plain(x, t.as_subclass(Wrapped))
+    seen = []
+
+    def f(x):
+        seen.append((torch.jit.is_tracing(), _lib.plain(x)))
+        return x + 1
+
+    torch.jit.trace(f, x)
+    assert (True, False) in seen and (True, True) not in seen
+    with FakeTensorMode():
+        assert not _lib.eager()
+    torch.func.grad(lambda x: (seen.append(_lib.plain(x)), x.sum())[1])(x)
+    assert seen[-1] is False and _lib.eager()
+
+
+# ---- GPU: the operators as functions of one tensor ---------------------------------------
+
+
+def cases():
+    g = torch.Generator().manual_seed(0)
+    t = torch.randint(-1, 33, (4, 6), generator=g).cuda()
+    ref = (-10 * torch.rand(4, generator=g)).cuda()
+    old = (-3.5 * torch.rand(4, 6, generator=g)).cuda()
+    adv = torch.randn(4, generator=g).cuda()
+    w, h = torch.rand(33, generator=g).cuda(), torch.randn(4, 6, 33, generator=g).cuda()
+
+    return {
+        "token_log_probs": lambda x: ops.token_log_probs(x, t).sum(),
+        "preference_loss": lambda x: ops.preference_loss(x, t, ref)[0],
+        "policy_loss": lambda x: ops.policy_loss(x, t, adv, old, old, kl_coef=0.1)[0],
+        "policy_loss_and_grad": lambda x: (h * ops.policy_loss_and_grad(x, t, adv, old)[1]).sum(),
+        "residual_norm": lambda x: sum(v.square().sum() for v in ops.residual_norm(
+            x, h, w, post_weight=w, gate=w, kind="rms")),
+    }
+
+
+DIFFERENTIABLE = ["token_log_probs", "preference_loss", "policy_loss", "residual_norm"]
+KINDS = [*DIFFERENTIABLE, "policy_loss_and_grad"]
+
+
+def inputs():
+    g = torch.Generator().manual_seed(1)
+    return [torch.randn(4, 6, 33, generator=g).cuda().requires_grad_(True) for _ in range(2)]
+
+
+def value_and_grad(f, x, kind):
+    v = f(x)
+    return (v.detach(), *(torch.autograd.grad(v, x) if kind in DIFFERENTIABLE else ()))
+
+
+def same(got, want):
+    assert len(got) == len(want)
+    for a, b in zip(got, want):
+        # the same kernels; what stands around them may add up in another order
+        torch.testing.assert_close(a, b, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_jit_trace_replays_on_new_inputs(kind):
+    f, (x, y) = cases()[kind], inputs()
+    traced = torch.jit.trace(f, x)
+    assert any("sqrtblock::" in n.kind() for n in traced.inlined_graph.nodes())
+    for v in (y, x):
+        same(value_and_grad(traced, v, kind), value_and_grad(f, v, kind))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("backend", ["aot_eager", "inductor"])
+@pytest.mark.parametrize("kind", KINDS)
+def test_compiles_without_a_break(kind, backend):
+    f, (x, y) = cases()[kind], inputs()
+    torch._dynamo.reset()
+    compiled = torch.compile(f, backend=backend, fullgraph=True)
+    for v in (x, y, x):
+        same(value_and_grad(compiled, v, kind), value_and_grad(f, v, kind))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", DIFFERENTIABLE)
+def test_transforms_are_refused(kind):
+    """Reverse and forward mode by torch.func, forward mode by dual tensors: an error, not a
+    derivative of zero."""
+    f, (x, y) = cases()[kind], inputs()
+    with pytest.raises(RuntimeError):
+        torch.func.grad(f)(x.detach())
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(f, (x.detach(),), (y.detach(),))
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda v: torch.func.vmap(f)(v[None]), (x.detach(),), (y.detach(),))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x.detach(), y.detach())
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            f(dual)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", DIFFERENTIABLE)
+def test_vmap_calls_once_for_each(kind):
+    f, (x, y) = cases()[kind], inputs()
+    got = torch.func.vmap(f)(torch.stack([x.detach(), y.detach()]))
+    same(got, [f(v).detach() for v in (x, y)])
