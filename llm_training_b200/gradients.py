@@ -62,6 +62,52 @@ def _done(fn, result):
     return result
 
 
+# ---- the operators, on tensors that fill one run of memory each.  An eager call goes to the
+# C++ binding; these are the same launches registered as custom ops, for traced calls.
+
+
+@torch.library.custom_op("sqrtblock::grad_norm", mutates_args=())
+def _grad_norm(tensors: list[torch.Tensor]) -> torch.Tensor:
+    return _done("grad_norm", _lib.binding().grad_norm(tensors))
+
+
+@torch.library.custom_op("sqrtblock::clip_grads", mutates_args=())
+def _clip_grads(grads: list[torch.Tensor], bf16: list[int], max_norm: float
+                ) -> list[torch.Tensor]:
+    """The clipped gradients, contiguous, bfloat16 where `bf16` is 1 and else float32; last
+    the norm.  (It writes to none of its inputs: torch.jit loses track of lists that an op
+    writes to.)"""
+    out = [torch.empty(g.shape, dtype=torch.bfloat16 if b else torch.float32, device=g.device)
+           for g, b in zip(grads, bf16)]
+    grads = [g.contiguous() for g in grads]
+    return [*out, _done("clip_grads", _lib.binding().clip(grads, out, max_norm, False))[1]]
+
+
+@_grad_norm.register_fake
+def _(tensors):
+    return tensors[0].new_empty((), dtype=torch.float32)
+
+
+@_clip_grads.register_fake
+def _(grads, bf16, max_norm):
+    out = [g.new_empty(g.shape, dtype=torch.bfloat16 if b else torch.float32)
+           for g, b in zip(grads, bf16)]
+    return [*out, grads[0].new_empty((), dtype=torch.float32)]
+
+
+def _clip_traced(grads, out, max_norm):
+    """(out, norm) of a traced call; out is written by ordinary copies."""
+    *clipped, norm = _clip_grads(grads, [int(o.dtype == torch.bfloat16) for o in out], max_norm)
+    with torch.no_grad():
+        for o, c in zip(out, clipped):
+            o.copy_(c)
+    return out, norm
+
+
+def _in_one_run(t):
+    return t if t.is_contiguous() or _dense(t) else t.contiguous()
+
+
 def grad_norm(tensors):
     """2-norm of all elements of ``tensors`` (CUDA float32 or bfloat16, any mixture, one
     device) as a float32 scalar on their device.  The squares are summed in 64 bits in a
@@ -69,11 +115,12 @@ def grad_norm(tensors):
     fn, tensors = "grad_norm", list(tensors)
     if not tensors:
         return torch.tensor(0.0)
-    norm = _lib.binding().grad_norm(tensors) if tensors[0].is_cuda else None
+    eager = _lib.eager()
+    norm = _lib.binding().grad_norm(tensors) if eager and tensors[0].is_cuda else None
     if norm is None:
         _checked(fn, tensors, "tensors")
-        norm = _done(fn, _lib.binding().grad_norm(
-            [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in tensors]))
+        tensors = [_in_one_run(t) for t in tensors]
+        norm = (_done(fn, _lib.binding().grad_norm(tensors)) if eager else _grad_norm(tensors))
     return norm
 
 
@@ -95,12 +142,19 @@ def clip_grads(grads, max_norm, out=None):
     grads, max_norm = list(grads), _bound(fn, max_norm)
     if not grads:
         return [], torch.tensor(0.0)
-    out = list(out) if out is not None else None
-    done = _lib.binding().clip(grads, out, max_norm, False) if grads[0].is_cuda else None
+    out, eager = list(out) if out is not None else None, _lib.eager()
+    done = _lib.binding().clip(grads, out, max_norm, False) if eager and grads[0].is_cuda else None
     if done is None:
         device = _checked(fn, grads)
         if out is not None:
             _check_out(fn, grads, out, device)
+            if eager:
+                _check_memory(fn, grads, out)
+        if not eager and out is not None:
+            return _clip_traced(grads, out, max_norm)
+        if not eager:
+            *out, norm = _clip_grads(grads, [int(g.dtype == torch.bfloat16) for g in grads], max_norm)
+            return out, norm
         grads = [g.contiguous() for g in grads]
         done = _done(fn, _lib.binding().clip(grads, out, max_norm, False))
     return out if out is not None else done[0], done[1]
@@ -113,6 +167,9 @@ def _check_out(fn, grads, out, device):
         raise ValueError(f"{fn}: out must be on the gradients' device, {device}")
     if not all([o.is_contiguous() for o in out]):
         raise ValueError(f"{fn}: out must be contiguous")
+
+
+def _check_memory(fn, grads, out):
     at = {o.data_ptr(): i for i, o in enumerate(out) if o.numel()}
     if len(at) < sum(o.numel() > 0 for o in out):
         raise ValueError(f"{fn}: out holds one tensor twice")
@@ -158,21 +215,24 @@ def clip_grad_norm_(parameters, max_norm):
     max_norm = _bound(fn, max_norm)
     if not grads:
         return torch.tensor(0.0)
-    done = _lib.binding().clip(grads, None, max_norm, True) if grads[0].is_cuda else None
+    eager = _lib.eager()
+    done = _lib.binding().clip(grads, None, max_norm, True) if eager and grads[0].is_cuda else None
     if done is not None:
         return done[1]
     _checked(fn, grads)
+    if not eager:
+        return _clip_traced(grads, grads, max_norm)[1]
     at = [g.data_ptr() for g in grads if g.numel()]
     if len(set(at)) < len(at):
         raise ValueError(f"{fn}: two parameters share one gradient")
+    if _overlap([g for g in grads if g.is_contiguous() or _dense(g)]):
+        raise ValueError(f"{fn}: two gradients overlap")
     # a gradient with gaps (a view of a larger buffer) goes through a copy
     for g in grads:
         if any(s == 0 and n > 1 for n, s in zip(g.shape, g.stride())):
             raise ValueError(f"{fn}: a gradient expanded over its own memory cannot be scaled "
                              "in place")
-    if _overlap([g for g in grads if g.is_contiguous() or _dense(g)]):
-        raise ValueError(f"{fn}: two gradients overlap")
-    work = [g if g.is_contiguous() or _dense(g) else g.contiguous() for g in grads]
+    work = [_in_one_run(g) for g in grads]
     _, norm = _done(fn, _lib.binding().clip(work, None, max_norm, True))
     with torch.no_grad():
         for g, w in zip(grads, work):

@@ -31,6 +31,18 @@ def test_what_runs_where_it_is_called():
     assert seen[-1] is False and _lib.eager()
 
 
+def test_clipping_of_fake_gradients():
+    with FakeTensorMode():
+        g = [torch.empty(3, 5, device="cuda"), torch.empty(7, device="cuda", dtype=torch.bfloat16)]
+        assert ops.grad_norm(g).shape == () and ops.grad_norm(g).dtype == torch.float32
+        out, norm = ops.clip_grads(g, 1.0)
+        assert [o.shape for o in out] == [v.shape for v in g] and norm.shape == ()
+        assert [o.dtype for o in out] == [v.dtype for v in g]
+        p = torch.nn.Parameter(torch.empty(3, 5, device="cuda"))
+        p.grad = g[0]
+        assert ops.clip_grad_norm_([p], 1.0).device.type == "cuda"
+
+
 # ---- GPU: the operators as functions of one tensor ---------------------------------------
 
 
@@ -41,6 +53,23 @@ def cases():
     old = (-3.5 * torch.rand(4, 6, generator=g)).cuda()
     adv = torch.randn(4, generator=g).cuda()
     w, h = torch.rand(33, generator=g).cuda(), torch.randn(4, 6, 33, generator=g).cuda()
+    p = torch.nn.Parameter(torch.zeros(4, 6, 33, device="cuda"))
+    p.grad = torch.zeros_like(p)
+
+    def clip(x):
+        out, norm = ops.clip_grads([x.detach() * 2, x.detach()[0].bfloat16()], 0.5)
+        return out[0].sum() + out[1].float().sum() + norm
+
+    def clip_into(x):
+        a, b = x.detach() * 2, torch.empty(4, 6, 33, device="cuda", dtype=torch.bfloat16)
+        _, norm = ops.clip_grads([a, a[1:]], 0.5, out=[b, torch.empty_like(a[1:])])
+        ops.clip_grads([a], 0.25, out=[a])  # in place
+        return a.sum() + b.float().sum() + norm
+
+    def in_place(x):
+        with torch.no_grad():
+            p.grad.copy_(x.detach() * 2)
+        return ops.clip_grad_norm_([p], 0.5) + p.grad.sum()
 
     return {
         "token_log_probs": lambda x: ops.token_log_probs(x, t).sum(),
@@ -49,11 +78,16 @@ def cases():
         "policy_loss_and_grad": lambda x: (h * ops.policy_loss_and_grad(x, t, adv, old)[1]).sum(),
         "residual_norm": lambda x: sum(v.square().sum() for v in ops.residual_norm(
             x, h, w, post_weight=w, gate=w, kind="rms")),
+        "grad_norm": lambda x: ops.grad_norm([x.detach(), x.detach()[1:, ::2]]),
+        "clip_grads": clip,
+        "clip_grads, out": clip_into,
+        "clip_grad_norm_": in_place,
     }
 
 
 DIFFERENTIABLE = ["token_log_probs", "preference_loss", "policy_loss", "residual_norm"]
-KINDS = [*DIFFERENTIABLE, "policy_loss_and_grad"]
+KINDS = [*DIFFERENTIABLE, "policy_loss_and_grad", "grad_norm", "clip_grads", "clip_grads, out",
+         "clip_grad_norm_"]
 
 
 def inputs():
