@@ -15,16 +15,21 @@
 // bf16 logits a clock and SM at 6.56 TB/s), which is why the sum is shaped around them.
 //
 // Sum of exponentials: of 2^(x log2(e) - c), c a whole number no smaller than the largest
-// x log2(e), so that a new maximum rescales by an exact power of two.  The arguments must
-// not be rounded either: rounding them, or rescaling by an approximate exponential, costs
-// as much and leaves 1e-7 of s in every row, the same sign in all - 5e-5 of a 512-token
-// answer's log-probability, against 1e-6 this way.
-//   bf16: with H = log2(e) cut to 15 bits, x H has at most 23 bits and x H - c is exact in
+// x log2(e), so that a new maximum rescales by an exact power of two.  The product x log2(e)
+// must not be rounded either: its rounding is the same for all rows that hold the same logit,
+// and with it, or with an approximate exponential to rescale by, 1e-7 of s is left in every
+// row, the same sign in all - 5e-5 of a 512-token answer's log-probability, against 1e-6 to
+// 1e-5 this way (2e-9 to 2e-8 a row).  The difference is then rounded at most where |x log2(e)|
+// is smaller than it: by 2^-24 of a difference d whose exponential is 2^-d, 2^-25 of s at most
+// and of either sign.  What is left is ex2.approx itself: where bf16 logits are so large that
+// they take a handful of values (600, in steps of 4), what it is off at these is shared by the
+// rows: 6e-8.
+//   bf16: with H = log2(e) cut to 15 bits, x H has at most 23 bits and x H - c is formed in
 //     one fused multiply-add.  What H lacks, exp(x) = 2^(x H) exp(x d) with
 //     d = 1 - H ln 2 (5e-6), is made up for once a row: sum e (1 + (x - x0) d) from the sums
 //     of e and of e x (the next term, ((x - x0) d)^2 / 2, is below 1e-8 where e counts).
-//   fp32: h = fl(x L), h - c is exact, and the rest of x log2(e), an fma's residual and the
-//     constant's low part, is summed as e r beside e.
+//   fp32: h = fl(x L), and the rest of x log2(e), an fma's residual and the constant's low
+//     part, is summed as e r beside e.
 // Rows whose maximum is beyond 2800 are summed again by one warp, with rounded arguments.
 
 #include <cuda_bf16.h>
@@ -46,9 +51,10 @@ constexpr double kLn2 = 0.6931471805599453;
 constexpr float kH = 23637.0f / 16384.0f;
 constexpr double kLack = 1.0 - (double)kH * kLn2;
 constexpr int kBound = 4096;  // of c in the exact form
-// ex2.approx of arguments below 0 falls short by 5.06e-8 in the mean (measured on B200 over
-// 2^20 arguments a binade, the same for all of [-16, 0)), about a third of its largest error.
-// All of a row's terms share it, and all rows: it is made up for in the sum.
+// ex2.approx of arguments below 0 falls short by 5.06e-8 in the mean (measured on B200, 2^18
+// arguments a binade: 4.9e-8 to 5.1e-8 in [-16, -1), 2e-8 to 6e-8 in [-1, 0) by the last bits of
+// the arguments; 3e-8 around the mean), about a fifth of its largest error.  All of a row's
+// terms share it, and all rows: it is made up for in the sum.
 constexpr double kExp2Short = 5.06e-8;
 
 struct View {  // (S, T, V) logits, unit stride on V; strides in elements
