@@ -141,21 +141,26 @@ def binding():
 
 
 _ORDINARY = (torch.Tensor, torch.nn.Parameter, type(None))
+# (looked up once: every call of a post-training op asks)
+_compiling = torch.compiler.is_compiling
+_transformed = torch._C._are_functorch_transforms_active
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_jit_traced = torch._C._is_tracing
 
 
 def eager() -> bool:
     """Whether an op is run where it is called: by no tracer (torch.compile's or torch.jit's),
     dispatch mode or torch.func transform, none of which would see a launch of the binding."""
-    if torch.compiler.is_compiling():
+    if _compiling():
         return False
-    if torch._C._are_functorch_transforms_active():
+    if _transformed():
         # the dispatcher takes an op without a forward-mode derivative for a constant
         jvp = torch._C._functorch.TransformType.Jvp
         if any(level.key() == jvp for level in torch._C._functorch.get_interpreter_stack()):
             raise NotImplementedError("the post-training operators have no forward-mode "
                                       "derivative")
         return False
-    return torch._C._len_torch_dispatch_stack() == 0 and torch._C._get_tracing_state() is None
+    return _dispatch_modes() == 0 and not _jit_traced()
 
 
 def plain(*tensors) -> bool:

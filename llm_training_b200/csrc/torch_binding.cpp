@@ -431,8 +431,14 @@ struct Tensors {
     std::sort(hi.begin(), hi.end());
     return {std::move(lo), std::move(hi)};
   }
-  // Spans are apart if and only if no k-th end is past the (k + 1)-th beginning.
+  // Spans are apart if and only if no k-th end is past the (k + 1)-th beginning.  (Pieces of one
+  // buffer in its order need no sorting.)
   bool apart() const {
+    bool ordered = true;
+    uintptr_t reached = 0;
+    for (size_t i = 0; i < at.size() && ordered; ++i)
+      if (numel[i]) ordered = begin(i) >= reached, reached = end(i);
+    if (ordered) return true;
     const auto [lo, hi] = ends();
     for (size_t k = 1; k < lo.size(); ++k)
       if (lo[k] < hi[k - 1]) return false;
