@@ -7,7 +7,7 @@
 // the interpreter's lock from the thread that waits for it.  A short preference step, forward
 // and backward, took 260 us as a registered custom op, 140 us as a Python function.
 // Clipping walks over the gradients here for the same reason: 24 small ones took 46 us from
-// Python, 15 us so.
+// Python, 16 us so.
 //
 // Arguments are checked by the Python entry points (clipping: here, and what does not pass,
 // there).  A failed call of the library throws
