@@ -74,6 +74,7 @@ def residual_step_fused(x, h) -> bool:
     """Whether ``add_forward`` with a post norm or a gate runs as the library's kernel."""
     kinds = (torch.float32, torch.bfloat16)
     return (x.is_cuda and x.dtype in kinds and h.dtype in kinds and x.shape[-1] <= 4096
+            and h.shape == x.shape and h.device == x.device
             and LayerNorm._out_dtype() is not None)
 
 
