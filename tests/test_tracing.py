@@ -153,3 +153,26 @@ def test_vmap_calls_once_for_each(kind):
     f, (x, y) = cases()[kind], inputs()
     got = torch.func.vmap(f)(torch.stack([x.detach(), y.detach()]))
     same(got, [f(v).detach() for v in (x, y)])
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("how", ["jit.trace", "compile"])
+def test_a_model_with_a_norm_and_a_gate_behind_its_blocks(how):
+    from llm_training_b200.config import ModelConfig
+    from llm_training_b200.model.gpt import GPT
+
+    torch.manual_seed(0)
+    m = GPT(ModelConfig(block_size=64, vocab_size=97, n_layer=2, n_head=2, n_embd=128, bias=False,
+                        attention="sqrt_block", post_norm=True, layer_scale=0.5)).cuda()
+    a, b = torch.randint(0, 97, (2, 2, 64), device="cuda")
+    if how == "compile":
+        torch._dynamo.reset()
+        traced = torch.compile(m, backend="aot_eager", fullgraph=True)
+    else:
+        traced = torch.jit.trace(m, a)
+        kinds = [n.kind() for n in traced.inlined_graph.nodes()]
+        assert kinds.count("sqrtblock::residual_norm_fwd") == 4
+    for tokens in (b, a):
+        # fp32 throughout, the same kernels
+        torch.testing.assert_close(traced(tokens), m(tokens), rtol=1e-5, atol=1e-5)
